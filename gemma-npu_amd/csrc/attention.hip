@@ -43,31 +43,9 @@
 #include <type_traits>
 #include <vector>
 
-#include "w8a8_common.h"
+#include "attn_common.h"
 
 namespace w8a8 {
-
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef short v8s __attribute__((ext_vector_type(8)));
-
-// v combined over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the same row of an MFMA tile in the four
-// 16-lane groups) by the gfx950 lane swaps, in VALU instead of two ds_bpermute round trips through
-// LDS: v_permlane16_swap exchanges 16-lane groups 0 <-> 1 and 2 <-> 3, v_permlane32_swap the two
-// halves, and of the two results one holds the lane's own value and the other its partner's.  The
-// pairs are those of a xor-16 then xor-32 butterfly and both combines are commutative, so the result
-// is bit-identical to that butterfly on every lane.
-__device__ __forceinline__ float lanes4_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float lanes4_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 
 constexpr int ATTN_NW = 8;        // waves per workgroup, 16 query rows each
 constexpr int ATTN_MAX_SEG = 16;     // segments of the causal work list (= most parts of one tile)
@@ -107,15 +85,6 @@ struct AttnParams {
 };
 static_assert(sizeof(AttnParams) <= 4096, "kernel arguments");
 
-template <int N>
-__device__ __forceinline__ void attn_wait_vmcnt() {
-  __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
-}
-
-__device__ __forceinline__ void attn_dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
-}
-
 // Key `key` is visible to the query at `pos`: key <= pos, pos - key < the window (wlim = window, or
 // 2^31 for no window) and key < Tk -- one unsigned compare per bound, combined bitwise, so the mask
 // compiles to compares and selects.  A short-circuit chain (key <= pos && ... && (win == 0 || ...))
@@ -128,11 +97,6 @@ __device__ __forceinline__ bool attn_key_visible(int key, int pos, int Tk, uint3
 __device__ __forceinline__ uint32_t attn_window_limit(int window) {
   return window > 0 ? uint32_t(window) : 0x80000000u;
 }
-// s where `vis`, else -inf, as a select of the bit patterns
-__device__ __forceinline__ float attn_mask(float s, bool vis) {
-  return __uint_as_float(vis ? __float_as_uint(s) : 0xff800000u);
-}
-
 __device__ __forceinline__ int attn_xcd_remap(int b, int nblocks) {
   const int full = nblocks & ~7;
   if (b >= full) return b;
@@ -1569,7 +1533,7 @@ static int64_t attn_part_bytes(int64_t D) {
 
 // Compute units of the current device (256 on MI355X), read once; the initialisation of a
 // function-local static is thread-safe, so concurrent first calls from several host threads agree.
-static int attn_cu_count() {
+int w8a8::attn_cu_count() {
   static const int cus = [] {
     int dev = 0, n = 0;
     if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) !=

@@ -1,0 +1,634 @@
+// Attention of drafted tokens over a cache: the queries are nodes of a tree whose keys and values stand
+// behind the context's in the cache.
+//
+//   o[h, i, :] = sum_j softmax_j(scale * q[h, i] . k[g, j]) v[g, j],   g = h / (H / KV),
+//
+// over the rows j that node i sees: the context's n_past rows and, of the M nodes' rows n_past + m, its
+// own and those above it in the tree (parents[m] in -1 .. m - 1, -1: the context's last token); with a
+// window W only rows whose position is less than W before the node's, a node's position being n_past +
+// its depth.  The queries are the last N of the M nodes, so a tree can be attended to level by level.
+// A node with a parent outside -1 .. m - 1 is unused: it and the nodes below it see nothing, and their
+// outputs are zero.  The reference decodes one token at a time (local_attn.py:44-83); this is that step
+// for many candidate tokens at once.
+//
+// Work split.  The rows (node, head) of one KV head, N x G of them, are cut into tiles of 16 RT rows, and
+// the keys into parts; a workgroup takes one tile and one part, so that few rows over a long cache still
+// fill the chip, and attn_tree_merge_kernel joins the parts by their logsumexp.  The tiles of one part
+// run next to each other on one XCD and share its L2's copy of the keys.
+//
+// Within a workgroup the key blocks pass through a two-slot LDS ring (buffer_load ... lds, K one block
+// further ahead than V), one barrier per block: iteration n makes S^T = K Q^T and the softmax of block
+// n + 1 and multiplies P V of block n.  Each wave owns 16 rows' S phase (with fewer row tiles than waves
+// several waves make the same one: the keys' way through memory is what bounds those) and D / NW columns
+// of O^T in the P V phase, its V^T operand read from the row-major V rows with ds_read_b64_tr_b16.
+// Scores, softmax and sums are fp32; the softmax weights are rounded to bf16 for the second product, at
+// most 2^-9 of each weight, as the other attention kernels do.
+//
+// Values a row does not see never reach it: blocks that some row sees only in part (those at the window's
+// edge and the tree's own) are searched for infinities and NaN in V, and where there are any the product
+// runs over the weights that are not zero only, instead of the MFMA, whose 0 * inf would be NaN.
+#include <algorithm>
+
+#include "attn_common.h"
+
+namespace w8a8 {
+
+constexpr int TREE_MAX_NODES = 128;   // M, so that a node's view of the tree is four words
+constexpr int TREE_WORDS = TREE_MAX_NODES / 32;
+constexpr int TREE_MAX_PARTS = 512;
+
+struct TreeParams {
+  const uint16_t* q; int64_t qhs, qrs;  // bf16 [H, N, D] (element strides, last dim contiguous)
+  const uint16_t* k; int64_t khs, krs;  // bf16 [KV, Tk, D]
+  const uint16_t* v; int64_t vhs, vrs;
+  uint16_t* o; int64_t ohs, ors;        // bf16 [H, N, D]
+  float* lse;                           // fp32 [H, N], or null
+  const int32_t* parents;               // [M]
+  const int32_t* past_dev;              // n_past in device memory, or null: past
+  int past;
+  int KV, G, N, M, Tk, window;
+  int rows, ntiles, nparts;             // N G rows, tiles of them, parts of the keys (at most)
+  float* part_o;                        // [KV][nparts][rows][D] unnormalised sums
+  float* part_ml;                       // [KV][nparts][rows][2] reference exponent and sum
+  float c;                              // scale * log2(e)
+};
+
+// The call's context length, first key, key blocks and live parts.  A length in device memory outside
+// 0 .. Tk - M is the caller's error: it is brought into that range, so nothing outside the cache is read.
+struct TreeGeom {
+  int past, klo, nblk, nparts;
+};
+template <int BN>
+__device__ __forceinline__ TreeGeom tree_geom(const TreeParams& p) {
+  TreeGeom t;
+  t.past = p.past_dev ? max(0, min(*p.past_dev, p.Tk - p.M)) : p.past;
+  t.klo = p.window > 0 ? max(0, t.past - p.window + 1) : 0;
+  t.nblk = (t.past + p.M - t.klo + BN - 1) / BN;
+  t.nparts = min(p.nparts, t.nblk);
+  return t;
+}
+
+constexpr int tree_waves(int rt) { return rt == 8 ? 8 : 4; }
+
+template <int D, int RT>
+struct TreeShape {
+  static constexpr int NW = tree_waves(RT);
+  static constexpr int NT = NW * 64;
+  static constexpr int BN = D == 128 ? 64 : 32;      // keys per block
+  static constexpr int R = RT * 16;                  // rows per tile
+  static constexpr int KCH = D / 8;                  // 16-byte chunks per K / V row
+  static constexpr int ROW = D * 2;
+  static constexpr int KV_SLOT = BN * ROW;
+  static constexpr int PLD = BN + 8;                 // padded P row, elements
+  static constexpr int P_SLOT = R * PLD * 2;
+  static constexpr int V_OFF = 2 * KV_SLOT, P_OFF = 4 * KV_SLOT, A_OFF = P_OFF + 2 * P_SLOT;
+  static constexpr int F_OFF = A_OFF + 2 * R * 4;    // alpha [2][R]; flags [2][16]
+  static constexpr int B_OFF = F_OFF + 2 * 16 * 4;   // the nodes' views [M][4]; depths [M]; chain ends [M]
+  static constexpr int LDS = B_OFF + TREE_MAX_NODES * (TREE_WORDS + 2) * 4;
+  static constexpr int NDW = D / NW / 16;            // 16-wide d tiles of O^T per wave
+};
+
+// The nodes' views of the tree into LDS: bits[m] = the nodes on m's chain (none: unused), depth[m].  Every
+// chain's known length doubles each round (bits of the node its known part ends at are added), so a
+// drafted tree of depth 8 takes three rounds.
+template <int NT>
+__device__ __forceinline__ void tree_resolve(const int32_t* parents, int M, uint32_t* bits, int* depth, int* end) {
+  const int m = threadIdx.x;
+  const bool on = m < M;
+  uint32_t b[TREE_WORDS] = {};
+  int e = -1;
+  if (on) {
+    const int par = parents[m];
+    e = par >= -1 && par < m ? par : -2;
+#pragma unroll
+    for (int w = 0; w < TREE_WORDS; ++w) {
+      b[w] = (m >> 5) == w ? 1u << (m & 31) : 0u;
+      bits[m * TREE_WORDS + w] = b[w];
+    }
+    end[m] = e;
+  }
+  while (__syncthreads_or(on && e >= 0)) {  // (at most 7 rounds: every parent is before its node)
+    int ne = e;
+    if (on && e >= 0) {
+#pragma unroll
+      for (int w = 0; w < TREE_WORDS; ++w) b[w] |= bits[e * TREE_WORDS + w];
+      ne = end[e];
+    }
+    __syncthreads();
+    if (on && e >= 0) {
+#pragma unroll
+      for (int w = 0; w < TREE_WORDS; ++w) bits[m * TREE_WORDS + w] = b[w];
+      end[m] = ne;
+    }
+    e = ne;
+  }
+  if (on) {
+    int n = -1;
+#pragma unroll
+    for (int w = 0; w < TREE_WORDS; ++w) {
+      n += __popc(b[w]);
+      if (e == -2) bits[m * TREE_WORDS + w] = 0u;
+    }
+    depth[m] = n;
+  }
+  __syncthreads();
+}
+
+template <int D, int RT>
+__global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeParams p) {
+  using S = TreeShape<D, RT>;
+  constexpr int NW = S::NW, NT = S::NT, BN = S::BN, R = S::R, KCH = S::KCH, ROW = S::ROW, PLD = S::PLD, NDW = S::NDW;
+  constexpr int NKC = BN / 32;              // 32-key chunks per block
+  constexpr int KU = BN * KCH / NT;         // DMA instructions per thread per K or V block
+  constexpr int NKK = D / 32;               // k-steps of S^T
+  static_assert(KU * NT == BN * KCH && NDW >= 1 && RT <= NW && NT >= TREE_MAX_NODES, "tiling");
+  static_assert(S::LDS <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) char lds[S::LDS];
+  float* const alpha_s = reinterpret_cast<float*>(lds + S::A_OFF);
+  int* const flag_s = reinterpret_cast<int*>(lds + S::F_OFF);
+  uint32_t* const bits_s = reinterpret_cast<uint32_t*>(lds + S::B_OFF);
+  int* const depth_s = reinterpret_cast<int*>(bits_s + TREE_MAX_NODES * TREE_WORDS);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qi = lane & 15, qq = lane >> 4;
+
+  // block b: XCD b % 8 runs the tiles of (KV head, part) pairs b % 8, b % 8 + 8, .. one after the other
+  const TreeGeom geo = tree_geom<BN>(p);
+  const int x = int(blockIdx.x) >> 3;
+  const int pair = (x / p.ntiles) * 8 + (int(blockIdx.x) & 7), tile = x % p.ntiles;
+  const int g = pair / p.nparts, part = pair % p.nparts;
+  if (g >= p.KV || part >= geo.nparts) return;  // (the whole workgroup, before any barrier)
+  const int past = geo.past, M = p.M, G = p.G, win = p.window;
+  const int n_lo = int(int64_t(part) * geo.nblk / geo.nparts), n_hi = int(int64_t(part + 1) * geo.nblk / geo.nparts);
+  const int kb0 = geo.klo + n_lo * BN, nblk = n_hi - n_lo;  // at least one block
+  const bool last_part = part == geo.nparts - 1;
+
+  // the part's keys as buffers of their own, so that a cache of any length has 32-bit offsets; rows past
+  // the last node's read zero
+  const int nkeys = min(nblk * BN, past + M - kb0);
+  const uint32_t krs2 = uint32_t(p.krs) * 2u, vrs2 = uint32_t(p.vrs) * 2u;
+  const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + int64_t(g) * p.khs + int64_t(kb0) * p.krs,
+                                              uint32_t(nkeys - 1) * krs2 + uint32_t(ROW));
+  const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + int64_t(g) * p.vhs + int64_t(kb0) * p.vrs,
+                                              uint32_t(nkeys - 1) * vrs2 + uint32_t(ROW));
+
+  // K chunk x of row r lands at stored chunk x ^ swz(r), swz(r) = (r & 3) | ((r >> 1) & 12); V chunk x of
+  // row r at x ^ 2 (r & 3)
+  uint32_t koff[KU], voff[KU];
+#pragma unroll
+  for (int u = 0; u < KU; ++u) {
+    const int xc = (u * NW + wave) * 64 + lane;
+    const int row = xc / KCH, cs = xc % KCH;
+    koff[u] = uint32_t(row) * krs2 + uint32_t(cs ^ ((row & 3) | ((row >> 1) & 12))) * 16u;
+    voff[u] = uint32_t(row) * vrs2 + uint32_t(cs ^ (2 * (row & 3))) * 16u;
+  }
+  auto issue_k = [&](int n) __attribute__((always_inline)) {
+    char* base = lds + (n & 1) * S::KV_SLOT;
+    const uint32_t rowoff = uint32_t(n * BN) * krs2;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) attn_dma16(rk, base + (u * NW + wave) * 1024, rowoff + koff[u]);
+  };
+  auto issue_v = [&](int n) __attribute__((always_inline)) {
+    char* base = lds + S::V_OFF + (n & 1) * S::KV_SLOT;
+    const uint32_t rowoff = uint32_t(n * BN) * vrs2;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) attn_dma16(rv, base + (u * NW + wave) * 1024, rowoff + voff[u]);
+  };
+
+  issue_k(0);
+  issue_v(0);
+  // Q (B operand: lane (qi, qq) holds q[row][32 kk + 8 qq .. + 7] of this wave's 16 rows)
+  const int srow = 16 * (wave % RT) + qi;
+  const int row = tile * R + srow;               // (node, head) row of the KV head
+  const bool valid = row < p.rows;
+  const int qnode = row / G, hl = row % G;
+  v8bf qf[NKK];
+  {
+    const uint16_t* qp = p.q + int64_t(g * G + hl) * p.qhs + int64_t(qnode) * p.qrs + 8 * qq;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      v4i t = v4i{0, 0, 0, 0};
+      if (valid) t = *reinterpret_cast<const v4i*>(qp + 32 * kk);
+      qf[kk] = __builtin_bit_cast(v8bf, t);
+    }
+  }
+  if (nblk > 1) issue_k(1);
+
+  // Block n is seen whole by every row when its keys are all context inside every node's window.
+  auto inner = [&](int n) __attribute__((always_inline)) {
+    const int kb = kb0 + n * BN;
+    return kb + BN <= past && (win <= 0 || kb > past + M - 1 - win);
+  };
+  // this row's view of the tree, where the part has blocks that are not seen whole
+  uint32_t bits[TREE_WORDS] = {};
+  int depth = 0;
+  if (!inner(0) || !inner(nblk - 1)) {
+    tree_resolve<NT>(p.parents, M, bits_s, depth_s, depth_s + TREE_MAX_NODES);
+    if (valid) {
+      const int m = M - p.N + qnode;
+#pragma unroll
+      for (int w = 0; w < TREE_WORDS; ++w) bits[w] = bits_s[m * TREE_WORDS + w];
+      depth = depth_s[m];
+    }
+  }
+  const bool live = (bits[0] | bits[1] | bits[2] | bits[3]) != 0u;
+  auto visible = [&](int key) __attribute__((always_inline)) {
+    const int rel = key - past;
+    const uint32_t w = rel < 64 ? (rel < 32 ? bits[0] : bits[1]) : (rel < 96 ? bits[2] : bits[3]);
+    const bool in_tree = (rel < M) & (((w >> (rel & 31)) & 1u) != 0u);
+    bool vis = live & ((rel < 0) | in_tree);
+    if (win > 0) {
+      const int kd = rel < 0 ? rel : depth_s[min(rel, TREE_MAX_NODES - 1)];  // the key's position - past
+      vis = vis & (depth - kd < win);
+    }
+    return vis;
+  };
+
+  const int krow = 8 * (qi >> 2) + (qi & 3);
+  uint32_t kofs[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) kofs[j] = uint32_t(krow * KCH * 16 + (((4 * j + qq) ^ qi) * 16));
+
+  // running softmax state of this lane's row: reference exponent ms (log2 units, trailing the maximum by
+  // at most 8) and this lane group's share l of sum exp2(s c - ms)
+  float ms = -__builtin_inff(), l = 0.0f;
+  const float c = p.c;
+
+  // S^T of block n, softmax, P rows and rescale factors into slot n % 2
+  auto s_phase = [&](int n) __attribute__((always_inline)) {
+    const int slot = n & 1;
+    v4f s[2 * NKC];
+    const char* kbase = lds + slot * S::KV_SLOT;
+#pragma unroll
+    for (int t = 0; t < 2 * NKC; ++t) s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+      for (int t = 0; t < 2 * NKC; ++t) {
+        const int row0 = 32 * (t >> 1) + 4 * (t & 1);
+        const v8bf a = *reinterpret_cast<const v8bf*>(kbase + kofs[kk % 4] + row0 * (KCH * 16) + (kk / 4) * 256);
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[kk], s[t], 0, 0, 0);
+      }
+    if (!inner(n)) {
+#pragma unroll
+      for (int t = 0; t < 2 * NKC; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[t][i] = attn_mask(s[t][i], visible(kb0 + n * BN + 32 * (t >> 1) + 8 * qq + 4 * (t & 1) + i));
+    }
+    float bm = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < 2 * NKC; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bm = fmaxf(bm, s[t][i]);
+    bm = lanes4_max(bm);
+    const float bmc = bm * c;
+    const bool grow = bmc > ms + 8.0f;  // false while every key so far is masked (bmc = -inf)
+    const bool had = ms != -__builtin_inff();
+    const float alpha = !grow ? 1.0f : (had ? __builtin_amdgcn_exp2f(ms - bmc) : 0.0f);
+    ms = grow ? bmc : ms;
+    const float mref = ms == -__builtin_inff() ? 0.0f : ms;
+    float bs = 0.0f;
+    uint16_t* prow = reinterpret_cast<uint16_t*>(lds + S::P_OFF + slot * S::P_SLOT) + srow * PLD + 8 * qq;
+#pragma unroll
+    for (int ch = 0; ch < NKC; ++ch) {
+      v8bf pb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * ch + (e >> 2)][e & 3], c, -mref));
+        bs += pe;
+        pb[e] = (__bf16)pe;
+      }
+      if (wave < RT) *reinterpret_cast<v8bf*>(prow + 32 * ch) = pb;
+    }
+    l = l * alpha + bs;
+    if (wave < RT) {
+      if (qq == 0) alpha_s[slot * R + srow] = alpha;
+      // a row whose maximum grew past a finite one needs its O rescaled (a row that had none has O = 0)
+      const bool any = __builtin_amdgcn_ballot_w64(grow && had) != 0;
+      if (lane == 0) flag_s[slot * 16 + wave] = any ? 1 : 0;
+    }
+  };
+
+  // O^T for columns [wave D/NW, (wave+1) D/NW) of all rows: o[dt][rt] register i of lane (qi, qq) is
+  // d = wave D/NW + 16 dt + 4 qq + i, row 16 rt + qi
+  v4f o[NDW][RT];
+#pragma unroll
+  for (int dt = 0; dt < NDW; ++dt)
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) o[dt][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const int vsrc = qq * 8 + (qi >> 2);  // this lane's V source row within a 32-key chunk (+4)
+  auto pv_phase = [&](int n) __attribute__((always_inline)) {
+    const int slot = n & 1;
+    int f = 0;
+#pragma unroll
+    for (int w = 0; w < RT; ++w) f |= flag_s[slot * 16 + w];
+    if (f != 0) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float a = alpha_s[slot * R + rt * 16 + qi];
+#pragma unroll
+        for (int dt = 0; dt < NDW; ++dt) o[dt][rt] *= a;
+      }
+    }
+    const char* vl = lds + S::V_OFF + slot * S::KV_SLOT;
+    const uint16_t* pl = reinterpret_cast<const uint16_t*>(lds + S::P_OFF + slot * S::P_SLOT);
+    if (!inner(n)) {
+      // an infinity or a NaN anywhere in the block's V (the same for the workgroup)
+      uint32_t bad = 0;
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const v4u w = *reinterpret_cast<const v4u*>(vl + (u * NT + tid) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          bad |= uint32_t((w[e] & 0x7f80u) == 0x7f80u) | uint32_t((w[e] & 0x7f800000u) == 0x7f800000u);
+      }
+      if (__syncthreads_or(int(bad))) {
+        for (int key = 0; key < BN; ++key)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const float pe = bf16_to_f32(pl[(rt * 16 + qi) * PLD + key]);
+            if (pe == 0.0f) continue;  // not seen
+#pragma unroll
+            for (int dt = 0; dt < NDW; ++dt) {
+              const int d = wave * (D / NW) + 16 * dt + 4 * qq;
+              const v2u w = *reinterpret_cast<const v2u*>(vl + key * ROW + (((d >> 3) ^ (2 * (key & 3))) * 16) + (d & 7) * 2);
+              o[dt][rt][0] = __builtin_fmaf(pe, __uint_as_float(w[0] << 16), o[dt][rt][0]);
+              o[dt][rt][1] = __builtin_fmaf(pe, __uint_as_float(w[0] & 0xffff0000u), o[dt][rt][1]);
+              o[dt][rt][2] = __builtin_fmaf(pe, __uint_as_float(w[1] << 16), o[dt][rt][2]);
+              o[dt][rt][3] = __builtin_fmaf(pe, __uint_as_float(w[1] & 0xffff0000u), o[dt][rt][3]);
+            }
+          }
+        return;
+      }
+    }
+#pragma unroll
+    for (int ch = 0; ch < NKC; ++ch) {
+      v8bf va[NDW];
+#pragma unroll
+      for (int dt = 0; dt < NDW; ++dt) {
+        const int d = wave * (D / NW) + 16 * dt + 4 * (qi & 3);  // this lane's 4 source columns
+        const int r0 = 32 * ch + vsrc, r1 = r0 + 4;
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(
+            vl + r0 * ROW + (((d >> 3) ^ (2 * (r0 & 3))) * 16) + (d & 7) * 2));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(
+            vl + r1 * ROW + (((d >> 3) ^ (2 * (r1 & 3))) * 16) + (d & 7) * 2));
+        va[dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const v8bf pb = *reinterpret_cast<const v8bf*>(pl + (rt * 16 + qi) * PLD + 32 * ch + 8 * qq);
+#pragma unroll
+        for (int dt = 0; dt < NDW; ++dt) o[dt][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[dt], pb, o[dt][rt], 0, 0, 0);
+      }
+    }
+  };
+
+  if (nblk > 1)
+    attn_wait_vmcnt<KU>();  // K(0), V(0) and Q have landed; K(1) may be in flight
+  else
+    attn_wait_vmcnt<0>();
+  __syncthreads();
+  s_phase(0);
+  for (int n = 0; n + 1 < nblk; ++n) {
+    attn_wait_vmcnt<0>();
+    __syncthreads();  // P(n) of every row; K(n + 1) and V(n) in LDS; the other slots free
+    if (n + 2 < nblk) issue_k(n + 2);
+    issue_v(n + 1);
+    s_phase(n + 1);
+    pv_phase(n);
+  }
+  attn_wait_vmcnt<0>();
+  __syncthreads();
+  pv_phase(nblk - 1);
+
+  // An unused node's row: the last part, which holds the tree, marks it with a sum of -1.
+  float lt = lanes4_sum(l);
+  if (last_part && !live) {
+    ms = -__builtin_inff();
+    lt = -1.0f;
+  }
+  const int d_lane = wave * (D / NW) + 4 * qq;  // + 16 dt + i
+  if (geo.nparts > 1) {
+    const int64_t base = (int64_t(g) * p.nparts + part) * p.rows;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = tile * R + rt * 16 + qi;
+      if (r < p.rows) {
+        float* po = p.part_o + (base + r) * D + d_lane;
+#pragma unroll
+        for (int dt = 0; dt < NDW; ++dt) *reinterpret_cast<v4f*>(po + 16 * dt) = o[dt][rt];
+      }
+    }
+    if (wave < RT && qq == 0 && valid) *reinterpret_cast<v2f*>(p.part_ml + (base + row) * 2) = v2f{ms, lt};
+    return;
+  }
+  // one part: normalise and store (the row factors over the rescale factors, read for the last time)
+  __syncthreads();
+  if (wave < RT && qq == 0) {
+    alpha_s[srow] = lt > 0.0f ? 1.0f / lt : (lt == lt ? 0.0f : lt);  // (a NaN sum stays one)
+    if (valid && p.lse)
+      p.lse[int64_t(g * G + hl) * p.N + qnode] =
+          lt > 0.0f ? ms * 0.69314718055994531f + __logf(lt) : (lt == lt ? -__builtin_inff() : lt);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = tile * R + rt * 16 + qi;
+    if (r < p.rows) {
+      const float inv = alpha_s[rt * 16 + qi];
+      uint16_t* op = p.o + int64_t(g * G + r % G) * p.ohs + int64_t(r / G) * p.ors + d_lane;
+#pragma unroll
+      for (int dt = 0; dt < NDW; ++dt) {
+        v2u w;
+        w[0] = inv != 0.0f ? pack_bf16x2(o[dt][rt][0] * inv, o[dt][rt][1] * inv) : 0u;
+        w[1] = inv != 0.0f ? pack_bf16x2(o[dt][rt][2] * inv, o[dt][rt][3] * inv) : 0u;
+        *reinterpret_cast<v2u*>(op + 16 * dt) = w;
+      }
+    }
+  }
+}
+
+// Joins the parts of each row: M = max m_s, w_s = exp2(m_s - M), o = sum_s w_s o_s / sum_s w_s l_s.  A
+// workgroup takes one row's 64 columns: thread t sums column group t % 16 over parts t / 16, + 16, ..,
+// eight loads in flight, and the 16 sums are added in order (the same result whatever the timing).
+template <int D, int BN>
+__global__ __launch_bounds__(256) void attn_tree_merge_kernel(TreeParams p) {
+  __shared__ float wsh[TREE_MAX_PARTS];
+  __shared__ v4f sums[256];
+  __shared__ float red[4][2];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int g = blockIdx.x / p.rows, row = blockIdx.x % p.rows;
+  const int np = tree_geom<BN>(p).nparts;
+  if (np <= 1) return;  // the attention kernel wrote the row
+  const int64_t base = int64_t(g) * p.nparts * p.rows + row;  // part s at base + s * rows
+  const v2f* ml = reinterpret_cast<const v2f*>(p.part_ml) + base;
+  float mx = -__builtin_inff();
+  for (int s = t; s < np; s += 256) mx = fmaxf(mx, ml[int64_t(s) * p.rows][0]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  if (lane == 0) red[wave][0] = mx;
+  const bool unused = ml[int64_t(np - 1) * p.rows][1] == -1.0f;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  const float mref = mx == -__builtin_inff() ? 0.0f : mx;
+  float L = 0.0f;
+  for (int s = t; s < np; s += 256) {
+    const v2f v = ml[int64_t(s) * p.rows];
+    const float w = __builtin_amdgcn_exp2f(v[0] - mref);
+    wsh[s] = w;
+    L = __builtin_fmaf(w, v[1], L);
+  }
+  L = wave_sum(L);
+  if (lane == 0) red[wave][1] = L;
+  __syncthreads();
+  L = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
+  const int col = blockIdx.y * 64 + 4 * (t & 15), p0 = t >> 4;
+  const float* po = p.part_o + base * D + col;
+  v4f acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = p0; s0 < np; s0 += 128) {
+    v4f v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + 16 * u;
+      v[u] = s < np ? *reinterpret_cast<const v4f*>(po + int64_t(s) * p.rows * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + 16 * u;
+      const float w = s < np ? wsh[s] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[u][i], acc[i]);
+    }
+  }
+  sums[t] = acc;
+  __syncthreads();
+  if (t >= 16) return;
+#pragma unroll
+  for (int s = 1; s < 16; ++s) acc += sums[16 * s + t];
+  const int node = row / p.G, h = g * p.G + row % p.G;
+  const bool none = unused || L == 0.0f;
+  v2u w = v2u{0u, 0u};
+  if (!none) {
+    const float inv = 1.0f / L;
+    w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+  }
+  *reinterpret_cast<v2u*>(p.o + int64_t(h) * p.ohs + int64_t(node) * p.ors + col) = w;
+  if (p.lse && col == 0)
+    p.lse[int64_t(h) * p.N + node] = none ? -__builtin_inff() : mx * 0.69314718055994531f + __logf(L);
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+// Row tile (in 16 rows) and key parts of a call.
+struct TreePlan {
+  int rt, ntiles, nparts;
+  int64_t nblk;  // key blocks of the longest span
+};
+
+static TreePlan tree_plan(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D, int64_t past,
+                          int64_t window) {
+  const int64_t rows = N * (H / KV);
+  TreePlan pl;
+  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+  pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
+  const int bn = D == 128 ? 64 : 32;
+  const int64_t ctx = past >= 0 ? past : Tk - M;  // a length in device memory: the longest
+  const int64_t span = (window > 0 && window - 1 < ctx ? window - 1 : ctx) + M;
+  pl.nblk = (span + bn - 1) / bn;
+  const int64_t np = attn_cu_count() / (KV * pl.ntiles);
+  pl.nparts = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(np, pl.nblk), TREE_MAX_PARTS)));
+  return pl;
+}
+
+template <int D>
+static void tree_launch(const TreeParams& p, int rt, hipStream_t stream) {
+  const unsigned pairs = unsigned(p.KV) * unsigned(p.nparts);
+  const dim3 grid{(pairs + 7) / 8 * 8 * unsigned(p.ntiles), 1, 1};
+  if (rt == 1)
+    attn_tree_kernel<D, 1><<<grid, TreeShape<D, 1>::NT, 0, stream>>>(p);
+  else if (rt == 2)
+    attn_tree_kernel<D, 2><<<grid, TreeShape<D, 2>::NT, 0, stream>>>(p);
+  else if (rt == 4)
+    attn_tree_kernel<D, 4><<<grid, TreeShape<D, 4>::NT, 0, stream>>>(p);
+  else
+    attn_tree_kernel<D, 8><<<grid, TreeShape<D, 8>::NT, 0, stream>>>(p);
+  if (p.nparts > 1)
+    attn_tree_merge_kernel<D, TreeShape<D, 1>::BN>
+        <<<dim3{unsigned(p.KV * p.rows), unsigned(D / 64), 1}, 256, 0, stream>>>(p);
+}
+
+static bool tree_shape_ok(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D, int64_t window) {
+  return H >= 1 && KV >= 1 && H % KV == 0 && H <= (1 << 16) && N >= 1 && N <= M && M <= TREE_MAX_NODES && Tk >= M &&
+         Tk <= INT32_MAX / 2 && window >= 0 && window <= INT32_MAX / 2 && (D == 128 || D == 256 || D == 512);
+}
+
+}  // namespace w8a8
+
+using namespace w8a8;
+
+extern "C" int64_t w8a8_attention_tree_workspace_bytes(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk,
+                                                       int64_t D, int64_t n_past, int64_t window) {
+  if (!tree_shape_ok(H, KV, N, M, Tk, D, window) || n_past < -1 || n_past > Tk - M) return -1;
+  const TreePlan pl = tree_plan(H, KV, N, M, Tk, D, n_past, window);
+  return pl.nparts > 1 ? int64_t(H) * N * pl.nparts * (D + 2) * 4 : 0;
+}
+
+extern "C" int w8a8_attention_tree_bf16(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride,
+                                        const uint16_t* k, int64_t k_head_stride, int64_t k_row_stride,
+                                        const uint16_t* v, int64_t v_head_stride, int64_t v_row_stride, int64_t H,
+                                        int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D,
+                                        const int32_t* parents, int64_t n_past, const int32_t* n_past_dev,
+                                        int64_t window, float scale, uint16_t* o, int64_t o_head_stride,
+                                        int64_t o_row_stride, float* lse, void* workspace, int64_t workspace_bytes,
+                                        hipStream_t stream) {
+  const char* what = "attention_tree";
+  if (D != 128 && D != 256 && D != 512)
+    return fail(W8A8_ENOTSUP, "%s: head_dim %lld (supported: 128, 256, 512)", what, (long long)D);
+  if (M > TREE_MAX_NODES) return fail(W8A8_ENOTSUP, "%s: %lld nodes (at most %d)", what, (long long)M, TREE_MAX_NODES);
+  if (!tree_shape_ok(H, KV, N, M, Tk, D, window))
+    return fail(W8A8_EINVAL, "%s: H=%lld KV=%lld N=%lld M=%lld Tk=%lld window=%lld", what, (long long)H, (long long)KV,
+                (long long)N, (long long)M, (long long)Tk, (long long)window);
+  if (n_past_dev ? n_past != -1 : (n_past < 0 || n_past > Tk - M))
+    return fail(W8A8_EINVAL, "%s: n_past=%lld (0 .. Tk - M = %lld, or -1 with n_past_dev)", what, (long long)n_past,
+                (long long)(Tk - M));
+  if (!(scale > 0.0f) || scale == __builtin_inff()) return fail(W8A8_EINVAL, "%s: scale must be positive", what);
+  if (!q || !k || !v || !o || !parents) return fail(W8A8_EINVAL, "%s: null pointer", what);
+  const TreePlan pl = tree_plan(H, KV, N, M, Tk, D, n_past, window);
+  const int64_t need = w8a8_attention_tree_workspace_bytes(H, KV, N, M, Tk, D, n_past, window);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(W8A8_EINVAL, "%s: workspace of %lld bytes, %lld needed", what, (long long)(workspace ? workspace_bytes : 0),
+                (long long)need);
+  const int64_t rs[4] = {k_row_stride, v_row_stride, N > 1 ? q_row_stride : D, N > 1 ? o_row_stride : D};
+  const int64_t hs[4] = {KV > 1 ? k_head_stride : 0, KV > 1 ? v_head_stride : 0, H > 1 ? q_head_stride : 0,
+                         H > 1 ? o_head_stride : 0};
+  for (int i = 0; i < 4; ++i) {
+    if (rs[i] < D || hs[i] < 0) return fail(W8A8_EINVAL, "%s: row strides smaller than head_dim, or negative", what);
+    if (rs[i] % 8 != 0 || hs[i] % 8 != 0) return fail(W8A8_EALIGN, "%s: strides must be multiples of 8 elements", what);
+  }
+  if ((uintptr_t)q % 16 || (uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)o % 16 || (uintptr_t)workspace % 16 ||
+      (uintptr_t)parents % 4 || (uintptr_t)n_past_dev % 4 || (uintptr_t)lse % 4)
+    return fail(W8A8_EALIGN, "%s: q, k, v, o and the workspace 16-byte, parents, n_past and lse 4-byte aligned", what);
+  // a part's rows are addressed by 32-bit offsets from its first one
+  const int bn = D == 128 ? 64 : 32;
+  const int64_t most = ((pl.nblk + pl.nparts - 1) / pl.nparts + 1) * bn;
+  if (std::max(k_row_stride, v_row_stride) * 2 * most >= (int64_t(1) << 32))
+    return fail(W8A8_ENOTSUP, "%s: %lld keys of %lld bytes each per workgroup pass 32-bit offsets", what, (long long)most,
+                (long long)(std::max(k_row_stride, v_row_stride) * 2));
+  TreeParams p{};
+  p.q = q; p.qhs = hs[2]; p.qrs = rs[2]; p.k = k; p.khs = hs[0]; p.krs = rs[0]; p.v = v; p.vhs = hs[1]; p.vrs = rs[1];
+  p.o = o; p.ohs = hs[3]; p.ors = rs[3]; p.lse = lse; p.parents = parents; p.past_dev = n_past_dev;
+  p.past = int(std::max<int64_t>(n_past, 0)); p.KV = int(KV); p.G = int(H / KV); p.N = int(N); p.M = int(M);
+  p.Tk = int(Tk); p.window = int(window); p.rows = int(N * (H / KV)); p.ntiles = pl.ntiles; p.nparts = pl.nparts;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + int64_t(H) * N * pl.nparts * D;
+  p.c = scale * 1.4426950408889634f;
+  if (D == 128)
+    tree_launch<128>(p, pl.rt, stream);
+  else if (D == 256)
+    tree_launch<256>(p, pl.rt, stream);
+  else
+    tree_launch<512>(p, pl.rt, stream);
+  return check_launch("attention_tree_bf16");
+}

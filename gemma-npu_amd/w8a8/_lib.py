@@ -99,6 +99,9 @@ SIGNATURES = {
                                                    _i64, _i64, _i32, _p, _i64, _f32, _p, _i64, _p, _i64, _p]),
     "w8a8_attention_decode_bf16": (_i32, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                           _i64, _f32, _p, _i64, _p, _p, _i64, _p]),
+    "w8a8_attention_tree_workspace_bytes": (_i64, [_i64] * 8),
+    "w8a8_attention_tree_bf16": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                        _i64, _p, _i64, _p, _i64, _f32, _p, _i64, _i64, _p, _p, _i64, _p]),
 }
 
 _lib = None
@@ -162,6 +165,16 @@ def launch_module():
     if getattr(_launch, "torch_build", None) != torch_build():
         return None
     return _launch if launch_sources() in (None, getattr(_launch, "sources", None)) else None
+
+
+def call_on(t, name, *args):
+    """call() with the device of tensor t current, whichever device the caller's is: the launch belongs to
+    t's stream."""
+    import torch
+    if t.device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(t.device):
+        return call(name, *args)
 
 
 def call(name, *args):

@@ -7,6 +7,7 @@ local_attn.py:71-107).
     split_kv_decode(query, key, value, scale)        -> [1, 1, H, D]      local_attn.py:44-68
     attention(q, k, v, q_start, window, scale)      -> o (and the logsumexp)
     decode(q, k, v, q_pos, window, scale)           -> o [H, D] (and the logsumexp)
+    decode_tree(q, k, v, parents, n_past, window)   -> o [H, N, D] of a tree of drafted tokens
 
 q is bf16 [H, Tq, D] at positions q_start.., k_all / v_all bf16 [KV, Tk, D] holding positions
 0.. (Tk >= q_start + Tq); any strides with a contiguous last dimension.  Scale 1.0 as Gemma uses.
@@ -21,7 +22,7 @@ import threading
 
 import torch
 
-from ._lib import call, lib
+from ._lib import call, call_on, lib
 from .ops import PackedActivation, _native, _stream, current_stream_handle, packed_act_bytes
 
 _WS = {}
@@ -318,6 +319,79 @@ def decode_qkv_at(y, cos, sin, qw, kw, eps, H, KV, D, k, v, pos, kv_write, windo
          pos.data_ptr(), int(window), float(scale), None if out is None else out.data_ptr(),
          D if out is None or H == 1 else out.stride(0), ws.data_ptr(), ws.numel(), _stream(y))
     return out
+
+
+def _check_out(t, name, shape, device):
+    _check3(t, name)
+    if tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{name}: expected shape {shape} on {device}, got {tuple(t.shape)} on {t.device}")
+
+
+def decode_tree_workspace_bytes(H, KV, N, M, Tk, D, n_past=None, window=0):
+    """Bytes of scratch decode_tree() needs (w8a8_attention_tree_workspace_bytes); n_past None: a length
+    held in device memory."""
+    n = lib().w8a8_attention_tree_workspace_bytes(H, KV, N, M, Tk, D, -1 if n_past is None else int(n_past), int(window))
+    if n < 0:
+        raise ValueError(f"decode_tree: invalid shape H={H} KV={KV} N={N} M={M} Tk={Tk} D={D} n_past={n_past} window={window}")
+    return n
+
+
+def decode_tree(q, k, v, parents, n_past, window=0, scale=1.0, out=None, return_lse=False, workspace=None):
+    """decode() for a tree of drafted tokens: several candidates for the next tokens attend to the cache in
+    one call, each to the context and to the drafted tokens above it only.
+
+    parents: int32 GPU tensor [M], M <= 128.  Node m's key and value are row n_past + m of k / v
+    [KV, Tk, D]; its parent is node parents[m] < m, or the context's last token with -1; its position is
+    n_past + its depth.  A node with any other parent is unused, as are the nodes below it: output zero.
+    q: bf16 [H, N, D], the last N nodes' queries (N = M: the whole tree; N < M: its newest levels).
+    n_past: the context's rows, an int, or an int32 GPU tensor of one element (the launch then does not
+    depend on it, so a captured step replays at each new length).
+    Returns o [H, N, D] (into `out` if given, any strides with a contiguous last dimension), and with
+    return_lse the fp32 [H, N] logsumexp.  workspace: a device uint8 tensor of at least
+    decode_tree_workspace_bytes(...); by default one from torch's allocator."""
+    _check3(q, "q")
+    _check3(k, "k")
+    _check3(v, "v")
+    H, N, D = q.shape
+    KV, Tk, Dk = k.shape
+    if tuple(v.shape) != (KV, Tk, Dk) or Dk != D:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
+    if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or parents.dim() != 1:
+        raise ValueError("decode_tree: parents must be an int32 GPU tensor [M]")
+    M = parents.shape[0]
+    if not 1 <= N <= M:
+        raise ValueError(f"decode_tree: {N} queries for {M} nodes")
+    if M > 1 and parents.stride(0) != 1:
+        raise ValueError("decode_tree: parents must be contiguous")
+    dev = None
+    if isinstance(n_past, torch.Tensor):
+        if n_past.dtype != torch.int32 or n_past.numel() != 1 or n_past.device != q.device:
+            raise ValueError("decode_tree: n_past must be an int or an int32 tensor of one element on q's device")
+        dev, n_past = n_past, -1
+    elif not 0 <= int(n_past) <= Tk - M:
+        raise ValueError(f"decode_tree: {n_past} context rows and {M} nodes in a cache of {Tk} rows")
+    if len({q.device, k.device, v.device, parents.device}) != 1:
+        raise ValueError("q, k, v and parents must be on one device")
+    if out is None:
+        out = torch.empty((H, N, D), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out(out, "out", (H, N, D), q.device)
+    lse = torch.empty((H, N), dtype=torch.float32, device=q.device) if return_lse else None
+    if workspace is None:
+        need = decode_tree_workspace_bytes(H, KV, N, M, Tk, D, None if dev is not None else n_past, window)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError(f"decode_tree: the workspace must be a contiguous tensor on {q.device}")
+    qhs, qrs = _strides(q)
+    khs, krs = _strides(k)
+    vhs, vrs = _strides(v)
+    ohs, ors = _strides(out)
+    call_on(q, "w8a8_attention_tree_bf16", q.data_ptr(), qhs, qrs, k.data_ptr(), khs, krs, v.data_ptr(), vhs, vrs, H, KV,
+            N, M, Tk, D, parents.data_ptr(), int(n_past), None if dev is None else dev.data_ptr(), int(window),
+            float(scale), out.data_ptr(), ohs, ors, lse.data_ptr() if return_lse else None,
+            None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
+    return (out, lse) if return_lse else out
 
 
 def split_kv_decode(query, key, value, scale):

@@ -541,6 +541,38 @@ int w8a8_attention_decode_qkv_dev_bf16(const uint16_t *y, const uint16_t *cos_, 
                                        float scale, uint16_t *o, int64_t o_head_stride, void *workspace,
                                        int64_t workspace_bytes, hipStream_t stream);
 
+/* ---- attention of drafted tokens ------------------------------------------------------------ */
+
+/* Attention of the nodes of a tree of drafted tokens over a cache (no counterpart in the reference, whose
+ * decode step takes one token, local_attn.py:44-83): rows 0 .. n_past - 1 of k / v are the context, row
+ * n_past + m is node m of M, whose parent is node parents[m] (int32 [M] in device memory; -1: the
+ * context's last token; always before its child).  The queries are the last N nodes.  Node i sees the
+ * context, itself and the nodes above it; its position is n_past + its depth, and with a window W > 0 it
+ * sees what lies less than W positions before it.
+ *   o[h, i, :] = sum_j softmax_j(scale * q[h, i] . k[g, j]) v[g, j],  g = h / (H / KV)
+ * A node whose parent is not in -1 .. m - 1 is unused, and so are the nodes below it: they see nothing,
+ * their output rows are zero and their lse is -inf (their keys and values are read by no other node).
+ * What a row does not see does not reach it, infinities and NaN included; rows of the cache behind the
+ * last node are not read.
+ *   q bf16 [H, N, D], k / v bf16 [KV, Tk, D], o bf16 [H, N, D] (element strides of heads and rows, the
+ *   last dimension contiguous); lse fp32 [H, N], contiguous, natural logarithm, or NULL
+ *   n_past: 0 .. Tk - M; or n_past = -1 and n_past_dev, an int32 in device memory that the launch does
+ *   not depend on (a captured step replays at each new length; outside 0 .. Tk - M it is the caller's
+ *   error: meaningless values, never an access outside k, v or the workspace)
+ *   workspace: w8a8_attention_tree_workspace_bytes(...) bytes or more (-1: invalid arguments; 0: none
+ *   needed, NULL allowed), 16-byte aligned, scratch: nothing is kept between calls, and calls that
+ *   overlap in time need separate ones
+ * D in {128, 256, 512}; 1 <= N <= M <= 128; strides multiples of 8 elements; pointers 16-byte aligned.
+ * Deterministic.  One or two launches. */
+int64_t w8a8_attention_tree_workspace_bytes(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D,
+                                            int64_t n_past, int64_t window);
+int w8a8_attention_tree_bf16(const uint16_t *q, int64_t q_head_stride, int64_t q_row_stride, const uint16_t *k,
+                             int64_t k_head_stride, int64_t k_row_stride, const uint16_t *v, int64_t v_head_stride,
+                             int64_t v_row_stride, int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D,
+                             const int32_t *parents, int64_t n_past, const int32_t *n_past_dev, int64_t window,
+                             float scale, uint16_t *o, int64_t o_head_stride, int64_t o_row_stride, float *lse,
+                             void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
