@@ -1,0 +1,385 @@
+// A beam search step's choice: of the nb beams' V continuations each, the k of the largest
+//
+//   score[i] + log_softmax(logits[i])[v],
+//
+// sorted, ties to the lowest i V + v.  Decode's greedy tail (the reference's loop, gemma_npu.py:292-295, takes
+// the argmax) for several sequences that are weighed against each other.
+//
+// beam_chunk_kernel reads the logits once.  A workgroup takes a run of BEAM_CHUNK logits of one beam into
+// registers, makes their maximum and sum of exponentials, and finds its k largest: the k-th largest of the
+// maxima of 64 lane groups is a bound that at least k logits reach and few more do, so those are listed and
+// ranked by counting.  Where too many reach it (equal logits, as a grammar's -inf), the k are taken one by
+// one instead.  Within a beam the order of logits is the order of scores, so nothing else can be among the
+// k best.  beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k
+// best of those lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and
+// the choice between them has to be right.
+#include <algorithm>
+
+#include "w8a8_common.h"
+
+namespace w8a8 {
+
+constexpr int BEAM_MAX_K = 64;
+constexpr int BEAM_MAX_BEAMS = 256;
+constexpr int BEAM_E = 32;                  // logits per thread
+constexpr int BEAM_CHUNK = 256 * BEAM_E;
+constexpr int BEAM_LIST = 512;              // most candidates that are ranked by counting
+
+struct BeamParams {
+  const void* x; int64_t gs, rs;            // logits [B, nb, V] bf16 or fp32 (element strides of groups and beams)
+  const float* score; int64_t ss;           // fp32 [B, nb]
+  int nb, V, k, nch;
+  float2* stat;                             // [B nb][nch] maximum and sum of exponentials
+  uint2* cand;                              // [B nb][nch][k] logit's bits and token
+  float* out_score; int64_t *out_beam, *out_tok;  // [B, k]
+};
+
+// Order-preserving bits: larger for larger values, NaN above +inf, -0 and +0 alike.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t b = __float_as_uint(x);
+  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if ((b & 0x7fffffffu) == 0u) return 0x80000000u;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_bits(double x) {
+  const uint64_t b = uint64_t(__double_as_longlong(x)), m = b & 0x7fffffffffffffffull;
+  if (m > 0x7ff0000000000000ull) return ~0ull;
+  if (m == 0) return 0x8000000000000000ull;
+  return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+// The k-th largest of 64 lanes' values (k <= 64): the value whose rank, ties by lane, is k - 1.
+template <class T>
+__device__ __forceinline__ T wave_kth(T v, int k) {
+  const int lane = threadIdx.x & 63;
+  int rank = 0;
+  for (int j = 0; j < 64; ++j) {
+    const T o = __shfl(v, j, 64);
+    rank += (o > v || (o == v && j < lane)) ? 1 : 0;
+  }
+  const uint64_t at = __builtin_amdgcn_ballot_w64(rank == k - 1);
+  return __shfl(v, __builtin_ctzll(at), 64);
+}
+
+// A candidate before another: larger, or equal and of the lower index.
+template <class T>
+__device__ __forceinline__ bool before(T a, uint32_t ai, T b, uint32_t bi) {
+  return a > b || (a == b && ai < bi);
+}
+
+// The best of a workgroup's candidates, given to every thread.
+template <class T, int NW>
+__device__ __forceinline__ void block_first(T& v, uint32_t& i, T* sv, uint32_t* si) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const T ov = __shfl_xor(v, o, 64);
+    const uint32_t oi = __shfl_xor(i, o, 64);
+    if (before(ov, oi, v, i)) v = ov, i = oi;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sv[threadIdx.x >> 6] = v, si[threadIdx.x >> 6] = i;
+  __syncthreads();
+  v = sv[0], i = si[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w)
+    if (before(sv[w], si[w], v, i)) v = sv[w], i = si[w];
+}
+
+template <class X>
+__global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
+  __shared__ uint32_t lv[BEAM_LIST], li[BEAM_LIST];
+  __shared__ uint32_t gmax[64];
+  __shared__ float red[4];
+  __shared__ uint32_t bound_s;
+  __shared__ int count;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int row = blockIdx.x / p.nch, ch = blockIdx.x % p.nch;
+  const X* xp = static_cast<const X*>(p.x) + int64_t(row / p.nb) * p.gs + int64_t(row % p.nb) * p.rs;
+  const int base = ch * BEAM_CHUNK, n = min(BEAM_CHUNK, p.V - base);
+  // element e of thread t is logit base + 8 (t + 256 (e / 8)) + e % 8
+  float v[BEAM_E];
+  const bool wide = (reinterpret_cast<uintptr_t>(xp) & 15) == 0;
+#pragma unroll
+  for (int c = 0; c < BEAM_E / 8; ++c) {
+    const int at = 8 * (t + 256 * c);
+    const X* src = xp + base + at;
+    if (wide && at + 8 <= n) {
+      if constexpr (sizeof(X) == 2) {
+        float f[8];
+        unpack8(*reinterpret_cast<const v4u*>(src), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * c + e] = f[e];
+      } else {
+        const v4f a = *reinterpret_cast<const v4f*>(src), b = *reinterpret_cast<const v4f*>(src + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[8 * c + e] = a[e], v[8 * c + 4 + e] = b[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float f = 0.0f;
+        if (at + e < n) {
+          if constexpr (sizeof(X) == 2)
+            f = bf16_to_f32(src[e]);
+          else
+            f = src[e];
+        }
+        v[8 * c + e] = f;
+      }
+    }
+  }
+  auto valid = [&](int e) __attribute__((always_inline)) { return 8 * (t + 256 * (e >> 3)) + (e & 7) < n; };
+  auto index = [&](int e) __attribute__((always_inline)) { return uint32_t(base + 8 * (t + 256 * (e >> 3)) + (e & 7)); };
+
+  // maximum (without NaN: one makes the sum NaN) and sum of exponentials
+  float m = -__builtin_inff();
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < BEAM_E; ++e)
+    if (valid(e)) {
+      m = fmaxf(m, v[e]);
+      top = max(top, order_bits(v[e]));
+    }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (lane == 0) red[wave] = m;
+  if (t == 0) count = 0;
+  // the maxima of groups of four lanes
+  top = max(top, uint32_t(__shfl_xor(top, 1, 64)));
+  top = max(top, uint32_t(__shfl_xor(top, 2, 64)));
+  if ((t & 3) == 0) gmax[t >> 2] = top;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (wave == 0) {
+    const uint32_t b = wave_kth(gmax[lane], p.k);
+    if (lane == 0) bound_s = b;
+  }
+  const float mref = m == -__builtin_inff() ? 0.0f : m;
+  float s = 0.0f;
+#pragma unroll
+  for (int e = 0; e < BEAM_E; ++e)
+    if (valid(e)) s += __expf(v[e] - mref);
+  s = wave_sum(s);
+  __syncthreads();
+  if (lane == 0) red[wave] = s;
+  const uint32_t bound = bound_s;  // (0, below every logit, where fewer than k groups hold any)
+#pragma unroll
+  for (int e = 0; e < BEAM_E; ++e)
+    if (valid(e) && order_bits(v[e]) >= bound) {
+      const int at = atomicAdd(&count, 1);
+      if (at < BEAM_LIST) lv[at] = order_bits(v[e]), li[at] = index(e);
+    }
+  __syncthreads();
+  const int64_t slot = int64_t(row) * p.nch + ch;
+  if (t == 0) p.stat[slot] = make_float2(m, (red[0] + red[1]) + (red[2] + red[3]));
+  uint2* out = p.cand + slot * p.k;
+  const int nc = count;
+  auto value = [&](uint32_t o) __attribute__((always_inline)) {  // the logit's bits again (NaN: the quiet one)
+    return o == 0xffffffffu ? 0x7fc00000u : (o & 0x80000000u ? o & 0x7fffffffu : ~o);
+  };
+  if (nc <= BEAM_LIST) {
+    for (int j = t; j < nc; j += 256) {
+      int rank = 0;
+      const uint32_t a = lv[j], ai = li[j];
+      for (int c = 0; c < nc; ++c) rank += before(lv[c], li[c], a, ai) ? 1 : 0;
+      if (rank < p.k) out[rank] = make_uint2(value(a), ai);
+    }
+    for (int j = nc + t; j < p.k; j += 256) out[j] = make_uint2(0u, 0xffffffffu);  // none
+    return;
+  }
+  // one by one: the best after the last one taken
+  uint32_t last = 0xffffffffu, lasti = 0;
+  bool any = false;
+  for (int j = 0; j < p.k; ++j) {
+    uint32_t b = 0, bi = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < BEAM_E; ++e) {
+      const uint32_t o = order_bits(v[e]), i = index(e);
+      if (valid(e) && (!any || before(last, lasti, o, i)) && before(o, i, b, bi)) b = o, bi = i;
+    }
+    block_first<uint32_t, 4>(b, bi, lv, li);
+    if (t == 0) out[j] = make_uint2(value(b), bi);
+    last = b, lasti = bi, any = true;
+  }
+}
+
+__global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
+  __shared__ double base_s[BEAM_MAX_BEAMS];
+  __shared__ uint64_t lv[BEAM_LIST], gmax[64], bound_s;
+  __shared__ uint32_t li[BEAM_LIST];
+  __shared__ int count;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int grp = blockIdx.x;
+  if (t == 0) count = 0;
+  // base[i] = score - logsumexp of beam i, one wave per beam
+  for (int i = wave; i < p.nb; i += 16) {
+    const float2* st = p.stat + (int64_t(grp) * p.nb + i) * p.nch;
+    float m = -__builtin_inff();
+    for (int c = lane; c < p.nch; c += 64) m = fmaxf(m, st[c].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    double s = 0.0;
+    for (int c = lane; c < p.nch; c += 64) {
+      const float2 a = st[c];
+      // a chunk of -inf only has the sum 0 of its reference 0
+      s += a.x == -__builtin_inff() ? double(a.y) : double(a.y) * exp(double(a.x) - double(m));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    const double sc = double(p.score[int64_t(grp) * p.ss + i]);
+    // no token can follow where all logits are -inf; +inf and NaN make NaN, as log_softmax does
+    const double b = m == -__builtin_inff() && s == 0.0 ? (sc != sc ? sc : -__builtin_inf()) : sc - (double(m) + log(s));
+    if (lane == 0) base_s[i] = b;
+  }
+  __syncthreads();
+  const int per = p.nch * p.k, total = p.nb * per;
+  const uint2* cand = p.cand + int64_t(grp) * p.nb * per;
+  // candidate j: its score's order bits and i V + v; false where there is none.  A beam whose base is not
+  // finite has that score for every token: its first tokens stand for it.
+  auto get = [&](int j, uint64_t& o, uint64_t& at) __attribute__((always_inline)) {
+    const int i = j / per, c = j % per;
+    const uint2 a = cand[j];
+    const double b = base_s[i];
+    uint32_t tok = a.y;
+    double sc = b + double(__uint_as_float(a.x));
+    if (!(b - b == 0.0)) {
+      sc = b;
+      tok = c < p.k && c < p.V ? uint32_t(c) : 0xffffffffu;
+    }
+    o = order_bits(sc);
+    at = uint64_t(i) * uint64_t(p.V) + tok;
+    return tok != 0xffffffffu;
+  };
+  uint64_t top = 0;
+  for (int j = t; j < total; j += 1024) {
+    uint64_t o, at;
+    if (get(j, o, at)) top = max(top, o);
+  }
+#pragma unroll
+  for (int x = 8; x > 0; x >>= 1) {
+    const uint64_t o = __shfl_xor(top, x, 64);
+    top = max(top, o);
+  }
+  if ((t & 15) == 0) gmax[t >> 4] = top;
+  __syncthreads();
+  if (wave == 0) {
+    const uint64_t b = wave_kth(gmax[lane], p.k);
+    if (lane == 0) bound_s = b;
+  }
+  __syncthreads();
+  const uint64_t bound = bound_s;
+  for (int j = t; j < total; j += 1024) {
+    uint64_t o, at;
+    if (get(j, o, at) && o >= bound) {
+      const int c = atomicAdd(&count, 1);
+      if (c < BEAM_LIST) lv[c] = o, li[c] = uint32_t(j);
+    }
+  }
+  __syncthreads();
+  auto store = [&](int r, int j) __attribute__((always_inline)) {
+    uint64_t o, at;
+    get(j, o, at);
+    const int i = j / per;
+    const uint64_t bits = o == ~0ull ? 0x7ff8000000000000ull : (o >> 63 ? o & 0x7fffffffffffffffull : ~o);
+    p.out_score[int64_t(grp) * p.k + r] = float(__longlong_as_double((long long)bits));
+    p.out_beam[int64_t(grp) * p.k + r] = i;
+    p.out_tok[int64_t(grp) * p.k + r] = int64_t(at - uint64_t(i) * uint64_t(p.V));
+  };
+  const int nc = count;
+  if (nc <= BEAM_LIST) {
+    for (int a = t; a < nc; a += 1024) {
+      uint64_t o, at, oo, oat;
+      get(int(li[a]), o, at);
+      int rank = 0;
+      for (int c = 0; c < nc; ++c) {
+        if (lv[c] < o) continue;
+        oo = lv[c];
+        bool first = oo > o;
+        if (!first) {
+          uint64_t dummy;
+          get(int(li[c]), dummy, oat);
+          first = oat < at;
+        }
+        rank += first ? 1 : 0;
+      }
+      if (rank < p.k) store(rank, int(li[a]));
+    }
+    return;
+  }
+  // one by one: the best after the last one taken
+  __shared__ uint64_t sv[16], sa[16];
+  __shared__ int sj[16];
+  uint64_t last = 0, lastat = 0;
+  for (int r = 0; r < p.k; ++r) {
+    uint64_t b = 0, ba = ~0ull;
+    int bj = -1;
+    for (int j = t; j < total; j += 1024) {
+      uint64_t o, at;
+      if (!get(j, o, at)) continue;
+      if (r > 0 && !(o < last || (o == last && at > lastat))) continue;
+      if (bj < 0 || o > b || (o == b && at < ba)) b = o, ba = at, bj = j;
+    }
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) {
+      const uint64_t ob = __shfl_xor(b, x, 64), oa = __shfl_xor(ba, x, 64);
+      const int oj = __shfl_xor(bj, x, 64);
+      if (oj >= 0 && (bj < 0 || ob > b || (ob == b && oa < ba))) b = ob, ba = oa, bj = oj;
+    }
+    __syncthreads();
+    if (lane == 0) sv[wave] = b, sa[wave] = ba, sj[wave] = bj;
+    __syncthreads();
+    b = sv[0], ba = sa[0], bj = sj[0];
+    for (int w = 1; w < 16; ++w)
+      if (sj[w] >= 0 && (bj < 0 || sv[w] > b || (sv[w] == b && sa[w] < ba))) b = sv[w], ba = sa[w], bj = sj[w];
+    if (t == 0) store(r, bj);
+    last = b, lastat = ba;
+  }
+}
+
+}  // namespace w8a8
+
+using namespace w8a8;
+
+static bool beam_shape_ok(int64_t B, int64_t nb, int64_t V, int64_t k) {
+  return B >= 1 && nb >= 1 && nb <= BEAM_MAX_BEAMS && V >= 1 && V <= INT32_MAX / 2 && k >= 1 && k <= BEAM_MAX_K &&
+         k <= nb * V && B * nb <= INT32_MAX / ((V + BEAM_CHUNK - 1) / BEAM_CHUNK * BEAM_MAX_K);
+}
+
+extern "C" int64_t w8a8_beam_select_workspace_bytes(int64_t B, int64_t nb, int64_t V, int64_t k) {
+  if (!beam_shape_ok(B, nb, V, k)) return -1;
+  return B * nb * ((V + BEAM_CHUNK - 1) / BEAM_CHUNK) * 8 * (k + 1);
+}
+
+extern "C" int w8a8_beam_select(const void* logits, int logits_are_f32, int64_t group_stride, int64_t row_stride,
+                                const float* scores, int64_t score_stride, int64_t B, int64_t nb, int64_t V, int64_t k,
+                                float* out_scores, int64_t* out_beams, int64_t* out_tokens, void* workspace,
+                                int64_t workspace_bytes, hipStream_t stream) {
+  const char* what = "beam_select";
+  if (!beam_shape_ok(B, nb, V, k))
+    return fail(W8A8_EINVAL, "%s: B=%lld nb=%lld V=%lld k=%lld (at most %d beams, k at most %d and nb V)", what, (long long)B,
+                (long long)nb, (long long)V, (long long)k, BEAM_MAX_BEAMS, BEAM_MAX_K);
+  if (!logits || !scores || !out_scores || !out_beams || !out_tokens || !workspace)
+    return fail(W8A8_EINVAL, "%s: null pointer", what);
+  if ((nb > 1 && row_stride < V) || (B > 1 && (group_stride < V || score_stride < nb)))
+    return fail(W8A8_EINVAL, "%s: strides smaller than the rows", what);
+  const int64_t need = w8a8_beam_select_workspace_bytes(B, nb, V, k);
+  if (workspace_bytes < need)
+    return fail(W8A8_EINVAL, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  if ((uintptr_t)logits % (logits_are_f32 ? 4 : 2) || (uintptr_t)scores % 4 || (uintptr_t)out_scores % 4 ||
+      (uintptr_t)out_beams % 8 || (uintptr_t)out_tokens % 8 || (uintptr_t)workspace % 8)
+    return fail(W8A8_EALIGN, "%s: operands naturally, the workspace 8-byte aligned", what);
+  BeamParams p{};
+  p.x = logits; p.gs = B > 1 ? group_stride : 0; p.rs = nb > 1 ? row_stride : 0;
+  p.score = scores; p.ss = B > 1 ? score_stride : 0;
+  p.nb = int(nb); p.V = int(V); p.k = int(k); p.nch = int((V + BEAM_CHUNK - 1) / BEAM_CHUNK);
+  p.stat = static_cast<float2*>(workspace);
+  p.cand = reinterpret_cast<uint2*>(p.stat + B * nb * p.nch);
+  p.out_score = out_scores; p.out_beam = out_beams; p.out_tok = out_tokens;
+  const unsigned grid = unsigned(B * nb * p.nch);
+  if (logits_are_f32)
+    beam_chunk_kernel<float><<<grid, 256, 0, stream>>>(p);
+  else
+    beam_chunk_kernel<uint16_t><<<grid, 256, 0, stream>>>(p);
+  beam_join_kernel<<<unsigned(B), 1024, 0, stream>>>(p);
+  return check_launch("beam_select");
+}

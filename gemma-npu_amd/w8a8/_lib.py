@@ -102,7 +102,23 @@ SIGNATURES = {
     "w8a8_attention_tree_workspace_bytes": (_i64, [_i64] * 8),
     "w8a8_attention_tree_bf16": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                         _i64, _p, _i64, _p, _i64, _f32, _p, _i64, _i64, _p, _p, _i64, _p]),
+    "w8a8_attention_key_weights_workspace_bytes": (_i64, [_i64] * 7),
+    "w8a8_attention_key_weights": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                          _p, _i64, _f32, _p, _i64, _p, _i64, _p]),
+    "w8a8_evict_workspace_bytes": (_i64, [_i64] * 3),
+    "w8a8_evict": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p,
+                          _i64, _p, _i64, _p, _i64, _p]),
+    "w8a8_reorder_rows": (_i32, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p]),
+    "w8a8_beam_select_workspace_bytes": (_i64, [_i64] * 4),
+    "w8a8_beam_select": (_i32, [_p, _i32, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
 }
+
+
+class Rows(ctypes.Structure):
+    """w8a8_rows: one tensor of w8a8_reorder_rows."""
+
+    _fields_ = [("data", _p), ("outer_stride", _i64), ("axis_stride", _i64), ("run_stride", _i64), ("runs", _i64),
+                ("run_bytes", _i64)]
 
 _lib = None
 _lock = threading.Lock()

@@ -8,6 +8,7 @@ local_attn.py:71-107).
     attention(q, k, v, q_start, window, scale)      -> o (and the logsumexp)
     decode(q, k, v, q_pos, window, scale)           -> o [H, D] (and the logsumexp)
     decode_tree(q, k, v, parents, n_past, window)   -> o [H, N, D] of a tree of drafted tokens
+    add_key_weights(q, k, lse, weights, q_start, W) -> weights [KV, Tk], what each key has drawn added
 
 q is bf16 [H, Tq, D] at positions q_start.., k_all / v_all bf16 [KV, Tk, D] holding positions
 0.. (Tk >= q_start + Tq); any strides with a contiguous last dimension.  Scale 1.0 as Gemma uses.
@@ -392,6 +393,53 @@ def decode_tree(q, k, v, parents, n_past, window=0, scale=1.0, out=None, return_
             None if workspace is None else workspace.data_ptr(),
             0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
     return (out, lse) if return_lse else out
+
+
+def add_key_weights(q, k, lse, weights, q_start=0, window=0, scale=1.0, workspace=None):
+    """weights[g, j] += the softmax weights that key j of KV head g drew in the attention call on the same
+    operands, summed over the group's heads and the queries: what cache.evict keeps rows by.
+
+    q: bf16 [H, Tq, D] at positions q_start.. ([H, D]: one query), k: bf16 [KV, Tk, D], lse: the fp32
+    [H, Tq] ([H]) logsumexp that attention(..., return_lse=True) or decode(..., return_lse=True) returned,
+    weights: fp32 [KV, Tk], changed in place and returned.  Keys are seen as in attention().  q_start: an int,
+    or with few rows (Tq * H // KV <= 32) an int32 GPU tensor of one element, so that a captured decode step
+    adds at each new position.  A query with an lse of -inf adds nothing.  Deterministic."""
+    if isinstance(q, torch.Tensor) and q.dim() == 2:
+        q = q[:, None]
+        lse = lse[:, None] if isinstance(lse, torch.Tensor) and lse.dim() == 1 else lse
+    _check3(q, "q")
+    _check3(k, "k")
+    H, Tq, D = q.shape
+    KV, Tk, Dk = k.shape
+    if Dk != D:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
+    for t, name, shape in ((lse, "lse", (H, Tq)), (weights, "weights", (KV, Tk))):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != shape:
+            raise ValueError(f"add_key_weights: {name} must be an fp32 GPU tensor {shape}")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"add_key_weights: {name} must have contiguous rows")
+    if len({q.device, k.device, lse.device, weights.device}) != 1:
+        raise ValueError("q, k, lse and weights must be on one device")
+    dev = None
+    if isinstance(q_start, torch.Tensor):
+        if q_start.dtype != torch.int32 or q_start.numel() != 1 or q_start.device != q.device:
+            raise ValueError("add_key_weights: q_start must be an int or an int32 tensor of one element on q's device")
+        dev, q_start = q_start, -1
+    elif not 0 <= int(q_start) <= Tk - Tq:
+        raise ValueError(f"add_key_weights: {Tq} queries from position {q_start} on and {Tk} keys")
+    if workspace is None:
+        need = lib().w8a8_attention_key_weights_workspace_bytes(H, KV, Tq, Tk, D, int(q_start), int(window))
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError(f"add_key_weights: the workspace must be a contiguous tensor on {q.device}")
+    qhs, qrs = _strides(q)
+    khs, krs = _strides(k)
+    call_on(q, "w8a8_attention_key_weights", q.data_ptr(), qhs, qrs, k.data_ptr(), khs, krs, lse.data_ptr(),
+            lse.stride(0) if H > 1 else Tq, H, KV, Tq, Tk, D, int(q_start), None if dev is None else dev.data_ptr(),
+            int(window), float(scale), weights.data_ptr(), weights.stride(0) if KV > 1 else Tk,
+            None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
+    return weights
 
 
 def split_kv_decode(query, key, value, scale):

@@ -6,7 +6,7 @@ ready for any later work on the same stream.  There is no CPU fallback.
 """
 import torch
 
-from ._lib import call, launch_module, lib
+from ._lib import call, call_on, launch_module, lib
 
 # The launch path in native code (csrc/bind.cpp), or None where it is not built.  Its functions take the
 # plain case of the wrappers below and return None for everything else, which then runs here.
@@ -464,6 +464,53 @@ def decode_tail(y, cap, pos, pos64, tok, emitted, n_emitted, logits=None, worksp
          tok.data_ptr(), emitted.data_ptr(), n_emitted.data_ptr(), emitted.numel(), ws.data_ptr(), ws.numel(),
          _stream(y))
     return logits
+
+
+def beam_select_workspace_bytes(B, nb, V, k):
+    """Bytes of scratch beam_select() needs (w8a8_beam_select_workspace_bytes)."""
+    n = lib().w8a8_beam_select_workspace_bytes(int(B), int(nb), int(V), int(k))
+    if n < 0:
+        raise ValueError(f"beam_select: {k} of {nb} beams x {V} tokens in {B} groups (at most 256 beams, k at most 64)")
+    return n
+
+
+def beam_select(logits, scores, k, workspace=None):
+    """A beam search step's choice: the k best of scores[i] + log_softmax(logits[i])[v] over beams and
+    vocabulary, sorted, ties to the lowest i * V + v.
+
+    logits: bf16 or fp32 [nb, V], or [B, nb, V] for B requests; scores: fp32 [nb] ([B, nb]), what the beams
+    have so far (-inf: a beam that is out, as all but the first before the first step).  Returns (scores fp32,
+    beams int64, tokens int64), each [k] ([B, k]); cache.reorder(states, beams) then puts the beams' keys
+    and values in order.  -inf logits are tokens that cannot follow; a NaN or +inf logit makes its beam's
+    scores NaN, which rank first, as torch.topk has it.  k <= 64, nb <= 256.  workspace: a device uint8
+    tensor of beam_select_workspace_bytes(...); by default one from torch's allocator."""
+    if not isinstance(logits, torch.Tensor) or not isinstance(scores, torch.Tensor):
+        raise TypeError("beam_select: logits and scores must be tensors")
+    if logits.device.type != "cuda" or scores.device != logits.device:
+        raise ValueError("beam_select: logits and scores must be on one GPU")
+    if logits.dtype not in (torch.bfloat16, torch.float32) or scores.dtype != torch.float32:
+        raise TypeError(f"beam_select: logits must be bf16 or fp32 and scores fp32, got {logits.dtype} and {scores.dtype}")
+    one = logits.dim() == 2
+    if one:
+        logits, scores = logits[None], scores[None] if scores.dim() == 1 else scores
+    if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]):
+        raise ValueError(f"beam_select: expected logits [B, nb, V] and scores [B, nb], got {tuple(logits.shape)} and "
+                         f"{tuple(scores.shape)}")
+    B, nb, V = logits.shape
+    if V > 1 and logits.stride(2) != 1 or nb > 1 and scores.stride(1) != 1:
+        raise ValueError("beam_select: the last dimensions must be contiguous")
+    need = beam_select_workspace_bytes(B, nb, V, k)
+    ws = workspace if workspace is not None else torch.empty(need, dtype=torch.uint8, device=logits.device)
+    if ws.device != logits.device or not ws.is_contiguous():
+        raise ValueError(f"beam_select: the workspace must be a contiguous tensor on {logits.device}")
+    value = torch.empty((B, k), dtype=torch.float32, device=logits.device)
+    beam = torch.empty((B, k), dtype=torch.int64, device=logits.device)
+    token = torch.empty((B, k), dtype=torch.int64, device=logits.device)
+    call_on(logits, "w8a8_beam_select", logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0,
+            logits.stride(0) if B > 1 else nb * V, logits.stride(1) if nb > 1 else V, scores.data_ptr(),
+            scores.stride(0) if B > 1 else nb, B, nb, V, int(k), value.data_ptr(), beam.data_ptr(), token.data_ptr(),
+            ws.data_ptr(), ws.numel() * ws.element_size(), _stream(logits))
+    return (value[0], beam[0], token[0]) if one else (value, beam, token)
 
 
 def rms_residual_norm(y, res, w1, w2, eps, scalar=None):

@@ -573,6 +573,82 @@ int w8a8_attention_tree_bf16(const uint16_t *q, int64_t q_head_stride, int64_t q
                              float scale, uint16_t *o, int64_t o_head_stride, int64_t o_row_stride, float *lse,
                              void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/* ---- a bounded cache, beams ---------------------------------------------------------------- */
+
+/* weights[g, j] += sum over the heads h of KV head g and the queries i that see key j of
+ *   exp(scale * q[h, i] . k[g, j] - lse[h, i]),
+ * the softmax weight that each key has drawn, with the logsumexp of the attention call on the same
+ * operands (w8a8_attention_ws_bf16, w8a8_attention_decode_bf16).  Query i stands at position q_start + i
+ * and sees keys j <= its position and, with a window W > 0, those less than W before it.  No counterpart
+ * in the reference; it is what w8a8_evict keeps rows by.
+ *   q bf16 [H, Tq, D], k bf16 [KV, Tk, D] (element strides), lse fp32 [H, Tq] (head stride; a query whose
+ *   lse is -inf saw nothing and adds nothing), weights fp32 [KV, Tk] (head stride), keys that no query
+ *   sees unchanged (or + 0)
+ *   q_start: 0 .. Tk - Tq; or -1 and q_start_dev, an int32 in device memory (Tq * H / KV <= 32: a decoded
+ *   token's rows), which the launch does not depend on
+ *   workspace: w8a8_attention_key_weights_workspace_bytes(...) bytes (-1: invalid; 0: none), 4-byte
+ *   aligned, scratch; calls that overlap in time need separate ones
+ * D in {128, 256, 512}; strides multiples of 8 elements; q and k 16-byte aligned.  fp32 scores and sums in
+ * a fixed order (deterministic).  One or two launches. */
+int64_t w8a8_attention_key_weights_workspace_bytes(int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D,
+                                                   int64_t q_start, int64_t window);
+int w8a8_attention_key_weights(const uint16_t *q, int64_t q_head_stride, int64_t q_row_stride, const uint16_t *k,
+                               int64_t k_head_stride, int64_t k_row_stride, const float *lse, int64_t lse_head_stride,
+                               int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D, int64_t q_start,
+                               const int32_t *q_start_dev, int64_t window, float scale, float *weights,
+                               int64_t weights_head_stride, void *workspace, int64_t workspace_bytes,
+                               hipStream_t stream);
+
+/* Cut a cache of n rows per KV head to `budget` rows, in place.  Kept are, per KV head, the rows whose
+ * position is within `recent` of the head's largest (position > largest - recent), then those of the
+ * largest weight; NaN counts as the largest weight, ties go to the lower row.  Kept rows below the budget
+ * stay; the others move, in row order, into the places that became free, in row order.  Rows at or past
+ * the budget are left as they were.  No counterpart in the reference, whose cache grows.
+ *   k / v: rows of row_bytes (a multiple of 16; any type), head and row strides in BYTES, 16-byte aligned
+ *   weights fp32 [KV, n], positions int32 [KV, n] (head strides in elements)
+ *   kept int32 [KV, budget]: the row that each row came from; weights_out, positions_out [KV, budget]: their
+ *   weights and positions (may be the first columns of weights / positions themselves, not otherwise
+ *   overlapping them)
+ *   workspace: w8a8_evict_workspace_bytes(KV, n, budget) bytes (-1: invalid), 4-byte aligned, scratch
+ * 1 <= budget <= n, 0 <= recent <= budget. */
+int64_t w8a8_evict_workspace_bytes(int64_t KV, int64_t n, int64_t budget);
+int w8a8_evict(void *k, int64_t k_head_stride, int64_t k_row_stride, void *v, int64_t v_head_stride,
+               int64_t v_row_stride, int64_t row_bytes, int64_t KV, int64_t n, const float *weights,
+               int64_t weights_stride, const int32_t *positions, int64_t positions_stride, int64_t budget,
+               int64_t recent, int32_t *kept, int64_t kept_stride, float *weights_out, int64_t weights_out_stride,
+               int32_t *positions_out, int64_t positions_out_stride, void *workspace, int64_t workspace_bytes,
+               hipStream_t stream);
+
+/* One tensor of w8a8_reorder_rows, strides in bytes: `outer` entries outer_stride apart, each with rows
+ * axis_stride apart, each row `runs` runs of run_bytes, run_stride apart. */
+typedef struct {
+  void *data;
+  int64_t outer_stride, axis_stride, run_stride, runs, run_bytes;
+} w8a8_rows;
+
+/* row[i] = row[index[i]] for i < n, in place, in every one of `count` tensors (a host array): the beams'
+ * keys and values put in the order a beam search step chose (index = w8a8_beam_select's beams), or the rows
+ * of an accepted path of drafted tokens moved up.  index int64 [n] in device memory, for all `outer`
+ * entries, or with index_stride > 0 [outer, n] of that row stride.  Rows 0 .. size - 1 can be taken, the
+ * first n <= 64 change; every row is read before any is written, so rows may be exchanged, repeated and
+ * dropped; an index outside 0 .. size - 1 leaves its row as it is.  Tensors must not overlap each other. */
+int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const int64_t *index, int64_t index_stride, int64_t n,
+                      int64_t size, int64_t outer, hipStream_t stream);
+
+/* A beam search step: per group of nb beams the k best of scores[i] + log_softmax(logits[i])[v], sorted, ties
+ * to the lowest i * V + v: their scores (fp32), beams and tokens (int64), [B, k] each, contiguous.
+ *   logits bf16 or fp32 [B, nb, V] (element strides of groups and beams), scores fp32 [B, nb] (group stride)
+ * Sums and ranking in 64 bits.  -inf logits are tokens that cannot follow; a beam whose score minus
+ * logsumexp is not finite (a score of -inf: a beam that is out; a NaN or +inf logit: NaN) gives that value
+ * to all its tokens, all -inf logits give -inf; NaN ranks first, as torch.topk has it.
+ * nb <= 256, k <= 64, k <= nb * V.  workspace: w8a8_beam_select_workspace_bytes(...) bytes (-1: invalid),
+ * 8-byte aligned, scratch.  Two launches, deterministic. */
+int64_t w8a8_beam_select_workspace_bytes(int64_t B, int64_t nb, int64_t V, int64_t k);
+int w8a8_beam_select(const void *logits, int logits_are_f32, int64_t group_stride, int64_t row_stride,
+                     const float *scores, int64_t score_stride, int64_t B, int64_t nb, int64_t V, int64_t k,
+                     float *out_scores, int64_t *out_beams, int64_t *out_tokens, void *workspace,
+                     int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
