@@ -24,9 +24,9 @@
 // Scores, softmax and sums are fp32; the softmax weights are rounded to bf16 for the second product, at
 // most 2^-9 of each weight, as the other attention kernels do.
 //
-// Values a row does not see never reach it: blocks that some row sees only in part (those at the window's
-// edge and the tree's own) are searched for infinities and NaN in V, and where there are any the product
-// runs over the weights that are not zero only, instead of the MFMA, whose 0 * inf would be NaN.
+// Values a row does not see never reach it: in the blocks that some row sees only in part (those at the
+// window's edge and the tree's own) infinities and NaN in V are replaced by zeros before the MFMA, whose
+// 0 * inf would be NaN, and added at the end to the rows that do see them.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -86,6 +86,7 @@ struct TreeShape {
   static constexpr int B_OFF = F_OFF + 2 * 16 * 4;   // the nodes' views [M][4]; depths [M]; chain ends [M]
   static constexpr int LDS = B_OFF + TREE_MAX_NODES * (TREE_WORDS + 2) * 4;
   static constexpr int NDW = D / NW / 16;            // 16-wide d tiles of O^T per wave
+  static constexpr int KR = 3;                       // K fragments in flight
 };
 
 // The nodes' views of the tree into LDS: bits[m] = the nodes on m's chain (none: unused), depth[m].  Every
@@ -232,14 +233,15 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     }
   }
   const bool live = (bits[0] | bits[1] | bits[2] | bits[3]) != 0u;
-  auto visible = [&](int key) __attribute__((always_inline)) {
+  // whether a node of this view and depth sees row `key`
+  auto sees = [&](const uint32_t(&b)[TREE_WORDS], int d, int key) __attribute__((always_inline)) {
     const int rel = key - past;
-    const uint32_t w = rel < 64 ? (rel < 32 ? bits[0] : bits[1]) : (rel < 96 ? bits[2] : bits[3]);
+    const uint32_t w = rel < 64 ? (rel < 32 ? b[0] : b[1]) : (rel < 96 ? b[2] : b[3]);
     const bool in_tree = (rel < M) & (((w >> (rel & 31)) & 1u) != 0u);
-    bool vis = live & ((rel < 0) | in_tree);
+    bool vis = ((b[0] | b[1] | b[2] | b[3]) != 0u) & ((rel < 0) | in_tree);
     if (win > 0) {
       const int kd = rel < 0 ? rel : depth_s[min(rel, TREE_MAX_NODES - 1)];  // the key's position - past
-      vis = vis & (depth - kd < win);
+      vis = vis & (d - kd < win);
     }
     return vis;
   };
@@ -261,20 +263,29 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     const char* kbase = lds + slot * S::KV_SLOT;
 #pragma unroll
     for (int t = 0; t < 2 * NKC; ++t) s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    // K fragments through a ring of KR registers: fragment i + KR is read once fragment i has fed its
+    // MFMA, so KR reads are in flight while the MFMAs run
+    constexpr int NR = NKK * 2 * NKC, KR = S::KR;
+    auto kfrag = [&](int i) __attribute__((always_inline)) {
+      const int kk = i / (2 * NKC), t = i % (2 * NKC);
+      const int row0 = 32 * (t >> 1) + 4 * (t & 1);
+      return *reinterpret_cast<const v8bf*>(kbase + kofs[kk % 4] + row0 * (KCH * 16) + (kk / 4) * 256);
+    };
+    v8bf kf[KR];
 #pragma unroll
-    for (int kk = 0; kk < NKK; ++kk)
+    for (int i = 0; i < KR; ++i) kf[i] = kfrag(i);
 #pragma unroll
-      for (int t = 0; t < 2 * NKC; ++t) {
-        const int row0 = 32 * (t >> 1) + 4 * (t & 1);
-        const v8bf a = *reinterpret_cast<const v8bf*>(kbase + kofs[kk % 4] + row0 * (KCH * 16) + (kk / 4) * 256);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[kk], s[t], 0, 0, 0);
-      }
+    for (int i = 0; i < NR; ++i) {
+      const int kk = i / (2 * NKC), t = i % (2 * NKC);
+      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % KR], qf[kk], s[t], 0, 0, 0);
+      if (i + KR < NR) kf[i % KR] = kfrag(i + KR);
+    }
     if (!inner(n)) {
 #pragma unroll
       for (int t = 0; t < 2 * NKC; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          s[t][i] = attn_mask(s[t][i], visible(kb0 + n * BN + 32 * (t >> 1) + 8 * qq + 4 * (t & 1) + i));
+          s[t][i] = attn_mask(s[t][i], sees(bits, depth, kb0 + n * BN + 32 * (t >> 1) + 8 * qq + 4 * (t & 1) + i));
     }
     float bm = -__builtin_inff();
 #pragma unroll
@@ -318,6 +329,7 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) o[dt][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const int vsrc = qq * 8 + (qi >> 2);  // this lane's V source row within a 32-key chunk (+4)
+  int found = 0;                        // infinities or NaN were taken out of V (the same for the workgroup)
   auto pv_phase = [&](int n) __attribute__((always_inline)) {
     const int slot = n & 1;
     int f = 0;
@@ -334,33 +346,23 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     const char* vl = lds + S::V_OFF + slot * S::KV_SLOT;
     const uint16_t* pl = reinterpret_cast<const uint16_t*>(lds + S::P_OFF + slot * S::P_SLOT);
     if (!inner(n)) {
-      // an infinity or a NaN anywhere in the block's V (the same for the workgroup)
-      uint32_t bad = 0;
+      // infinities and NaN in the block's V are taken out of the product (0 * inf would be NaN) and added
+      // at the end to the rows that see them
+      int bad = 0;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
-        const v4u w = *reinterpret_cast<const v4u*>(vl + (u * NT + tid) * 16);
+        v4u* const at = reinterpret_cast<v4u*>(lds + S::V_OFF + slot * S::KV_SLOT + (u * NT + tid) * 16);
+        v4u w = *at;
+        int b = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          bad |= uint32_t((w[e] & 0x7f80u) == 0x7f80u) | uint32_t((w[e] & 0x7f800000u) == 0x7f800000u);
+        for (int e = 0; e < 4; ++e) {
+          if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, b = 1;
+          if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, b = 1;
+        }
+        if (b) *at = w;
+        bad |= b;
       }
-      if (__syncthreads_or(int(bad))) {
-        for (int key = 0; key < BN; ++key)
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const float pe = bf16_to_f32(pl[(rt * 16 + qi) * PLD + key]);
-            if (pe == 0.0f) continue;  // not seen
-#pragma unroll
-            for (int dt = 0; dt < NDW; ++dt) {
-              const int d = wave * (D / NW) + 16 * dt + 4 * qq;
-              const v2u w = *reinterpret_cast<const v2u*>(vl + key * ROW + (((d >> 3) ^ (2 * (key & 3))) * 16) + (d & 7) * 2);
-              o[dt][rt][0] = __builtin_fmaf(pe, __uint_as_float(w[0] << 16), o[dt][rt][0]);
-              o[dt][rt][1] = __builtin_fmaf(pe, __uint_as_float(w[0] & 0xffff0000u), o[dt][rt][1]);
-              o[dt][rt][2] = __builtin_fmaf(pe, __uint_as_float(w[1] << 16), o[dt][rt][2]);
-              o[dt][rt][3] = __builtin_fmaf(pe, __uint_as_float(w[1] & 0xffff0000u), o[dt][rt][3]);
-            }
-          }
-        return;
-      }
+      found |= __syncthreads_or(bad);
     }
 #pragma unroll
     for (int ch = 0; ch < NKC; ++ch) {
@@ -402,13 +404,50 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
   __syncthreads();
   pv_phase(nblk - 1);
 
+  const int d_lane = wave * (D / NW) + 4 * qq;  // + 16 dt + i
+  if (found) {
+#pragma unroll 1
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = tile * R + rt * 16 + qi;
+      uint32_t b[TREE_WORDS] = {};
+      int d = 0;
+      if (r < p.rows) {
+        const int m = M - p.N + r / G;
+#pragma unroll
+        for (int w = 0; w < TREE_WORDS; ++w) b[w] = bits_s[m * TREE_WORDS + w];
+        d = depth_s[m];
+      }
+      v4f add[NDW];
+#pragma unroll
+      for (int dt = 0; dt < NDW; ++dt) add[dt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j = 0; j < nkeys; ++j) {
+        if (inner(j / BN) || !sees(b, d, kb0 + j)) continue;
+        const uint16_t* vp = p.v + int64_t(g) * p.vhs + int64_t(kb0 + j) * p.vrs + d_lane;
+#pragma unroll
+        for (int dt = 0; dt < NDW; ++dt) {
+          const v2u w = *reinterpret_cast<const v2u*>(vp + 16 * dt);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = (i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16;
+            if ((x & 0x7f800000u) == 0x7f800000u) add[dt][i] += __uint_as_float(x);
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        if (t == rt) {
+#pragma unroll
+          for (int dt = 0; dt < NDW; ++dt) o[dt][t] += add[dt];
+        }
+    }
+  }
+
   // An unused node's row: the last part, which holds the tree, marks it with a sum of -1.
   float lt = lanes4_sum(l);
   if (last_part && !live) {
     ms = -__builtin_inff();
     lt = -1.0f;
   }
-  const int d_lane = wave * (D / NW) + 4 * qq;  // + 16 dt + i
   if (geo.nparts > 1) {
     const int64_t base = (int64_t(g) * p.nparts + part) * p.rows;
 #pragma unroll
