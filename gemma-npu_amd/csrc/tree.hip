@@ -28,6 +28,7 @@
 // window's edge and the tree's own) infinities and NaN in V are replaced by zeros before the MFMA, whose
 // 0 * inf would be NaN, and added at the end to the rows that do see them.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 
@@ -81,17 +82,17 @@ struct TreeShape {
   static constexpr int KV_SLOT = BN * ROW;
   static constexpr int PLD = BN + 8;                 // padded P row, elements
   static constexpr int P_SLOT = R * PLD * 2;
-  static constexpr int V_OFF = 2 * KV_SLOT, P_OFF = 4 * KV_SLOT, A_OFF = P_OFF + 2 * P_SLOT;
-  static constexpr int F_OFF = A_OFF + 2 * R * 4;    // alpha [2][R]; flags [2][16]
-  static constexpr int B_OFF = F_OFF + 2 * 16 * 4;   // the nodes' views [M][4]; depths [M]; chain ends [M]
-  static constexpr int LDS = B_OFF + TREE_MAX_NODES * (TREE_WORDS + 2) * 4;
+  static constexpr int A_OFF = 2 * P_SLOT;           // P [2]; ..
+  static constexpr int F_OFF = A_OFF + 2 * R * 4;    // alpha [2][R]; flags [2][16], found [16]
+  static constexpr int B_OFF = F_OFF + 3 * 16 * 4;   // the nodes' views [M][4]; depths [M]; chain ends [M]
+  static constexpr int AUX = B_OFF + TREE_MAX_NODES * (TREE_WORDS + 2) * 4;
   static constexpr int NDW = D / NW / 16;            // 16-wide d tiles of O^T per wave
   static constexpr int KR = 3;                       // K fragments in flight
+  static constexpr bool SPLIT = D < 512 || RT < 4;   // a variable per slot (the others would spill)
 };
 
 // The nodes' views of the tree into LDS: bits[m] = the nodes on m's chain (none: unused), depth[m].  Every
-// chain's known length doubles each round (bits of the node its known part ends at are added), so a
-// drafted tree of depth 8 takes three rounds.
+// chain's known length doubles each round (the bits of the node its known part ends at are added).
 template <int NT>
 __device__ __forceinline__ void tree_resolve(const int32_t* parents, int M, uint32_t* bits, int* depth, int* end) {
   const int m = threadIdx.x;
@@ -108,7 +109,8 @@ __device__ __forceinline__ void tree_resolve(const int32_t* parents, int M, uint
     }
     end[m] = e;
   }
-  while (__syncthreads_or(on && e >= 0)) {  // (at most 7 rounds: every parent is before its node)
+  __syncthreads();
+  for (int known = 1; known < M; known *= 2) {
     int ne = e;
     if (on && e >= 0) {
 #pragma unroll
@@ -122,6 +124,7 @@ __device__ __forceinline__ void tree_resolve(const int32_t* parents, int M, uint
       end[m] = ne;
     }
     e = ne;
+    __syncthreads();
   }
   if (on) {
     int n = -1;
@@ -143,11 +146,28 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
   constexpr int KU = BN * KCH / NT;         // DMA instructions per thread per K or V block
   constexpr int NKK = D / 32;               // k-steps of S^T
   static_assert(KU * NT == BN * KCH && NDW >= 1 && RT <= NW && NT >= TREE_MAX_NODES, "tiling");
-  static_assert(S::LDS <= 160 * 1024, "LDS");
-  __shared__ __attribute__((aligned(1024))) char lds[S::LDS];
-  float* const alpha_s = reinterpret_cast<float*>(lds + S::A_OFF);
-  int* const flag_s = reinterpret_cast<int*>(lds + S::F_OFF);
-  uint32_t* const bits_s = reinterpret_cast<uint32_t*>(lds + S::B_OFF);
+  static_assert(4 * S::KV_SLOT + S::AUX <= 160 * 1024, "LDS");
+  // With SPLIT every slot is a variable of its own: from one array the compiler has a read of V wait for all
+  // the DMAs in flight, those into the other slot too, as it cannot tell the slots apart.
+  constexpr bool SPLIT = S::SPLIT;
+  __shared__ __attribute__((aligned(1024))) char k0[S::KV_SLOT], k1[S::KV_SLOT], v0[S::KV_SLOT], v1[S::KV_SLOT];
+  __shared__ __attribute__((aligned(1024))) char aux_s[S::AUX];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * S::KV_SLOT + S::AUX];
+  auto k_slot = [&](auto slot) __attribute__((always_inline)) -> char* {
+    if constexpr (SPLIT) return slot ? k1 : k0;
+    else return lds + slot * S::KV_SLOT;
+  };
+  auto v_slot = [&](auto slot) __attribute__((always_inline)) -> char* {
+    if constexpr (SPLIT) return slot ? v1 : v0;
+    else return lds + (2 + slot) * S::KV_SLOT;
+  };
+  char* aux;
+  if constexpr (SPLIT) aux = aux_s;
+  else aux = lds + 4 * S::KV_SLOT;
+  float* const alpha_s = reinterpret_cast<float*>(aux + S::A_OFF);
+  int* const flag_s = reinterpret_cast<int*>(aux + S::F_OFF);
+  int* const found_s = flag_s + 32;
+  uint32_t* const bits_s = reinterpret_cast<uint32_t*>(aux + S::B_OFF);
   int* const depth_s = reinterpret_cast<int*>(bits_s + TREE_MAX_NODES * TREE_WORDS);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -183,21 +203,22 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     koff[u] = uint32_t(row) * krs2 + uint32_t(cs ^ ((row & 3) | ((row >> 1) & 12))) * 16u;
     voff[u] = uint32_t(row) * vrs2 + uint32_t(cs ^ (2 * (row & 3))) * 16u;
   }
-  auto issue_k = [&](int n) __attribute__((always_inline)) {
-    char* base = lds + (n & 1) * S::KV_SLOT;
+  // block n goes to slot n % 2 (with SPLIT a type, so that each access names its slot's variable)
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 1>;
+  auto issue_k = [&](auto slot, int n) __attribute__((always_inline)) {
     const uint32_t rowoff = uint32_t(n * BN) * krs2;
 #pragma unroll
-    for (int u = 0; u < KU; ++u) attn_dma16(rk, base + (u * NW + wave) * 1024, rowoff + koff[u]);
+    for (int u = 0; u < KU; ++u) attn_dma16(rk, k_slot(slot) + (u * NW + wave) * 1024, rowoff + koff[u]);
   };
-  auto issue_v = [&](int n) __attribute__((always_inline)) {
-    char* base = lds + S::V_OFF + (n & 1) * S::KV_SLOT;
+  auto issue_v = [&](auto slot, int n) __attribute__((always_inline)) {
     const uint32_t rowoff = uint32_t(n * BN) * vrs2;
 #pragma unroll
-    for (int u = 0; u < KU; ++u) attn_dma16(rv, base + (u * NW + wave) * 1024, rowoff + voff[u]);
+    for (int u = 0; u < KU; ++u) attn_dma16(rv, v_slot(slot) + (u * NW + wave) * 1024, rowoff + voff[u]);
   };
 
-  issue_k(0);
-  issue_v(0);
+  issue_k(Even{}, 0);
+  issue_v(Even{}, 0);
   // Q (B operand: lane (qi, qq) holds q[row][32 kk + 8 qq .. + 7] of this wave's 16 rows)
   const int srow = 16 * (wave % RT) + qi;
   const int row = tile * R + srow;               // (node, head) row of the KV head
@@ -213,37 +234,50 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
       qf[kk] = __builtin_bit_cast(v8bf, t);
     }
   }
-  if (nblk > 1) issue_k(1);
+  if (nblk > 1) issue_k(Odd{}, 1);
 
   // Block n is seen whole by every row when its keys are all context inside every node's window.
   auto inner = [&](int n) __attribute__((always_inline)) {
     const int kb = kb0 + n * BN;
     return kb + BN <= past && (win <= 0 || kb > past + M - 1 - win);
   };
-  // this row's view of the tree, where the part has blocks that are not seen whole
+  // A row's view of the tree's rows, where the part has blocks that are not seen whole: the nodes on its
+  // chain, with a window those less than it deep below the node.
+  auto view = [&](int r, uint32_t(&bits)[TREE_WORDS], int& depth) __attribute__((always_inline)) {
+    const int m = M - p.N + r / G;
+#pragma unroll
+    for (int w = 0; w < TREE_WORDS; ++w) bits[w] = r < p.rows ? bits_s[m * TREE_WORDS + w] : 0u;
+    depth = r < p.rows ? depth_s[m] : 0;
+    if (win > 0 && win < M)
+#pragma unroll
+      for (int w = 0; w < TREE_WORDS; ++w)
+        for (uint32_t left = bits[w]; left; left &= left - 1) {
+          const int at = __builtin_ctz(left);
+          if (depth - depth_s[32 * w + at] >= win) bits[w] &= ~(1u << at);
+        }
+  };
   uint32_t bits[TREE_WORDS] = {};
   int depth = 0;
   if (!inner(0) || !inner(nblk - 1)) {
     tree_resolve<NT>(p.parents, M, bits_s, depth_s, depth_s + TREE_MAX_NODES);
-    if (valid) {
-      const int m = M - p.N + qnode;
-#pragma unroll
-      for (int w = 0; w < TREE_WORDS; ++w) bits[w] = bits_s[m * TREE_WORDS + w];
-      depth = depth_s[m];
-    }
+    view(row, bits, depth);
   }
   const bool live = (bits[0] | bits[1] | bits[2] | bits[3]) != 0u;
-  // whether a node of this view and depth sees row `key`
-  auto sees = [&](const uint32_t(&b)[TREE_WORDS], int d, int key) __attribute__((always_inline)) {
-    const int rel = key - past;
-    const uint32_t w = rel < 64 ? (rel < 32 ? b[0] : b[1]) : (rel < 96 ? b[2] : b[3]);
-    const bool in_tree = (rel < M) & (((w >> (rel & 31)) & 1u) != 0u);
-    bool vis = ((b[0] | b[1] | b[2] | b[3]) != 0u) & ((rel < 0) | in_tree);
-    if (win > 0) {
-      const int kd = rel < 0 ? rel : depth_s[min(rel, TREE_MAX_NODES - 1)];  // the key's position - past
-      vis = vis & (d - kd < win);
+  // The keys kb .. kb + 31 that a row of this view and depth sees, as bits: its context rows (position below
+  // `past`, within the window) and its nodes.
+  auto seen = [&](const uint32_t(&b)[TREE_WORDS], int d, int kb) __attribute__((always_inline)) {
+    auto word = [&](int w) { return w < 2 ? (w == 0 ? b[0] : b[1]) : w < 4 ? (w == 2 ? b[2] : b[3]) : 0u; };
+    const int off = kb - past;  // the first key's node, or minus the context rows from it on
+    uint32_t m = 0u;
+    if (off >= 0)
+      m = __builtin_amdgcn_alignbit(word((off >> 5) + 1), word(off >> 5), uint32_t(off & 31));
+    else {
+      const int n = -off;
+      m = n < 32 ? (b[0] << n) | ((1u << n) - 1u) : ~0u;
+      const int cut = win > 0 ? past + d - win + 1 - kb : 0;  // the first key inside the window
+      if (cut > 0) m &= cut < n ? (cut < 32 ? ~0u << cut : 0u) : (n < 32 ? ~0u << n : 0u);
     }
-    return vis;
+    return (b[0] | b[1] | b[2] | b[3]) != 0u ? m : 0u;
   };
 
   const int krow = 8 * (qi >> 2) + (qi & 3);
@@ -257,10 +291,9 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
   const float c = p.c;
 
   // S^T of block n, softmax, P rows and rescale factors into slot n % 2
-  auto s_phase = [&](int n) __attribute__((always_inline)) {
-    const int slot = n & 1;
+  auto s_phase = [&](auto slot, int n) __attribute__((always_inline)) {
     v4f s[2 * NKC];
-    const char* kbase = lds + slot * S::KV_SLOT;
+    const char* kbase = k_slot(slot);
 #pragma unroll
     for (int t = 0; t < 2 * NKC; ++t) s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     // K fragments through a ring of KR registers: fragment i + KR is read once fragment i has fed its
@@ -282,10 +315,11 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     }
     if (!inner(n)) {
 #pragma unroll
-      for (int t = 0; t < 2 * NKC; ++t)
+      for (int ch = 0; ch < NKC; ++ch) {
+        const uint32_t m = seen(bits, depth, kb0 + n * BN + 32 * ch) >> (8 * qq);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[t][i] = attn_mask(s[t][i], sees(bits, depth, kb0 + n * BN + 32 * (t >> 1) + 8 * qq + 4 * (t & 1) + i));
+        for (int e = 0; e < 8; ++e) s[2 * ch + (e >> 2)][e & 3] = attn_mask(s[2 * ch + (e >> 2)][e & 3], ((m >> e) & 1u) != 0u);
+      }
     }
     float bm = -__builtin_inff();
 #pragma unroll
@@ -300,7 +334,7 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     ms = grow ? bmc : ms;
     const float mref = ms == -__builtin_inff() ? 0.0f : ms;
     float bs = 0.0f;
-    uint16_t* prow = reinterpret_cast<uint16_t*>(lds + S::P_OFF + slot * S::P_SLOT) + srow * PLD + 8 * qq;
+    uint16_t* prow = reinterpret_cast<uint16_t*>(aux + slot * S::P_SLOT) + srow * PLD + 8 * qq;
 #pragma unroll
     for (int ch = 0; ch < NKC; ++ch) {
       v8bf pb;
@@ -330,8 +364,7 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
     for (int rt = 0; rt < RT; ++rt) o[dt][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const int vsrc = qq * 8 + (qi >> 2);  // this lane's V source row within a 32-key chunk (+4)
   int found = 0;                        // infinities or NaN were taken out of V (the same for the workgroup)
-  auto pv_phase = [&](int n) __attribute__((always_inline)) {
-    const int slot = n & 1;
+  auto pv_phase = [&](auto slot, int n) __attribute__((always_inline)) {
     int f = 0;
 #pragma unroll
     for (int w = 0; w < RT; ++w) f |= flag_s[slot * 16 + w];
@@ -343,15 +376,15 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
         for (int dt = 0; dt < NDW; ++dt) o[dt][rt] *= a;
       }
     }
-    const char* vl = lds + S::V_OFF + slot * S::KV_SLOT;
-    const uint16_t* pl = reinterpret_cast<const uint16_t*>(lds + S::P_OFF + slot * S::P_SLOT);
+    char* const vl = v_slot(slot);
+    const uint16_t* pl = reinterpret_cast<const uint16_t*>(aux + slot * S::P_SLOT);
     if (!inner(n)) {
       // infinities and NaN in the block's V are taken out of the product (0 * inf would be NaN) and added
       // at the end to the rows that see them
       int bad = 0;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
-        v4u* const at = reinterpret_cast<v4u*>(lds + S::V_OFF + slot * S::KV_SLOT + (u * NT + tid) * 16);
+        v4u* const at = reinterpret_cast<v4u*>(vl + (u * NT + tid) * 16);
         v4u w = *at;
         int b = 0;
 #pragma unroll
@@ -362,7 +395,11 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
         if (b) *at = w;
         bad |= b;
       }
-      found |= __syncthreads_or(bad);
+      const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+      if (lane == 0) found_s[wave] = any ? 1 : 0;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) found |= found_s[w];
     }
 #pragma unroll
     for (int ch = 0; ch < NKC; ++ch) {
@@ -391,37 +428,51 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
   else
     attn_wait_vmcnt<0>();
   __syncthreads();
-  s_phase(0);
-  for (int n = 0; n + 1 < nblk; ++n) {
+  s_phase(Even{}, 0);
+  auto step = [&](auto slot, auto other, int n) __attribute__((always_inline)) {
     attn_wait_vmcnt<0>();
     __syncthreads();  // P(n) of every row; K(n + 1) and V(n) in LDS; the other slots free
-    if (n + 2 < nblk) issue_k(n + 2);
-    issue_v(n + 1);
-    s_phase(n + 1);
-    pv_phase(n);
+    if (n + 2 < nblk) issue_k(slot, n + 2);
+    issue_v(other, n + 1);
+    s_phase(other, n + 1);
+    __builtin_amdgcn_sched_barrier(0);  // (the two phases' registers together spill)
+    pv_phase(slot, n);
+  };
+  auto last = [&](auto slot, int n) __attribute__((always_inline)) {
+    attn_wait_vmcnt<0>();
+    __syncthreads();
+    pv_phase(slot, n);
+  };
+  if constexpr (SPLIT) {
+    int n = 0;
+    for (; n + 2 < nblk; n += 2) {
+      step(Even{}, Odd{}, n);
+      step(Odd{}, Even{}, n + 1);
+    }
+    if (n + 1 < nblk) {
+      step(Even{}, Odd{}, n);
+      last(Odd{}, n + 1);
+    } else {
+      last(Even{}, n);
+    }
+  } else {
+    for (int n = 0; n + 1 < nblk; ++n) step(n & 1, (n + 1) & 1, n);
+    last((nblk - 1) & 1, nblk - 1);
   }
-  attn_wait_vmcnt<0>();
-  __syncthreads();
-  pv_phase(nblk - 1);
 
   const int d_lane = wave * (D / NW) + 4 * qq;  // + 16 dt + i
   if (found) {
 #pragma unroll 1
     for (int rt = 0; rt < RT; ++rt) {
       const int r = tile * R + rt * 16 + qi;
-      uint32_t b[TREE_WORDS] = {};
-      int d = 0;
-      if (r < p.rows) {
-        const int m = M - p.N + r / G;
-#pragma unroll
-        for (int w = 0; w < TREE_WORDS; ++w) b[w] = bits_s[m * TREE_WORDS + w];
-        d = depth_s[m];
-      }
+      uint32_t b[TREE_WORDS];
+      int d;
+      view(r, b, d);
       v4f add[NDW];
 #pragma unroll
       for (int dt = 0; dt < NDW; ++dt) add[dt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
       for (int j = 0; j < nkeys; ++j) {
-        if (inner(j / BN) || !sees(b, d, kb0 + j)) continue;
+        if (inner(j / BN) || !((seen(b, d, kb0 + (j & ~31)) >> (j & 31)) & 1u)) continue;
         const uint16_t* vp = p.v + int64_t(g) * p.vhs + int64_t(kb0 + j) * p.vrs + d_lane;
 #pragma unroll
         for (int dt = 0; dt < NDW; ++dt) {
@@ -569,16 +620,39 @@ struct TreePlan {
 static TreePlan tree_plan(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D, int64_t past,
                           int64_t window) {
   const int64_t rows = N * (H / KV);
-  TreePlan pl;
-  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
-  pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
   const int bn = D == 128 ? 64 : 32;
   const int64_t ctx = past >= 0 ? past : Tk - M;  // a length in device memory: the longest
   const int64_t span = (window > 0 && window - 1 < ctx ? window - 1 : ctx) + M;
-  pl.nblk = (span + bn - 1) / bn;
-  const int64_t np = attn_cu_count() / (KV * pl.ntiles);
-  pl.nparts = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(np, pl.nblk), TREE_MAX_PARTS)));
-  return pl;
+  TreePlan best{}, pl;
+  pl.nblk = best.nblk = (span + bn - 1) / bn;
+  // Of the row tiles and part counts that put a quarter of a workgroup to two workgroups on every CU, the
+  // one that a model of the call finishes first: each CU's key blocks, the start and the first block's way
+  // through memory, the tile's store, and the parts written and read back.  The times of a block
+  // (64 KiB of K and V at head_dim 512, 32 KiB else) are fitted to calls of 8 to 1024 rows over 700 to
+  // 65521 keys; small tiles read the keys more often, large ones leave more to be joined.  8 heads of
+  // 512, us at 16 / 32 / 64 / 128 rows a tile: 16 nodes over 3658 rows 20 / 21 / 24 / 31, over 32749 rows
+  // 58 / 43 / 39 / 45, 64 nodes over 32749 rows 198 / 121 / 91 / 73.
+  static const double block[3][4] = {{0.63, 0.75, 1.2, 1.6}, {0.55, 0.8, 1.15, 1.75}, {1.45, 1.7, 2.3, 3.2}};
+  const int di = D == 128 ? 0 : D == 256 ? 1 : 2;
+  const int64_t cus = attn_cu_count();
+  double least = 0.0;
+  for (int r = 0; r < 4; ++r) {
+    pl.rt = 1 << r;
+    if (r > 0 && rows <= 8 * pl.rt) break;  // half the tile holds them all
+    pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
+    const bool two = di < 2 && pl.rt <= (di == 0 ? 2 : 4);  // two workgroups fit a CU's LDS
+    for (int64_t quarters : {1, 2, 4, 8}) {
+      const int64_t want = std::max<int64_t>(1, quarters * cus / (4 * KV * pl.ntiles));
+      pl.nparts = int(std::min<int64_t>(std::min<int64_t>(want, pl.nblk), TREE_MAX_PARTS));
+      const int64_t wgs = KV * pl.ntiles * pl.nparts, per_cu = (wgs + cus - 1) / cus;
+      const double t = double((pl.nblk + pl.nparts - 1) / pl.nparts) * double(per_cu) * block[di][r] *
+                           (two && per_cu == 1 ? 1.25 : 1.0) +
+                       double(16 * pl.rt * D * 4) / 60e3 +
+                       (pl.nparts > 1 ? 1.5 + double(KV * rows * pl.nparts * D * 8) / 8e6 : 0.0);
+      if (best.rt == 0 || t < least) least = t, best = pl;
+    }
+  }
+  return best;
 }
 
 template <int D>
