@@ -69,7 +69,7 @@ __device__ __forceinline__ TreeGeom tree_geom(const TreeParams& p) {
   return t;
 }
 
-constexpr int tree_waves(int rt) { return rt == 8 ? 8 : 4; }
+constexpr int tree_waves(int rt) { return rt > 4 ? 8 : 4; }
 
 template <int D, int RT>
 struct TreeShape {
@@ -292,6 +292,7 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
 
   // S^T of block n, softmax, P rows and rescale factors into slot n % 2
   auto s_phase = [&](auto slot, int n) __attribute__((always_inline)) {
+    if (wave >= RT) return;
     v4f s[2 * NKC];
     const char* kbase = k_slot(slot);
 #pragma unroll
@@ -344,15 +345,13 @@ __global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeP
         bs += pe;
         pb[e] = (__bf16)pe;
       }
-      if (wave < RT) *reinterpret_cast<v8bf*>(prow + 32 * ch) = pb;
+      *reinterpret_cast<v8bf*>(prow + 32 * ch) = pb;
     }
     l = l * alpha + bs;
-    if (wave < RT) {
-      if (qq == 0) alpha_s[slot * R + srow] = alpha;
-      // a row whose maximum grew past a finite one needs its O rescaled (a row that had none has O = 0)
-      const bool any = __builtin_amdgcn_ballot_w64(grow && had) != 0;
-      if (lane == 0) flag_s[slot * 16 + wave] = any ? 1 : 0;
-    }
+    if (qq == 0) alpha_s[slot * R + srow] = alpha;
+    // a row whose maximum grew past a finite one needs its O rescaled (a row that had none has O = 0)
+    const bool any = __builtin_amdgcn_ballot_w64(grow && had) != 0;
+    if (lane == 0) flag_s[slot * 16 + wave] = any ? 1 : 0;
   };
 
   // O^T for columns [wave D/NW, (wave+1) D/NW) of all rows: o[dt][rt] register i of lane (qi, qq) is
@@ -629,22 +628,26 @@ static TreePlan tree_plan(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t T
   // one that a model of the call finishes first: each CU's key blocks, the start and the first block's way
   // through memory, the tile's store, and the parts written and read back.  The times of a block
   // (64 KiB of K and V at head_dim 512, 32 KiB else) are fitted to calls of 8 to 1024 rows over 700 to
-  // 65521 keys; small tiles read the keys more often, large ones leave more to be joined.  8 heads of
-  // 512, us at 16 / 32 / 64 / 128 rows a tile: 16 nodes over 3658 rows 20 / 21 / 24 / 31, over 32749 rows
-  // 58 / 43 / 39 / 45, 64 nodes over 32749 rows 198 / 121 / 91 / 73.
-  static const double block[3][4] = {{0.63, 0.75, 1.2, 1.6}, {0.55, 0.8, 1.15, 1.75}, {1.45, 1.7, 2.3, 3.2}};
+  // 65521 keys; small tiles read the keys more often, large ones leave more to be joined.  us at 16 / 32 /
+  // 64 / 80 / 96 / 128 rows a tile: 8 heads of 512, 16 nodes over 3658 rows 20 / 22 / 25 / 26 / 27 / 31, over
+  // 32749 rows 57 / 42 / 39 / 39 / 39 / 45, 64 nodes over 32749 rows 194 / 121 / 92 / - / - / 71; 32 heads of
+  // 128 on 8, 33 nodes over 65521 rows 163 / 114 / 131 / 96 / 103 / 112.
+  static const int tiles[6] = {1, 2, 4, 5, 6, 8};
+  static const double block[3][6] = {{0.63, 0.75, 1.2, 1.27, 1.4, 1.6}, {0.55, 0.8, 1.15, 1.3, 1.45, 1.75},
+                                     {1.45, 1.7, 2.3, 2.4, 2.5, 2.9}};
   const int di = D == 128 ? 0 : D == 256 ? 1 : 2;
-  const int64_t cus = attn_cu_count();
+  const int64_t xcd_cus = std::max(1, attn_cu_count() / 8);
   double least = 0.0;
-  for (int r = 0; r < 4; ++r) {
-    pl.rt = 1 << r;
-    if (r > 0 && rows <= 8 * pl.rt) break;  // half the tile holds them all
+  for (int r = 0; r < 6; ++r) {
+    pl.rt = tiles[r];
+    if (r > 0 && rows <= 16 * tiles[r - 1]) break;  // the tile before holds them all
     pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
     const bool two = di < 2 && pl.rt <= (di == 0 ? 2 : 4);  // two workgroups fit a CU's LDS
     for (int64_t quarters : {1, 2, 4, 8}) {
-      const int64_t want = std::max<int64_t>(1, quarters * cus / (4 * KV * pl.ntiles));
+      const int64_t pairs = std::max<int64_t>(1, quarters * xcd_cus / (4 * pl.ntiles));  // (KV head, part)s on an XCD
+      const int64_t want = std::max<int64_t>(1, pairs * 8 / KV);
       pl.nparts = int(std::min<int64_t>(std::min<int64_t>(want, pl.nblk), TREE_MAX_PARTS));
-      const int64_t wgs = KV * pl.ntiles * pl.nparts, per_cu = (wgs + cus - 1) / cus;
+      const int64_t wgs = (KV * pl.nparts + 7) / 8 * pl.ntiles, per_cu = (wgs + xcd_cus - 1) / xcd_cus;
       const double t = double((pl.nblk + pl.nparts - 1) / pl.nparts) * double(per_cu) * block[di][r] *
                            (two && per_cu == 1 ? 1.25 : 1.0) +
                        double(16 * pl.rt * D * 4) / 60e3 +
@@ -659,14 +662,14 @@ template <int D>
 static void tree_launch(const TreeParams& p, int rt, hipStream_t stream) {
   const unsigned pairs = unsigned(p.KV) * unsigned(p.nparts);
   const dim3 grid{(pairs + 7) / 8 * 8 * unsigned(p.ntiles), 1, 1};
-  if (rt == 1)
-    attn_tree_kernel<D, 1><<<grid, TreeShape<D, 1>::NT, 0, stream>>>(p);
-  else if (rt == 2)
-    attn_tree_kernel<D, 2><<<grid, TreeShape<D, 2>::NT, 0, stream>>>(p);
-  else if (rt == 4)
-    attn_tree_kernel<D, 4><<<grid, TreeShape<D, 4>::NT, 0, stream>>>(p);
-  else
-    attn_tree_kernel<D, 8><<<grid, TreeShape<D, 8>::NT, 0, stream>>>(p);
+  switch (rt) {
+    case 1: attn_tree_kernel<D, 1><<<grid, TreeShape<D, 1>::NT, 0, stream>>>(p); break;
+    case 2: attn_tree_kernel<D, 2><<<grid, TreeShape<D, 2>::NT, 0, stream>>>(p); break;
+    case 4: attn_tree_kernel<D, 4><<<grid, TreeShape<D, 4>::NT, 0, stream>>>(p); break;
+    case 5: attn_tree_kernel<D, 5><<<grid, TreeShape<D, 5>::NT, 0, stream>>>(p); break;
+    case 6: attn_tree_kernel<D, 6><<<grid, TreeShape<D, 6>::NT, 0, stream>>>(p); break;
+    default: attn_tree_kernel<D, 8><<<grid, TreeShape<D, 8>::NT, 0, stream>>>(p);
+  }
   if (p.nparts > 1)
     attn_tree_merge_kernel<D, TreeShape<D, 1>::BN>
         <<<dim3{unsigned(p.KV * p.rows), unsigned(D / 64), 1}, 256, 0, stream>>>(p);
@@ -686,6 +689,16 @@ extern "C" int64_t w8a8_attention_tree_workspace_bytes(int64_t H, int64_t KV, in
   if (!tree_shape_ok(H, KV, N, M, Tk, D, window) || n_past < -1 || n_past > Tk - M) return -1;
   const TreePlan pl = tree_plan(H, KV, N, M, Tk, D, n_past, window);
   return pl.nparts > 1 ? int64_t(H) * N * pl.nparts * (D + 2) * 4 : 0;
+}
+
+extern "C" int w8a8_attention_tree_plan(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D,
+                                        int64_t n_past, int64_t window, int* row_tile, int* parts) {
+  if (!tree_shape_ok(H, KV, N, M, Tk, D, window) || n_past < -1 || n_past > Tk - M)
+    return fail(W8A8_EINVAL, "attention_tree_plan: invalid arguments");
+  const TreePlan pl = tree_plan(H, KV, N, M, Tk, D, n_past, window);
+  if (row_tile) *row_tile = 16 * pl.rt;
+  if (parts) *parts = pl.nparts;
+  return W8A8_OK;
 }
 
 extern "C" int w8a8_attention_tree_bf16(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride,

@@ -100,6 +100,7 @@ SIGNATURES = {
     "w8a8_attention_decode_bf16": (_i32, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                           _i64, _f32, _p, _i64, _p, _p, _i64, _p]),
     "w8a8_attention_tree_workspace_bytes": (_i64, [_i64] * 8),
+    "w8a8_attention_tree_plan": (_i32, [_i64] * 8 + [_p, _p]),
     "w8a8_attention_tree_bf16": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                         _i64, _p, _i64, _p, _i64, _f32, _p, _i64, _i64, _p, _p, _i64, _p]),
     "w8a8_attention_key_weights_workspace_bytes": (_i64, [_i64] * 7),

@@ -566,6 +566,10 @@ int w8a8_attention_decode_qkv_dev_bf16(const uint16_t *y, const uint16_t *cos_, 
  * Deterministic.  One or two launches. */
 int64_t w8a8_attention_tree_workspace_bytes(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D,
                                             int64_t n_past, int64_t window);
+/* Diagnostic (for tests that must reach every form): the rows (node, head) per workgroup and the parts the keys
+ * are split into for these arguments. */
+int w8a8_attention_tree_plan(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D, int64_t n_past,
+                             int64_t window, int *row_tile, int *parts);
 int w8a8_attention_tree_bf16(const uint16_t *q, int64_t q_head_stride, int64_t q_row_stride, const uint16_t *k,
                              int64_t k_head_stride, int64_t k_row_stride, const uint16_t *v, int64_t v_head_stride,
                              int64_t v_row_stride, int64_t H, int64_t KV, int64_t N, int64_t M, int64_t Tk, int64_t D,

@@ -297,3 +297,50 @@ def test_refusals():
     many = torch.full((129,), -1, dtype=torch.int32, device=DEV)
     with pytest.raises((ValueError, W8A8Error)):
         attn.decode_tree(q, torch.cat([k, k], 1), torch.cat([v, v], 1), many, 10)
+
+
+PLANS = [
+    # H, KV, N, past, D, rows per workgroup, several parts
+    (16, 1, 33, 0, 128, 32, False), (1024, 64, 10, 0, 128, 64, False), (1024, 64, 20, 0, 128, 80, False), (384, 64, 64, 0, 128, 96, False),
+    (512, 32, 64, 0, 128, 128, False), (16, 1, 128, 0, 128, 64, True), (16, 1, 33, 2000, 128, 80, True), (10, 2, 33, 8000, 128, 96, True),
+    (256, 16, 33, 500, 128, 128, True), (32, 2, 33, 100, 256, 32, True), (16, 16, 33, 2000, 256, 64, True), (16, 1, 33, 2000, 256, 80, True),
+    (10, 2, 33, 8000, 256, 96, True), (24, 8, 33, 8000, 256, 128, True), (512, 32, 64, 0, 256, 128, False), (16, 1, 33, 0, 512, 32, True),
+    (1024, 64, 10, 0, 512, 64, False), (16, 1, 128, 0, 512, 64, True), (6, 1, 128, 2000, 512, 80, True), (10, 2, 33, 8000, 512, 96, True),
+    (24, 4, 33, 8000, 512, 128, True), (512, 32, 64, 0, 512, 128, False),
+]
+
+
+def plan(H, KV, N, M, Tk, D, past, window=0):
+    import ctypes
+
+    from w8a8 import _lib
+    tile, parts = ctypes.c_int(), ctypes.c_int()
+    assert _lib.lib().w8a8_attention_tree_plan(H, KV, N, M, Tk, D, past, window, ctypes.byref(tile), ctypes.byref(parts)) == 0
+    return tile.value, parts.value
+
+
+@pytest.mark.parametrize("case", PLANS, ids=lambda c: "x".join(map(str, c)))
+def test_every_row_tile(case):
+    """Each row tile of the plan, with one part of the keys and with several; a branch's V holds an infinity."""
+    H, KV, N, past, D, tile, several = case
+    got = plan(H, KV, N, N, past + N, D, past)
+    assert got[0] == tile and (got[1] > 1) == several, got
+    q, k, v = (t.to(DEV) for t in make(H, KV, N, past + N, D, seed=tile))
+    parents = random_tree(N, seed=N)
+    parents[-1] = -1
+    v[:, past + N - 1, 3] = math.inf    # the last node: a branch of its own
+    o, lse = attn.decode_tree(q, k, v, torch.tensor(parents, dtype=torch.int32, device=DEV), past, return_lse=True)
+    seen = torch.ones(N, past + N, dtype=torch.bool, device=DEV)
+    seen[:, past:] = False
+    for i in range(N):
+        seen[i, [past + c for c in chain_of(parents, i)]] = True
+    s = torch.matmul(q.double().view(KV, -1, D), k.double().transpose(1, 2).contiguous()).view(H, N, -1)
+    s = s.masked_fill(~seen, -math.inf)
+    rl = torch.logsumexp(s, -1)
+    p = torch.softmax(s, -1).view(KV, -1, past + N)
+    clean = v.double().clone()
+    clean[:, past + N - 1, 3] = 0.0
+    ro, mag = torch.matmul(p, clean).view(H, N, D), torch.matmul(p, clean.abs()).view(H, N, D)
+    assert torch.isinf(o[:, -1, 3]).all()
+    o[:, -1, 3] = ro[:, -1, 3].bfloat16()
+    check(o, lse, (ro.cpu(), mag.cpu(), rl.cpu()), str(case))
