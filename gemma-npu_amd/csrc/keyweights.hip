@@ -11,8 +11,8 @@
 // end, when 16 lanes are added.  No atomics: a key's sum is made by one workgroup, or (long prompts) by one
 // per part of the queries, and the parts are added in order, so the result does not depend on timing.
 //
-// The terms are made as exp2(log2 e (scale s - lse)) with the product's rounding error carried along: at
-// |scale s - lse| = 20 the plain product would be off by 2e-6 of the weight.
+// A term is exp2(s c - lse log2 e), c = scale log2 e held in two parts: rounded to one, c's error would be
+// the same sign for all keys (6e-8 of |s c|); the others are half a step of the argument, either way.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -29,21 +29,17 @@ struct KeyWeightParams {
   int key0;                             // first key of the launch
   float* part; int nparts, len;         // [nparts][KV][keys] partial sums of a split launch; row blocks per part
   int keys, nkb;                        // keys from key0 on, and blocks of them
-  float scale;
+  float c, c_lo;                        // scale * log2(e) = c + c_lo
 };
 
-__device__ __forceinline__ float key_weight(float s, float scale, float lse) {
-  constexpr float L2E = 1.44269502162933349609375f, L2E_LO = 1.925963033500011e-8f;  // log2 e in two parts
-  const float d = __builtin_fmaf(s, scale, -lse);
-  const float e = d * L2E;
-  const float r = __builtin_fmaf(d, L2E, -e) + d * L2E_LO;
-  // exp2(e + r) = exp2(e) (1 + r ln 2): r is below 2^-22 |e|
-  const float x = __builtin_amdgcn_exp2f(e);
-  return e > -200.0f ? __builtin_fmaf(x * 0.69314718055994531f, r, x) : x;  // (-inf: r is NaN)
+// log2 of a term: s c - lse log2 e, given minus the latter.
+__device__ __forceinline__ float key_weight_log2(float s, float c, float c_lo, float nl2) {
+  return __builtin_fmaf(s, c, __builtin_fmaf(s, c_lo, nl2));
 }
-
-// A query's logsumexp as a term's subtrahend: one that saw nothing (-inf) adds nothing.
-__device__ __forceinline__ float seen_lse(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse; }
+// -lse log2 e; a query that saw nothing (-inf) adds nothing.
+__device__ __forceinline__ float key_weight_ref(float lse) {
+  return lse == -__builtin_inff() ? lse : -lse * 1.4426950408889634f;
+}
 
 // v summed over the 16 lanes of a group (every lane gets the sum).
 __device__ __forceinline__ float lanes16_sum(float v) {
@@ -73,6 +69,10 @@ __global__ __launch_bounds__(256) void key_weights_few_kernel(KeyWeightParams p)
 #pragma unroll
   for (int kk = 0; kk < NKK; ++kk)
     kf[kk] = __builtin_bit_cast(v8bf, buf_load16(rk, uint32_t(qi) * krs2 + uint32_t(32 * kk + 8 * qq) * 2u));
+  // lane qi = e of group qq adds key 4 qq + e: its weight so far is asked for with the keys
+  float* const wp = p.w + int64_t(g) * p.whs + kb + 4 * qq + qi;
+  const bool mine = qi < 4 && 4 * qq + qi < nk;
+  const float before = mine ? *wp : 0.0f;
   const int rows = p.Tq * p.G;
   float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void key_weights_few_kernel(KeyWeightParams p)
     const bool valid = r < rows;
     const int i = valid ? r / p.G : 0, h = g * p.G + (valid ? r % p.G : 0);
     const uint16_t* qp = p.q + int64_t(h) * p.qhs + int64_t(i) * p.qrs + 8 * qq;
-    const float lse = valid ? seen_lse(p.lse[int64_t(h) * p.lhs + i]) : __builtin_inff();
+    const float nl2 = valid ? key_weight_ref(p.lse[int64_t(h) * p.lhs + i]) : -__builtin_inff();
     v4f s0 = v4f{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
@@ -99,27 +99,32 @@ __global__ __launch_bounds__(256) void key_weights_few_kernel(KeyWeightParams p)
     for (int e = 0; e < 4; ++e) {
       const int key = kb + 4 * qq + e;
       const bool vis = valid & (uint32_t(pos - key) < wlim);
-      w[e] += key_weight(attn_mask(s0[e] + s1[e], vis), p.scale, lse);
+      w[e] += __builtin_amdgcn_exp2f(attn_mask(key_weight_log2(s0[e] + s1[e], p.c, p.c_lo, nl2), vis));
     }
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = lanes16_sum(w[e]);
-  float* wp = p.w + int64_t(g) * p.whs + kb;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (qi == e && 4 * qq + e < nk) wp[4 * qq + e] += w[e];
+  if (mine) *wp = before + (qi < 2 ? (qi == 0 ? w[0] : w[1]) : (qi == 2 ? w[2] : w[3]));
 }
 
-// Many rows (prompts).  A wave holds 64 keys in registers as A operands for the whole launch, the four
-// waves of a workgroup 256; the queries of one head after the other pass through a two-slot LDS ring in
-// blocks of QB consecutive positions, each fragment read once per wave and fed to four MFMAs.  A part is a run
-// of (position block, head) pairs among those that see the key block.
+// Many rows (prompts).  A wave holds 16 KT keys in registers as A operands for the whole launch, the waves of
+// a workgroup 256; the queries of one head after the other pass through a two-slot LDS ring in blocks of QB
+// consecutive positions, each fragment read once per wave, KR of them ahead, and fed to KT MFMAs.  A part is a
+// run of (position block, head) pairs among those that see the key block.  At head_dim 512 eight waves of 32
+// keys, two a SIMD, whose products and exponentials overlap, beat four of 64 with half the LDS reads:
+// 205 -> 74 us for 3658 tokens of 8 heads (740 TFLOP/s; a large library product reaches 1210), 299 us for 8192
+// (919 TFLOP/s).  The LDS reads of the queries (as many cycles as the products) and the first load of the keys
+// bound it.
 template <int D>
 struct KeyWeightShape {
   static constexpr int QB = D == 128 ? 64 : 32;
   static constexpr int KB = 256;
+  static constexpr int KT = D == 512 ? 2 : 4;
+  static constexpr int NW = KB / (16 * KT);
+  static constexpr int KR = 8;
   static constexpr int SLOT = QB * D * 2;
 };
+constexpr int key_weight_threads(int d) { return d == 512 ? 512 : 256; }
 
 // Position blocks that see keys [kb, kb + 256): first and one past the last.
 template <int QB>
@@ -135,32 +140,37 @@ __host__ __device__ inline void key_weight_range(int kb, int start, int Tq, int 
 }
 
 template <int D>
-__global__ __launch_bounds__(256, D == 512 ? 1 : 2) void key_weights_kernel(KeyWeightParams p) {
+__global__ __launch_bounds__(key_weight_threads(D), D == 512 ? 1 : 2) void key_weights_kernel(KeyWeightParams p) {
   using S = KeyWeightShape<D>;
-  constexpr int QB = S::QB, NKK = D / 32, KCH = D / 8, ROW = D * 2;
-  constexpr int U = QB * KCH / 256;  // DMA instructions per thread per block
+  constexpr int QB = S::QB, NKK = D / 32, KCH = D / 8, ROW = D * 2, KT = S::KT, NW = S::NW, KR = S::KR, KEYS = 16 * KT;
+  constexpr int U = QB * KCH / (NW * 64);  // DMA instructions per thread per block
+  static_assert(NW * 64 == key_weight_threads(D) && U * NW * 64 == QB * KCH, "tiling");
   __shared__ __attribute__((aligned(1024))) char lds[2 * S::SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 15, qq = lane >> 4;
-  const int part = blockIdx.x % p.nparts, x = blockIdx.x / p.nparts;
-  const int g = x % p.KV, b = x / p.KV;
-  const int kb = p.key0 + b * S::KB, kw = kb + wave * 64;  // this workgroup's and wave's keys
-  int lo, hi;
-  key_weight_range<QB>(kb, p.start, p.Tq, p.window, lo, hi);
-  const int total = (hi - lo) * p.G;
-  const int np = max(1, (total + p.len - 1) / p.len);
-  if (part >= np) return;  // (the whole workgroup, before any barrier)
+  // workgroup x of KV head g: part x of the first key block's, or what is left of the next ones'
+  const int g = blockIdx.x % p.KV;
+  int part = blockIdx.x / p.KV, b = 0, lo, hi, total, np;
+  for (;; ++b) {
+    key_weight_range<QB>(p.key0 + b * S::KB, p.start, p.Tq, p.window, lo, hi);
+    total = (hi - lo) * p.G;
+    np = max(1, (total + p.len - 1) / p.len);
+    if (part < np) break;
+    part -= np;
+    if (b + 1 >= p.nkb) return;  // (never: the grid is the sum of the key blocks' parts)
+  }
+  const int kb = p.key0 + b * S::KB, kw = kb + wave * KEYS;  // this workgroup's and wave's keys
   const int n0 = int(int64_t(part) * total / np), n1 = int(int64_t(part + 1) * total / np);
 
   const int end = min(p.start + p.Tq, p.Tk);
-  const int nk = max(0, min(64, end - kw));
+  const int nk = max(0, min(KEYS, end - kw));
   const uint32_t krs2 = uint32_t(p.krs) * 2u, qrs2 = uint32_t(p.qrs) * 2u;
   const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + int64_t(g) * p.khs + int64_t(nk > 0 ? kw : 0) * p.krs,
                                               nk > 0 ? uint32_t(nk - 1) * krs2 + uint32_t(ROW) : 0u);
   uint32_t qoff[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int xc = (u * 4 + wave) * 64 + lane;
+    const int xc = (u * NW + wave) * 64 + lane;
     const int row = xc / KCH, cs = xc % KCH;
     qoff[u] = uint32_t(row) * qrs2 + uint32_t(cs ^ (row & 15)) * 16u;
   }
@@ -171,7 +181,7 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void key_weights_kernel(KeyW
                                                 uint32_t(min(QB, p.Tq - i0) - 1) * qrs2 + uint32_t(ROW));
     char* base = lds + ((n - n0) & 1) * S::SLOT;
 #pragma unroll
-    for (int u = 0; u < U; ++u) attn_dma16(rq, base + (u * 4 + wave) * 1024, qoff[u]);
+    for (int u = 0; u < U; ++u) attn_dma16(rq, base + (u * NW + wave) * 1024, qoff[u]);
 #pragma unroll
     for (int t = 0; t < QB / 16; ++t) {
       const int i = i0 + 16 * t + qi;
@@ -179,61 +189,76 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void key_weights_kernel(KeyW
     }
   };
   if (n0 < n1) fetch(n0);
-  v8bf kf[4][NKK];
+  v8bf kf[KT][NKK];
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk)
       kf[t][kk] = __builtin_bit_cast(
           v8bf, buf_load16(rk, uint32_t(16 * t + qi) * krs2 + uint32_t(32 * kk + 8 * qq) * 2u));
-  float w[4][4] = {};
+  float w[KT][4] = {};
   const uint32_t wlim = p.window > 0 ? uint32_t(p.window) : 0x80000000u;
+  const float c = p.c, c_lo = p.c_lo;
+  uint32_t qofs[4];  // this lane's fragment kk of a row lies at qofs[kk % 4] + 256 (kk / 4)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) qofs[j] = uint32_t(qi * ROW + ((4 * j + qq) ^ qi) * 16);
   for (int n = n0; n < n1; ++n) {
     attn_wait_vmcnt<0>();
     __syncthreads();  // block n is in LDS; the other slot is free
-    float lse[QB / 16];
+    float nl2[QB / 16];
 #pragma unroll
-    for (int t = 0; t < QB / 16; ++t) lse[t] = seen_lse(ln[t]);
+    for (int t = 0; t < QB / 16; ++t) nl2[t] = key_weight_ref(ln[t]);
     if (n + 1 < n1) fetch(n + 1);
     const char* base = lds + ((n - n0) & 1) * S::SLOT;
     const int p0 = p.start + (lo + n / p.G) * QB;  // the block's first position
-    const bool none = kw > p0 + QB - 1 || (p.window > 0 && int64_t(kw) + 63 <= int64_t(p0) - p.window);
+    const bool none = kw > p0 + QB - 1 || (p.window > 0 && int64_t(kw) + KEYS - 1 <= int64_t(p0) - p.window);
     if (none) continue;
-    const bool whole = kw + 63 <= p0 && (p.window <= 0 || kw > p0 + QB - 1 - p.window);
+    const bool whole = kw + KEYS - 1 <= p0 && (p.window <= 0 || kw > p0 + QB - 1 - p.window);
+    auto qfrag = [&](int i) __attribute__((always_inline)) {  // fragment kk = i % NKK of row tile i / NKK
+      const int kk = i % NKK;
+      return *reinterpret_cast<const v8bf*>(base + qofs[kk % 4] + (kk / 4) * 256 + (i / NKK) * (16 * ROW));
+    };
+    v8bf qf[KR];
+#pragma unroll
+    for (int i = 0; i < KR; ++i) qf[i] = qfrag(i);
 #pragma unroll
     for (int rt = 0; rt < QB / 16; ++rt) {
-      v4f s[4];
+      v4f s[KT];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      const char* qr = base + (16 * rt + qi) * ROW;
+      for (int t = 0; t < KT; ++t) s[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kk = 0; kk < NKK; ++kk) {
-        const v8bf q = *reinterpret_cast<const v8bf*>(qr + (((4 * kk + qq) ^ qi) * 16));
+        const int i = rt * NKK + kk;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], q, s[t], 0, 0, 0);
+        for (int t = 0; t < KT; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][kk], qf[i % KR], s[t], 0, 0, 0);
+        if (i + KR < QB / 16 * NKK) qf[i % KR] = qfrag(i + KR);
       }
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = key_weight_log2(s[t][e], c, c_lo, nl2[rt]);
       if (!whole) {
         const int pos = p0 + 16 * rt + qi;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             s[t][e] = attn_mask(s[t][e], uint32_t(pos - (kw + 16 * t + 4 * qq + e)) < wlim);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[t][e] += key_weight(s[t][e], p.scale, lse[rt]);
+        for (int e = 0; e < 4; ++e) w[t][e] += __builtin_amdgcn_exp2f(s[t][e]);
     }
   }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[t][e] = lanes16_sum(w[t][e]);
   // lane qi = 4 t + e of group qq holds key 16 t + 4 qq + e
   float v = 0.0f;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) v = qi == 4 * t + e ? w[t][e] : v;
   const int j = 16 * (qi >> 2) + 4 * qq + (qi & 3);
@@ -253,8 +278,16 @@ __global__ __launch_bounds__(256) void key_weights_add_kernel(KeyWeightParams p)
   key_weight_range<QB>(p.key0 + int(blockIdx.x) * 256, p.start, p.Tq, p.window, lo, hi);
   const int np = max(1, ((hi - lo) * p.G + p.len - 1) / p.len);
   float* wp = p.w + int64_t(g) * p.whs + p.key0 + j;
+  const float* pp = p.part + int64_t(g) * p.keys + j;
+  const int64_t step = int64_t(p.KV) * p.keys;
   float v = 0.0f;
-  for (int s = 0; s < np; ++s) v += p.part[(int64_t(s) * p.KV + g) * p.keys + j];
+  for (int s0 = 0; s0 < np; s0 += 16) {  // 16 loads in flight
+    float x[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) x[u] = s0 + u < np ? pp[(s0 + u) * step] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) v += x[u];
+  }
   *wp += v;
 }
 
@@ -265,6 +298,7 @@ constexpr int KEYW_FEW = 32;  // rows of the kernel that reads the queries from 
 struct KeyWeightPlan {
   bool few;
   int key0, keys, nkb, nparts, len;
+  int64_t wgs;  // parts of all key blocks
 };
 
 static int64_t key_weight_total(const KeyWeightPlan& pl, int64_t D, int64_t G, int64_t start, int64_t Tq, int64_t window,
@@ -293,19 +327,23 @@ static KeyWeightPlan key_weight_plan(int64_t H, int64_t KV, int64_t Tq, int64_t 
   pl.nkb = (pl.keys + 255) / 256;
   pl.nparts = 1;
   pl.len = 1;
+  pl.wgs = pl.nkb;
   if (pl.few) return pl;
-  // parts of so many row blocks that the chip takes them in whole rounds, each paying its keys' load
-  // (about four row blocks' time)
+  // Parts of so many row blocks that they fill the chip in whole rounds, each paying its keys' load (about
+  // four row blocks' time).  (The grid holds no workgroup without work: with empty ones between them an XCD
+  // got more than its CUs' share and the call took two rounds, 133 us for 3658 tokens of 8 heads of 512.)
   const int64_t slots = int64_t(attn_cu_count()) * (D == 512 ? 1 : 2);
   int most;
   const int64_t total = key_weight_total(pl, D, G, start, Tq, window, 1, &most) * KV;
   int64_t best = INT64_MAX;
   for (int64_t rounds = 1; rounds <= 6; ++rounds) {
-    const int64_t room = rounds * slots - int64_t(pl.nkb) * KV;  // (each key block's last part is not full)
-    const int64_t len = room > 0 ? (total + room - 1) / room : total;
-    const int64_t n = key_weight_total(pl, D, G, start, Tq, window, int(len), &most) * KV;
+    int64_t len = std::max<int64_t>(1, total / (rounds * slots)), n;
+    for (;; len += 1 + len / 32) {
+      n = key_weight_total(pl, D, G, start, Tq, window, int(len), &most) * KV;
+      if (n <= rounds * slots || n == int64_t(pl.nkb) * KV) break;
+    }
     const int64_t cost = (n + slots - 1) / slots * (len + 4);
-    if (cost < best) best = cost, pl.len = int(len), pl.nparts = most;
+    if (cost < best) best = cost, pl.len = int(len), pl.nparts = most, pl.wgs = n / KV;
   }
   return pl;
 }
@@ -337,7 +375,7 @@ static void key_weight_launch(KeyWeightParams& p, const KeyWeightPlan& pl, int64
       key_weights_few_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
     return;
   }
-  key_weights_kernel<D><<<dim3{unsigned(pl.nkb * p.KV * pl.nparts), 1, 1}, 256, 0, stream>>>(p);
+  key_weights_kernel<D><<<dim3{unsigned(pl.wgs * p.KV), 1, 1}, key_weight_threads(D), 0, stream>>>(p);
   if (pl.nparts > 1)
     key_weights_add_kernel<KeyWeightShape<D>::QB><<<dim3{unsigned(pl.nkb), unsigned(p.KV), 1}, 256, 0, stream>>>(p);
 }
@@ -382,7 +420,9 @@ extern "C" int w8a8_attention_key_weights(const uint16_t* q, int64_t q_head_stri
   p.q = q; p.qhs = hs[1]; p.qrs = rs[1]; p.k = k; p.khs = hs[0]; p.krs = rs[0]; p.lse = lse;
   p.lhs = H > 1 ? lse_head_stride : 0; p.w = weights; p.whs = KV > 1 ? weights_head_stride : 0;
   p.start_dev = q_start_dev; p.start = int(std::max<int64_t>(q_start, 0)); p.KV = int(KV); p.G = int(H / KV);
-  p.Tq = int(Tq); p.Tk = int(Tk); p.window = int(window); p.scale = scale;
+  p.Tq = int(Tq); p.Tk = int(Tk); p.window = int(window);
+  const double c = double(scale) * 1.4426950408889634;
+  p.c = float(c); p.c_lo = float(c - double(p.c));
   const KeyWeightPlan pl = key_weight_plan(H, KV, Tq, D, p.start, window);
   p.key0 = pl.key0; p.keys = pl.keys; p.nkb = pl.nkb; p.nparts = pl.nparts; p.len = pl.len;
   p.part = static_cast<float*>(workspace);
