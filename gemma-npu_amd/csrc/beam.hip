@@ -5,14 +5,15 @@
 // sorted, ties to the lowest i V + v.  Decode's greedy tail (the reference's loop, gemma_npu.py:292-295, takes
 // the argmax) for several sequences that are weighed against each other.
 //
-// beam_chunk_kernel reads the logits once.  A workgroup takes a run of BEAM_CHUNK logits of one beam into
-// registers, makes their maximum and sum of exponentials, and finds its k largest: the k-th largest of the
-// maxima of 64 lane groups is a bound that at least k logits reach and few more do, so those are listed and
-// ranked by counting.  Where too many reach it (equal logits, as a grammar's -inf), the k are taken one by
-// one instead.  Within a beam the order of logits is the order of scores, so nothing else can be among the
-// k best.  beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k
+// beam_chunk_kernel reads the logits once.  A workgroup takes a run of 256 E logits of one beam into registers,
+// makes their maximum and sum of exponentials, and finds its k largest: the k-th largest of the maxima of 64
+// lane groups is a bound that at least k logits reach and few more do, so those are listed and ranked by
+// counting.  Where too many reach it (equal logits, as a grammar's -inf), or there is a NaN, the k are taken
+// one by one instead.  Within a beam the order of logits is the order of scores, so nothing else can be among
+// the k best.  beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k
 // best of those lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and
-// the choice between them has to be right.
+// the choice between them has to be right.  The logits' way through memory bounds large calls (64 beams of
+// 262144 fp32 logits: 43 -> 30 us, 67 MB), two kernels' starts and barriers small ones (4 beams of bf16: 20 -> 15 us).
 #include <algorithm>
 
 #include "w8a8_common.h"
@@ -21,9 +22,8 @@ namespace w8a8 {
 
 constexpr int BEAM_MAX_K = 64;
 constexpr int BEAM_MAX_BEAMS = 256;
-constexpr int BEAM_E = 32;                  // logits per thread
-constexpr int BEAM_CHUNK = 256 * BEAM_E;
 constexpr int BEAM_LIST = 512;              // most candidates that are ranked by counting
+constexpr int BEAM_HELD = 8;                // candidates that a thread of the join keeps in registers
 
 struct BeamParams {
   const void* x; int64_t gs, rs;            // logits [B, nb, V] bf16 or fp32 (element strides of groups and beams)
@@ -48,17 +48,24 @@ __device__ __forceinline__ uint64_t order_bits(double x) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// The k-th largest of 64 lanes' values (k <= 64): the value whose rank, ties by lane, is k - 1.
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int j) { return uint32_t(__builtin_amdgcn_readlane(int(v), j)); }
+__device__ __forceinline__ float lane_value(float v, int j) { return __uint_as_float(lane_value(__float_as_uint(v), j)); }
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int j) {
+  return uint64_t(lane_value(uint32_t(v), j)) | (uint64_t(lane_value(uint32_t(v >> 32), j)) << 32);
+}
+
+// The k-th largest of 64 lanes' values (k <= 64, none of them NaN): the value whose rank, ties by lane, is k - 1.
 template <class T>
 __device__ __forceinline__ T wave_kth(T v, int k) {
   const int lane = threadIdx.x & 63;
   int rank = 0;
+#pragma unroll 16
   for (int j = 0; j < 64; ++j) {
-    const T o = __shfl(v, j, 64);
+    const T o = lane_value(v, j);
     rank += (o > v || (o == v && j < lane)) ? 1 : 0;
   }
   const uint64_t at = __builtin_amdgcn_ballot_w64(rank == k - 1);
-  return __shfl(v, __builtin_ctzll(at), 64);
+  return lane_value(v, __builtin_ctzll(at));
 }
 
 // A candidate before another: larger, or equal and of the lower index.
@@ -85,22 +92,23 @@ __device__ __forceinline__ void block_first(T& v, uint32_t& i, T* sv, uint32_t* 
     if (before(sv[w], si[w], v, i)) v = sv[w], i = si[w];
 }
 
-template <class X>
+template <class X, int E>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
+  constexpr int CHUNK = 256 * E;
   __shared__ uint32_t lv[BEAM_LIST], li[BEAM_LIST];
-  __shared__ uint32_t gmax[64];
-  __shared__ float red[4];
-  __shared__ uint32_t bound_s;
+  __shared__ float gmax[64];
+  __shared__ float red[4], red2[4];
+  __shared__ float bound_s;
   __shared__ int count;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int row = blockIdx.x / p.nch, ch = blockIdx.x % p.nch;
   const X* xp = static_cast<const X*>(p.x) + int64_t(row / p.nb) * p.gs + int64_t(row % p.nb) * p.rs;
-  const int base = ch * BEAM_CHUNK, n = min(BEAM_CHUNK, p.V - base);
-  // element e of thread t is logit base + 8 (t + 256 (e / 8)) + e % 8
-  float v[BEAM_E];
+  const int base = ch * CHUNK, n = min(CHUNK, p.V - base);
+  // element e of thread t is logit base + 8 (t + 256 (e / 8)) + e % 8; past the last one -inf
+  float v[E];
   const bool wide = (reinterpret_cast<uintptr_t>(xp) & 15) == 0;
 #pragma unroll
-  for (int c = 0; c < BEAM_E / 8; ++c) {
+  for (int c = 0; c < E / 8; ++c) {
     const int at = 8 * (t + 256 * c);
     const X* src = xp + base + at;
     if (wide && at + 8 <= n) {
@@ -117,7 +125,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float f = 0.0f;
+        float f = -__builtin_inff();
         if (at + e < n) {
           if constexpr (sizeof(X) == 2)
             f = bf16_to_f32(src[e]);
@@ -131,60 +139,58 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
   auto valid = [&](int e) __attribute__((always_inline)) { return 8 * (t + 256 * (e >> 3)) + (e & 7) < n; };
   auto index = [&](int e) __attribute__((always_inline)) { return uint32_t(base + 8 * (t + 256 * (e >> 3)) + (e & 7)); };
 
-  // maximum (without NaN: one makes the sum NaN) and sum of exponentials
+  // the maximum (fmaxf passes NaN over), and those of groups of four lanes
   float m = -__builtin_inff();
-  uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < BEAM_E; ++e)
-    if (valid(e)) {
-      m = fmaxf(m, v[e]);
-      top = max(top, order_bits(v[e]));
-    }
+  for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+  float mw = fmaxf(m, __shfl_xor(m, 1, 64));
+  mw = fmaxf(mw, __shfl_xor(mw, 2, 64));
+  if ((t & 3) == 0) gmax[t >> 2] = mw;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (lane == 0) red[wave] = m;
+  for (int o = 32; o >= 4; o >>= 1) mw = fmaxf(mw, __shfl_xor(mw, o, 64));
+  if (lane == 0) red[wave] = mw;
   if (t == 0) count = 0;
-  // the maxima of groups of four lanes
-  top = max(top, uint32_t(__shfl_xor(top, 1, 64)));
-  top = max(top, uint32_t(__shfl_xor(top, 2, 64)));
-  if ((t & 3) == 0) gmax[t >> 2] = top;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   if (wave == 0) {
-    const uint32_t b = wave_kth(gmax[lane], p.k);
+    const float b = wave_kth(gmax[lane], p.k);
     if (lane == 0) bound_s = b;
   }
-  const float mref = m == -__builtin_inff() ? 0.0f : m;
+  const float l2e = 1.4426950408889634f, mref = top == -__builtin_inff() ? 0.0f : top * l2e;
   float s = 0.0f;
 #pragma unroll
-  for (int e = 0; e < BEAM_E; ++e)
-    if (valid(e)) s += __expf(v[e] - mref);
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], l2e, -mref));
   s = wave_sum(s);
+  if (lane == 0) red2[wave] = s;
   __syncthreads();
-  if (lane == 0) red[wave] = s;
-  const uint32_t bound = bound_s;  // (0, below every logit, where fewer than k groups hold any)
+  s = (red2[0] + red2[1]) + (red2[2] + red2[3]);  // NaN with a NaN or +inf among the logits
+  // the sum against exp2(mref), a rounded exponent: against the maximum itself
+  const float scale = __builtin_amdgcn_exp2f(__builtin_fmaf(-top, l2e, mref));
+  const float bound = bound_s;  // (-inf where fewer than k groups hold any)
+  const bool plain = s == s && bound > -__builtin_inff();
+  if (plain && m >= bound) {
 #pragma unroll
-  for (int e = 0; e < BEAM_E; ++e)
-    if (valid(e) && order_bits(v[e]) >= bound) {
-      const int at = atomicAdd(&count, 1);
-      if (at < BEAM_LIST) lv[at] = order_bits(v[e]), li[at] = index(e);
-    }
+    for (int e = 0; e < E; ++e)
+      if (v[e] >= bound) {
+        const int at = atomicAdd(&count, 1);
+        if (at < BEAM_LIST) lv[at] = order_bits(v[e]), li[at] = index(e);
+      }
+  }
   __syncthreads();
   const int64_t slot = int64_t(row) * p.nch + ch;
-  if (t == 0) p.stat[slot] = make_float2(m, (red[0] + red[1]) + (red[2] + red[3]));
+  if (t == 0) p.stat[slot] = make_float2(top, top == -__builtin_inff() ? s : s * scale);
   uint2* out = p.cand + slot * p.k;
   const int nc = count;
   auto value = [&](uint32_t o) __attribute__((always_inline)) {  // the logit's bits again (NaN: the quiet one)
     return o == 0xffffffffu ? 0x7fc00000u : (o & 0x80000000u ? o & 0x7fffffffu : ~o);
   };
-  if (nc <= BEAM_LIST) {
+  if (plain && nc <= BEAM_LIST) {
     for (int j = t; j < nc; j += 256) {
       int rank = 0;
       const uint32_t a = lv[j], ai = li[j];
       for (int c = 0; c < nc; ++c) rank += before(lv[c], li[c], a, ai) ? 1 : 0;
       if (rank < p.k) out[rank] = make_uint2(value(a), ai);
     }
-    for (int j = nc + t; j < p.k; j += 256) out[j] = make_uint2(0u, 0xffffffffu);  // none
     return;
   }
   // one by one: the best after the last one taken
@@ -193,12 +199,12 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
   for (int j = 0; j < p.k; ++j) {
     uint32_t b = 0, bi = 0xffffffffu;
 #pragma unroll
-    for (int e = 0; e < BEAM_E; ++e) {
+    for (int e = 0; e < E; ++e) {
       const uint32_t o = order_bits(v[e]), i = index(e);
       if (valid(e) && (!any || before(last, lasti, o, i)) && before(o, i, b, bi)) b = o, bi = i;
     }
     block_first<uint32_t, 4>(b, bi, lv, li);
-    if (t == 0) out[j] = make_uint2(value(b), bi);
+    if (t == 0) out[j] = make_uint2(value(b), bi);  // (none left: token 0xffffffff)
     last = b, lasti = bi, any = true;
   }
 }
@@ -210,6 +216,12 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
   __shared__ int count;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int grp = blockIdx.x;
+  const int per = p.nch * p.k, total = p.nb * per;
+  const uint2* cand = p.cand + int64_t(grp) * p.nb * per;
+  // the first candidates are asked for before the beams' sums are made
+  uint2 held[BEAM_HELD];
+#pragma unroll
+  for (int u = 0; u < BEAM_HELD; ++u) held[u] = t + 1024 * u < total ? cand[t + 1024 * u] : make_uint2(0u, 0xffffffffu);
   if (t == 0) count = 0;
   // base[i] = score - logsumexp of beam i, one wave per beam
   for (int i = wave; i < p.nb; i += 16) {
@@ -232,13 +244,10 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     if (lane == 0) base_s[i] = b;
   }
   __syncthreads();
-  const int per = p.nch * p.k, total = p.nb * per;
-  const uint2* cand = p.cand + int64_t(grp) * p.nb * per;
-  // candidate j: its score's order bits and i V + v; false where there is none.  A beam whose base is not
-  // finite has that score for every token: its first tokens stand for it.
-  auto get = [&](int j, uint64_t& o, uint64_t& at) __attribute__((always_inline)) {
+  // a candidate's score's order bits and i V + v; false where there is none.  A beam whose base is not finite
+  // has that score for every token: its first tokens stand for it.
+  auto score = [&](int j, uint2 a, uint64_t& o, uint64_t& at) __attribute__((always_inline)) {
     const int i = j / per, c = j % per;
-    const uint2 a = cand[j];
     const double b = base_s[i];
     uint32_t tok = a.y;
     double sc = b + double(__uint_as_float(a.x));
@@ -250,8 +259,16 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     at = uint64_t(i) * uint64_t(p.V) + tok;
     return tok != 0xffffffffu;
   };
-  uint64_t top = 0;
-  for (int j = t; j < total; j += 1024) {
+  auto get = [&](int j, uint64_t& o, uint64_t& at) __attribute__((always_inline)) { return score(j, cand[j], o, at); };
+  uint64_t bits[BEAM_HELD], top = 0;  // (0, below every score: none)
+#pragma unroll
+  for (int u = 0; u < BEAM_HELD; ++u) {
+    uint64_t o = 0, at;
+    const int j = t + 1024 * u;
+    bits[u] = j < total && score(j, held[u], o, at) ? o : 0;
+    top = max(top, bits[u]);
+  }
+  for (int j = t + 1024 * BEAM_HELD; j < total; j += 1024) {
     uint64_t o, at;
     if (get(j, o, at)) top = max(top, o);
   }
@@ -267,37 +284,39 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     if (lane == 0) bound_s = b;
   }
   __syncthreads();
-  const uint64_t bound = bound_s;
-  for (int j = t; j < total; j += 1024) {
+  const uint64_t bound = max(bound_s, uint64_t(1));
+  auto list = [&](uint64_t o, int j) __attribute__((always_inline)) {
+    const int c = atomicAdd(&count, 1);
+    if (c < BEAM_LIST) lv[c] = o, li[c] = uint32_t(j);
+  };
+#pragma unroll
+  for (int u = 0; u < BEAM_HELD; ++u)
+    if (bits[u] >= bound) list(bits[u], t + 1024 * u);
+  for (int j = t + 1024 * BEAM_HELD; j < total; j += 1024) {
     uint64_t o, at;
-    if (get(j, o, at) && o >= bound) {
-      const int c = atomicAdd(&count, 1);
-      if (c < BEAM_LIST) lv[c] = o, li[c] = uint32_t(j);
-    }
+    if (get(j, o, at) && o >= bound) list(o, j);
   }
   __syncthreads();
   auto store = [&](int r, int j) __attribute__((always_inline)) {
     uint64_t o, at;
     get(j, o, at);
     const int i = j / per;
-    const uint64_t bits = o == ~0ull ? 0x7ff8000000000000ull : (o >> 63 ? o & 0x7fffffffffffffffull : ~o);
-    p.out_score[int64_t(grp) * p.k + r] = float(__longlong_as_double((long long)bits));
+    const uint64_t b = o == ~0ull ? 0x7ff8000000000000ull : (o >> 63 ? o & 0x7fffffffffffffffull : ~o);
+    p.out_score[int64_t(grp) * p.k + r] = float(__longlong_as_double((long long)b));
     p.out_beam[int64_t(grp) * p.k + r] = i;
     p.out_tok[int64_t(grp) * p.k + r] = int64_t(at - uint64_t(i) * uint64_t(p.V));
   };
   const int nc = count;
   if (nc <= BEAM_LIST) {
     for (int a = t; a < nc; a += 1024) {
-      uint64_t o, at, oo, oat;
+      uint64_t o, at;
       get(int(li[a]), o, at);
       int rank = 0;
       for (int c = 0; c < nc; ++c) {
-        if (lv[c] < o) continue;
-        oo = lv[c];
-        bool first = oo > o;
-        if (!first) {
-          uint64_t dummy;
-          get(int(li[c]), dummy, oat);
+        bool first = lv[c] > o;
+        if (lv[c] == o && c != a) {
+          uint64_t oo, oat;
+          get(int(li[c]), oo, oat);
           first = oat < at;
         }
         rank += first ? 1 : 0;
@@ -340,14 +359,21 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
 
 using namespace w8a8;
 
+// Logits per thread of the chunk kernel: 32, or 16 where that leaves CUs without a workgroup.
+static int beam_e(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) < 2 * 256 ? 16 : 32; }
+static int64_t beam_chunks(int64_t rows, int64_t V) {
+  const int64_t chunk = 256 * beam_e(rows, V);
+  return (V + chunk - 1) / chunk;
+}
+
 static bool beam_shape_ok(int64_t B, int64_t nb, int64_t V, int64_t k) {
-  return B >= 1 && nb >= 1 && nb <= BEAM_MAX_BEAMS && V >= 1 && V <= INT32_MAX / 2 && k >= 1 && k <= BEAM_MAX_K &&
-         k <= nb * V && B * nb <= INT32_MAX / ((V + BEAM_CHUNK - 1) / BEAM_CHUNK * BEAM_MAX_K);
+  return B >= 1 && B <= INT32_MAX && nb >= 1 && nb <= BEAM_MAX_BEAMS && V >= 1 && V <= INT32_MAX / 2 && k >= 1 &&
+         k <= BEAM_MAX_K && k <= nb * V && B * nb <= INT32_MAX / (beam_chunks(B * nb, V) * BEAM_MAX_K);
 }
 
 extern "C" int64_t w8a8_beam_select_workspace_bytes(int64_t B, int64_t nb, int64_t V, int64_t k) {
   if (!beam_shape_ok(B, nb, V, k)) return -1;
-  return B * nb * ((V + BEAM_CHUNK - 1) / BEAM_CHUNK) * 8 * (k + 1);
+  return B * nb * beam_chunks(B * nb, V) * 8 * (k + 1);
 }
 
 extern "C" int w8a8_beam_select(const void* logits, int logits_are_f32, int64_t group_stride, int64_t row_stride,
@@ -371,15 +397,17 @@ extern "C" int w8a8_beam_select(const void* logits, int logits_are_f32, int64_t 
   BeamParams p{};
   p.x = logits; p.gs = B > 1 ? group_stride : 0; p.rs = nb > 1 ? row_stride : 0;
   p.score = scores; p.ss = B > 1 ? score_stride : 0;
-  p.nb = int(nb); p.V = int(V); p.k = int(k); p.nch = int((V + BEAM_CHUNK - 1) / BEAM_CHUNK);
+  p.nb = int(nb); p.V = int(V); p.k = int(k); p.nch = int(beam_chunks(B * nb, V));
   p.stat = static_cast<float2*>(workspace);
   p.cand = reinterpret_cast<uint2*>(p.stat + B * nb * p.nch);
   p.out_score = out_scores; p.out_beam = out_beams; p.out_tok = out_tokens;
   const unsigned grid = unsigned(B * nb * p.nch);
+  const bool e16 = beam_e(B * nb, V) == 16;
   if (logits_are_f32)
-    beam_chunk_kernel<float><<<grid, 256, 0, stream>>>(p);
+    e16 ? beam_chunk_kernel<float, 16><<<grid, 256, 0, stream>>>(p) : beam_chunk_kernel<float, 32><<<grid, 256, 0, stream>>>(p);
   else
-    beam_chunk_kernel<uint16_t><<<grid, 256, 0, stream>>>(p);
+    e16 ? beam_chunk_kernel<uint16_t, 16><<<grid, 256, 0, stream>>>(p)
+        : beam_chunk_kernel<uint16_t, 32><<<grid, 256, 0, stream>>>(p);
   beam_join_kernel<<<unsigned(B), 1024, 0, stream>>>(p);
   return check_launch("beam_select");
 }

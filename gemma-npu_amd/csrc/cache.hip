@@ -35,28 +35,30 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
   int x = 0;
   while (x + 1 < p.ntensors && int(blockIdx.x) >= p.t[x + 1].block0) ++x;
   const ReorderTensor& d = p.t[x];
-  const int64_t col = int64_t(int(blockIdx.x) - d.block0) * 256 + threadIdx.x;
-  const int64_t per = d.run * d.ninner;
+  const uint32_t run = uint32_t(d.run), per = run * uint32_t(d.ninner);
+  const uint32_t col = uint32_t(int(blockIdx.x) - d.block0) * 256u + threadIdx.x;
+  if (col >= per) return;
   const int o = blockIdx.y;
-  const bool on = col < per;
-  char* base = d.base + int64_t(o) * d.outer + (on ? (col / d.run) * d.inner + (col % d.run) * int64_t(sizeof(C)) : 0);
+  const uint32_t in = d.ninner > 1 ? col / run : 0u;
+  char* base = d.base + int64_t(o) * d.outer + int64_t(in) * d.inner + int64_t(col - in * run) * int64_t(sizeof(C));
   const int64_t* index = p.index + int64_t(o) * p.is;
   C v[N];
-  int64_t src[N];
+  int src[N];  // (the same for the workgroup)
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     src[i] = i;
     if (i < p.n) {
       const int64_t s = index[i];
-      if (s >= 0 && s < p.size) src[i] = s;  // an index outside the axis leaves the row as it is
+      if (s >= 0 && s < p.size) src[i] = int(s);  // an index outside the axis leaves the row as it is
     }
+    src[i] = __builtin_amdgcn_readfirstlane(src[i]);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (src[i] != i && on) v[i] = *reinterpret_cast<const C*>(base + src[i] * d.axis);
+    if (src[i] != i) v[i] = *reinterpret_cast<const C*>(base + int64_t(src[i]) * d.axis);
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (src[i] != i && on) *reinterpret_cast<C*>(base + int64_t(i) * d.axis) = v[i];
+    if (src[i] != i) *reinterpret_cast<C*>(base + int64_t(i) * d.axis) = v[i];
 }
 
 // ---- a cache cut to its budget ---------------------------------------------------------------------------
@@ -66,19 +68,24 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
 // of the rows, so the kept rows below the budget stay where they are and the others move, in order, into
 // the places that became free: the least that can be moved, in place, and no row is both read and written.
 //
-// evict_select_kernel: one workgroup per KV head reads the weights and positions once into registers and
-// finds the budget-th largest key by a radix select over digits of 11, 11 and 10 bits; the first digit's
-// counting is the only one that all rows take part in.  Every wave owns a run of rows, so what comes before
-// it in row order is a sum over the waves before.  Up to EVICT_FUSED rows the waves then walk their rows with
-// ballots and list the free places and the moving rows; above that one workgroup per KV head would be walking
-// alone for long, so it leaves the sums before each segment of 1024 rows, and evict_list_kernel lists them
-// from a workgroup per segment.  evict_move_kernel copies the rows.  In all the keys are read by
-// one CU per head, which bounds the choice: 64 KiB rows of 8 heads 242 us reading them again at each step,
-// @SEL@
+// The budget-th largest key is found by a radix select over digits of 11, 11 and 10 bits.  What comes before a
+// row in row order (equal keys, free places, moving rows) is a sum over the waves or chunks before it and
+// ballots within, so ranks come out in row order.  Up to EVICT_ONE rows one workgroup per KV head does it all
+// from keys in LDS (evict_select_kernel).  Above that the rows are read by a workgroup per chunk of 4096:
+//   evict_newest_kernel  each chunk's newest position
+//   evict_digit_kernel   the keys' first digits counted per chunk
+//   evict_split_kernel   the first digit of the budget-th key from those counts; rows of larger digits are
+//                        counted, the keys of that digit listed, in row order
+//   evict_least_kernel   one workgroup per KV head finds the key among those, and what is before each chunk
+//   evict_list_kernel    the lists of free places and moving rows, chunk by chunk
+// and evict_move_kernel copies the rows.  Loops are not unrolled over a thread's rows: a workgroup runs
+// through such code once, and fetching it took longer than the work (65521 rows of 8 heads with the keys in
+// registers 84 us for the select alone, 242 us reading them again at each step; in chunks 34).
 
 constexpr int EVICT_NW = 16;
-constexpr int EVICT_SEG = 1024;            // rows per workgroup of evict_list_kernel
-constexpr int EVICT_FUSED = 1024 * 16;
+constexpr int EVICT_ONE = 16384;           // most rows of evict_select_kernel
+constexpr int EVICT_CHUNK = 4096;          // rows per workgroup of the others
+constexpr int EVICT_INFO = 6;              // words of a chunk's counts
 
 struct EvictParams {
   const float* w; int64_t whs;          // fp32 [KV, n]
@@ -90,10 +97,12 @@ struct EvictParams {
   int32_t* hole;                        // [KV][most] free places, ascending
   int32_t* mover;                       // [KV][most] rows that fill them, ascending
   int32_t* count;                       // [KV]
-  int32_t* head;                        // [KV][4] newest position - recent as two words, the least key kept, how many of it
-  int32_t* before;                      // [KV][nseg][3] equal keys, free places and moving rows before a segment
-  int most;                             // min(budget, n - budget)
-  int steps, nsub, nseg;                // steps of 64 rows per wave; segments per wave and per head
+  int32_t* least;                       // [KV][2] the least key kept, how many rows of it
+  int32_t* info;                        // [KV][nch][EVICT_INFO] a chunk's newest position; rows of larger digits below the
+                                        // budget and from it on, of the digit likewise; then what is before it
+  uint32_t* digit;                      // [KV][nch][1024] counts of two first digits each
+  uint32_t* open;                       // [KV][nch][4096] keys of the budget-th key's first digit
+  int most, nch;                        // min(budget, n - budget); chunks
   char* k; int64_t kh, kr;              // the cache's bytes: strides of heads and rows
   char* v; int64_t vh, vr;
   int row_cols;                         // 16-byte columns per row
@@ -107,292 +116,396 @@ __device__ __forceinline__ uint32_t evict_key(float w, int32_t pos, int64_t old)
   return int64_t(pos) > old ? 0xffffffffu : k;
 }
 
-// E rows per thread in registers (n <= 1024 E), or with E = 0 read again at each step.
-template <int E>
+__device__ __forceinline__ int evict_count(bool b) { return __popcll(__builtin_amdgcn_ballot_w64(b)); }
+__device__ __forceinline__ int evict_rank(bool b) {  // lanes before this one with b
+  return __popcll(__builtin_amdgcn_ballot_w64(b) & ((1ull << (threadIdx.x & 63)) - 1ull));
+}
+
+// v summed over the 16 waves before this one (buf [16], not in use by others until the next barrier after).
+__device__ __forceinline__ int evict_before(int v, int* buf) {
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) buf[wave] = v;
+  __syncthreads();
+  int s = 0;
+  for (int x = 0; x < EVICT_NW; ++x) s += x < wave ? buf[x] : 0;
+  return s;
+}
+
+// The digit that holds the need-th largest of the counted rows, and how many of its rows that leaves: thread t
+// of 1024 gives the counts c0 and c1 of digits 2047 - 2 t and 2046 - 2 t.
+__device__ __forceinline__ void evict_pick(int c0, int c1, int* red, uint32_t* digit_s, int* need_s, uint32_t& digit,
+                                           int& need) {
+  const int t = threadIdx.x, lane = t & 63, hi = 2047 - 2 * t;
+  int sum = c0 + c1;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += v;
+  }
+  const int total = __shfl(sum, 63, 64);
+  const int above = evict_before(total, red) + sum - c0 - c1;  // rows of larger digits
+  if (above < need && above + c0 >= need) *digit_s = uint32_t(hi), *need_s = need - above;
+  if (above + c0 < need && above + c0 + c1 >= need) *digit_s = uint32_t(hi - 1), *need_s = need - above - c0;
+  __syncthreads();
+  digit = *digit_s;
+  need = *need_s;
+}
+
+// The largest of v over the workgroup's 1024 threads.
+__device__ __forceinline__ int evict_max(int v, int* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  for (int x = 0; x < EVICT_NW; ++x) v = max(v, red[x]);
+  return v;
+}
+
 __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams p) {
-  constexpr bool LISTS = E > 0 && E <= 16;
-  constexpr int SEG_STEPS = EVICT_SEG / 64;
+  __shared__ uint32_t key[EVICT_ONE];
+  __shared__ int32_t ps[EVICT_ONE];
   __shared__ uint32_t hist[2048];
-  __shared__ int red[EVICT_NW], red2[EVICT_NW];
+  __shared__ int red[EVICT_NW], red2[EVICT_NW], red3[EVICT_NW];
   __shared__ uint32_t digit_s;
   __shared__ int need_s;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = blockIdx.x;
   const float* w = p.w + int64_t(g) * p.whs;
   const int32_t* pos = p.pos + int64_t(g) * p.phs;
-  const int n = p.n, budget = p.budget, steps = p.steps;
-  const int wave0 = wave * steps * 64, row0 = wave0 + lane;  // this wave's rows: steps of 64 from wave0 on
-
-  uint32_t key[E > 0 ? E : 1];
-  int32_t ps[LISTS ? E : 1];
-  int newest = INT32_MIN;
-  if constexpr (LISTS) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int r = row0 + 64 * e;
-      const bool ok = e < steps && r < n;
-      ps[e] = ok ? pos[r] : INT32_MIN;
-      key[e] = ok ? __float_as_uint(w[r]) : 0u;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) newest = max(newest, ps[e]);
-  } else {
-    for (int r = t; r < n; r += 8192) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (r + 1024 * u < n) newest = max(newest, pos[r + 1024 * u]);
-    }
-  }
+  const int n = p.n, budget = p.budget;
   hist[t] = 0u;
   hist[t + 1024] = 0u;
+  // the weights' bits and the positions into LDS while the newest is found
+  int newest = INT32_MIN;
+  for (int r0 = t; r0 < n; r0 += 4096) {
+    float x[4];
+    int32_t y[4];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, 64));
-  if (lane == 0) red[wave] = newest;
-  __syncthreads();
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + 1024 * u;
+      x[u] = r < n ? w[r] : 0.0f;
+      y[u] = r < n ? pos[r] : INT32_MIN;
+    }
 #pragma unroll
-  for (int x = 0; x < EVICT_NW; ++x) newest = max(newest, red[x]);
-  const int64_t old = int64_t(newest) - p.recent;
-  if constexpr (LISTS) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = evict_key(__uint_as_float(key[e]), ps[e], old);
-  } else if constexpr (E > 0) {
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(w, uint32_t(n) * 4u), rp = make_rsrc(pos, uint32_t(n) * 4u);
-    const int left = min(n, wave0 + steps * 64) - row0;  // this lane's rows are those of 64 e below it
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t off = uint32_t(row0 + 64 * e) * 4u;
-      const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rw, off, 0, 0));
-      const int32_t y = int32_t(__builtin_amdgcn_raw_buffer_load_b32(rp, off, 0, 0));
-      key[e] = 64 * e < left ? evict_key(x, y, old) : 0u;
-      if (e % 16 == 15) __builtin_amdgcn_sched_barrier(0);  // (all 128 loads at once would spill)
+    for (int u = 0; u < 4; ++u) {
+      if (r0 + 1024 * u < n) key[r0 + 1024 * u] = __float_as_uint(x[u]), ps[r0 + 1024 * u] = y[u];
+      newest = max(newest, y[u]);
     }
   }
-  // f(key, step) for each of this thread's rows, in order; the whole wave takes part in each step
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    if constexpr (E > 0) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e < steps) f(key[e], e);
-    } else {
-      for (int e0 = 0; e0 < steps; e0 += 8) {
-        uint32_t k[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int r = row0 + 64 * (e0 + u);
-          k[u] = e0 + u < steps && r < n ? evict_key(w[r], pos[r], old) : 0u;
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (e0 + u < steps) f(k[u], e0 + u);
-      }
-    }
-  };
-
-  // the budget-th largest key: its digits from the top, and how many of the rows with that key are kept
-  uint32_t prefix = 0;
+  newest = evict_max(newest, red);  // (its barrier: hist is cleared)
+  const int64_t old = int64_t(newest) - p.recent;
+#pragma unroll 2
+  for (int r = t; r < n; r += 1024) {
+    const uint32_t k = evict_key(__uint_as_float(key[r]), ps[r], old);
+    key[r] = k;
+    atomicAdd(&hist[k >> 21], 1u);
+  }
+  uint32_t prefix = 0, digit;
   int need = budget;
 #pragma unroll 1
   for (int d = 0; d < 3; ++d) {
     const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
-    const uint32_t digits = d == 2 ? 1023u : 2047u, mask = d == 0 ? 0u : d == 1 ? 0xffe00000u : 0xfffffc00u;
-    // (keys of no row are the smallest: they count in digits that are never reached)
-    each([&](uint32_t k, int) {
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1u);
-    });
+    if (d > 0) {
+      const uint32_t mask = d == 1 ? 0xffe00000u : 0xfffffc00u, digits = d == 1 ? 2047u : 1023u;
+#pragma unroll 4
+      for (int r = t; r < n; r += 1024)
+        if ((key[r] & mask) == prefix) atomicAdd(&hist[(key[r] >> shift) & digits], 1u);
+    }
     __syncthreads();
-    // thread t: digits hi and hi - 1; larger digits are with the threads before it
-    const int hi = 2047 - 2 * t;
-    const int c0 = int(hist[hi]), c1 = int(hist[hi - 1]);
+    const int hi = 2047 - 2 * t, c0 = int(hist[hi]), c1 = int(hist[hi - 1]);
     hist[hi] = 0u;
     hist[hi - 1] = 0u;
-    int above = c0 + c1;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(above, o, 64);
-      if (lane >= o) above += v;
-    }
-    if (lane == 63) red[wave] = above;
-    __syncthreads();
-    for (int x = 0; x < wave; ++x) above += red[x];
-    above -= c0 + c1;  // rows of larger digits
-    if (above < need && above + c0 >= need) digit_s = uint32_t(hi), need_s = need - above;
-    if (above + c0 < need && above + c0 + c1 >= need) digit_s = uint32_t(hi - 1), need_s = need - above - c0;
-    __syncthreads();
-    prefix |= digit_s << shift;
-    need = need_s;
+    evict_pick(c0, c1, red2, &digit_s, &need_s, digit, need);
+    prefix |= digit << shift;
   }
 
-  // sum over the waves before this one
-  auto scan = [&](int v, int* buf) __attribute__((always_inline)) {
-    if (lane == 0) buf[wave] = v;
-    __syncthreads();
-    int s = 0;
-    for (int x = 0; x < wave; ++x) s += buf[x];
-    return s;
-  };
-  if constexpr (LISTS) {
-    int neq = 0;
-    each([&](uint32_t k, int) { neq += __popcll(__builtin_amdgcn_ballot_w64(k == prefix)); });
-    int seen = scan(neq, red2);
-    const uint64_t below = (1ull << lane) - 1ull;
-    uint32_t keep_bits = 0;
-    int nhole = 0, nmove = 0;
-    each([&](uint32_t k, int e) {
-      const uint64_t b = __builtin_amdgcn_ballot_w64(k == prefix);
-      const bool keep = k > prefix || (k == prefix && seen + __popcll(b & below) < need);
-      seen += __popcll(b);
-      keep_bits |= keep ? 1u << e : 0u;
-      const bool low = row0 + 64 * e < budget;
-      nhole += __popcll(__builtin_amdgcn_ballot_w64(low && !keep));
-      nmove += __popcll(__builtin_amdgcn_ballot_w64(!low && keep));
-    });
-    __syncthreads();
-    int hole = scan(nhole, red), move = scan(nmove, red2);
-    int32_t* const holes = p.hole + int64_t(g) * p.most;
-    int32_t* const movers = p.mover + int64_t(g) * p.most;
-    int32_t* const ko = p.kept + int64_t(g) * p.khs;
-    float* const wo = p.w_out + int64_t(g) * p.wos;
-    int32_t* const po = p.pos_out + int64_t(g) * p.pos_os;
+  // wave w's rows: steps of 64 from w * steps * 64 on
+  const int steps = (n + 64 * EVICT_NW - 1) / (64 * EVICT_NW), row0 = wave * steps * 64 + lane;
+  int neq = 0;
+#pragma unroll 4
+  for (int e = 0; e < steps; ++e) {
+    const int r = row0 + 64 * e;
+    neq += evict_count(r < n && key[r] == prefix);
+  }
+  int seen = evict_before(neq, red3);
+  const int seen0 = seen;
+  int nhole = 0, nmove = 0;
+#pragma unroll 2
+  for (int e = 0; e < steps; ++e) {
+    const int r = row0 + 64 * e;
+    const uint32_t k = r < n ? key[r] : 0u;
+    const bool eq = r < n && k == prefix, low = r < budget;
+    const bool keep = r < n && (k > prefix || (eq && seen + evict_rank(eq) < need));
+    seen += evict_count(eq);
+    nhole += evict_count(low && !keep);
+    nmove += evict_count(!low && keep);
+  }
+  __syncthreads();
+  int hole = evict_before(nhole, red), move = evict_before(nmove, red2);
+  seen = seen0;
+  int32_t* const holes = p.hole + int64_t(g) * p.most;
+  int32_t* const movers = p.mover + int64_t(g) * p.most;
+  int32_t* const ko = p.kept + int64_t(g) * p.khs;
+  float* const wo = p.w_out + int64_t(g) * p.wos;
+  int32_t* const po = p.pos_out + int64_t(g) * p.pos_os;
+  for (int e0 = 0; e0 < steps; e0 += 4) {
+    float x[4];  // (the keys are not the weights' bits)
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e < steps) {
-        const int r = row0 + 64 * e;
-        const bool keep = (keep_bits >> e) & 1u, low = r < budget;
-        const uint64_t bh = __builtin_amdgcn_ballot_w64(low && !keep), bm = __builtin_amdgcn_ballot_w64(!low && keep);
-        if (low && !keep) holes[hole + __popcll(bh & below)] = r;
-        if (!low && keep) movers[move + __popcll(bm & below)] = r;
-        hole += __popcll(bh);
-        move += __popcll(bm);
-        if (low && keep) ko[r] = r, wo[r] = w[r], po[r] = ps[e];
-      }
-    if (wave == EVICT_NW - 1 && lane == 0) p.count[g] = hole;
-  } else {
-    // per segment of this wave: rows of larger keys and of equal ones, below the budget and from it on
-    int32_t* const bf = p.before + (int64_t(g) * p.nseg + wave * p.nsub) * 3;
-    int gt = 0, eq = 0, gt_low = 0, eq_low = 0;           // this lane's, of the segment so far
-    int all_eq = 0;                                       // the wave's
-    auto flush = [&](int j) __attribute__((always_inline)) {
-      int v[4] = {gt, eq, gt_low, eq_low};
+    for (int u = 0; u < 4; ++u) x[u] = row0 + 64 * (e0 + u) < budget ? w[row0 + 64 * (e0 + u)] : 0.0f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v[x] += __shfl_xor(v[x], o, 64);
-      // packed for the second round: (larger, equal) counts of the segment and of its part below the budget
-      if (lane == 0) bf[3 * j] = v[0] | (v[1] << 16), bf[3 * j + 1] = v[2] | (v[3] << 16);
-      all_eq += v[1];
-      gt = eq = gt_low = eq_low = 0;
-    };
-    each([&](uint32_t k, int e) {
-      const bool low = row0 + 64 * e < budget, a = k > prefix, b = k == prefix;
-      gt += a ? 1 : 0;
-      eq += b ? 1 : 0;
-      gt_low += a && low ? 1 : 0;
-      eq_low += b && low ? 1 : 0;
-      if (e % SEG_STEPS == SEG_STEPS - 1 || e == steps - 1) flush(e / SEG_STEPS);
-    });
-    int seen = scan(all_eq, red2);
-    // lane 0 turns the counts into the sums before each segment
-    int nhole = 0, nmove = 0;
-    if (lane == 0) {
-      int s = seen;
-      for (int j = 0; j < p.nsub; ++j) {
-        const int a = bf[3 * j], b = bf[3 * j + 1];
-        const int eqs = a >> 16, eql = b >> 16, first = wave0 + j * EVICT_SEG;
-        const int rows = max(0, min(min(EVICT_SEG, steps * 64 - j * EVICT_SEG), n - first));
-        const int low = max(0, min(rows, budget - first));
-        const int kept_low = (b & 0xffff) + max(0, min(eql, need - s));
-        const int kept = (a & 0xffff) + max(0, min(eqs, need - s));
-        bf[3 * j] = s;
-        bf[3 * j + 1] = nhole;
-        bf[3 * j + 2] = nmove;
-        s += eqs;
-        nhole += low - kept_low;
-        nmove += kept - kept_low;
-      }
+    for (int u = 0; u < 4; ++u) {
+      if (e0 + u >= steps) break;
+      const int r = row0 + 64 * (e0 + u);
+      const uint32_t k = r < n ? key[r] : 0u;
+      const bool eq = r < n && k == prefix, low = r < budget;
+      const bool keep = r < n && (k > prefix || (eq && seen + evict_rank(eq) < need));
+      seen += evict_count(eq);
+      if (low && !keep) holes[hole + evict_rank(low && !keep)] = r;
+      hole += evict_count(low && !keep);
+      if (!low && keep) movers[move + evict_rank(!low && keep)] = r;
+      move += evict_count(!low && keep);
+      if (low && keep) ko[r] = r, wo[r] = x[u], po[r] = ps[r];
     }
-    nhole = __builtin_amdgcn_readfirstlane(nhole);
-    nmove = __builtin_amdgcn_readfirstlane(nmove);
-    __syncthreads();
-    const int hole = scan(nhole, red), move = scan(nmove, red2);
-    if (lane == 0)
-      for (int j = 0; j < p.nsub; ++j) bf[3 * j + 1] += hole, bf[3 * j + 2] += move;
-    if (t == 0) {
-      int32_t* const h = p.head + 4 * g;
-      h[0] = int32_t(uint32_t(uint64_t(old)));
-      h[1] = int32_t(old >> 32);
-      h[2] = int32_t(prefix);
-      h[3] = need;
-    }
-    if (wave == EVICT_NW - 1 && lane == 0) p.count[g] = hole + nhole;
+  }
+  if (wave == EVICT_NW - 1 && lane == 0) p.count[g] = hole;
+}
+
+// A chunk's rows of thread t: chunk * 4096 + 256 (t / 64) + t % 64, + 64, + 128, + 192.
+struct EvictRows {
+  float w[4];
+  int32_t pos[4];
+  int row0;
+};
+__device__ __forceinline__ EvictRows evict_rows(const EvictParams& p, int g, int c) {
+  EvictRows x;
+  x.row0 = c * EVICT_CHUNK + 256 * int(threadIdx.x >> 6) + int(threadIdx.x & 63);
+  const float* w = p.w + int64_t(g) * p.whs;
+  const int32_t* pos = p.pos + int64_t(g) * p.phs;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = x.row0 + 64 * e;
+    x.w[e] = r < p.n ? w[r] : 0.0f;
+    x.pos[e] = r < p.n ? pos[r] : INT32_MIN;
+  }
+  return x;
+}
+// Rows of a position up to this one are not `recent`: from the chunks' newest.
+__device__ __forceinline__ int64_t evict_old(const EvictParams& p, int g, int* red) {
+  int newest = INT32_MIN;
+  for (int c = threadIdx.x; c < p.nch; c += 1024) newest = max(newest, p.info[(int64_t(g) * p.nch + c) * EVICT_INFO]);
+  return int64_t(evict_max(newest, red)) - p.recent;
+}
+
+__global__ __launch_bounds__(1024) void evict_newest_kernel(EvictParams p) {
+  __shared__ int red[EVICT_NW];
+  const int c = blockIdx.x, g = blockIdx.y;
+  const int32_t* pos = p.pos + int64_t(g) * p.phs;
+  int newest = INT32_MIN;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = c * EVICT_CHUNK + 1024 * e + int(threadIdx.x);
+    if (r < p.n) newest = max(newest, pos[r]);
+  }
+  newest = evict_max(newest, red);
+  if (threadIdx.x == 0) p.info[(int64_t(g) * p.nch + c) * EVICT_INFO] = newest;
+}
+
+__global__ __launch_bounds__(1024) void evict_digit_kernel(EvictParams p) {
+  __shared__ uint32_t hist[2048];
+  __shared__ int red[EVICT_NW];
+  const int t = threadIdx.x, c = blockIdx.x, g = blockIdx.y;
+  const EvictRows x = evict_rows(p, g, c);
+  hist[t] = 0u;
+  hist[t + 1024] = 0u;
+  const int64_t old = evict_old(p, g, red);  // (its barrier: hist is cleared)
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (x.row0 + 64 * e < p.n) atomicAdd(&hist[evict_key(x.w[e], x.pos[e], old) >> 21], 1u);
+  __syncthreads();
+  // word t: digits 2047 - 2 t (low half) and 2046 - 2 t
+  p.digit[(int64_t(g) * p.nch + c) * 1024 + t] = hist[2047 - 2 * t] | (hist[2046 - 2 * t] << 16);
+}
+
+__global__ __launch_bounds__(1024) void evict_split_kernel(EvictParams p) {
+  __shared__ int red[EVICT_NW], red2[EVICT_NW], sums[4];
+  __shared__ uint32_t digit_s;
+  __shared__ int need_s;
+  const int t = threadIdx.x, lane = t & 63, c = blockIdx.x, g = blockIdx.y;
+  const EvictRows x = evict_rows(p, g, c);
+  const int64_t old = evict_old(p, g, red);
+  int c0 = 0, c1 = 0;
+  const uint32_t* dg = p.digit + int64_t(g) * p.nch * 1024 + t;
+#pragma unroll 8
+  for (int i = 0; i < p.nch; ++i) {
+    const uint32_t v = dg[int64_t(i) * 1024];
+    c0 += int(v & 0xffffu);
+    c1 += int(v >> 16);
+  }
+  if (t < 4) sums[t] = 0;
+  uint32_t digit;
+  int need = p.budget;
+  evict_pick(c0, c1, red2, &digit_s, &need_s, digit, need);
+  // rows of larger digits are kept; those of the digit are left open, listed in row order
+  uint32_t key[4];
+  int nopen = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool ok = x.row0 + 64 * e < p.n;
+    key[e] = ok ? evict_key(x.w[e], x.pos[e], old) : 0u;
+    nopen += evict_count(ok && key[e] >> 21 == digit);
+  }
+  __syncthreads();  // (red2 has been read)
+  int at = evict_before(nopen, red2);
+  uint32_t* const open = p.open + (int64_t(g) * p.nch + c) * EVICT_CHUNK;
+  int cnt[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool ok = x.row0 + 64 * e < p.n, low = x.row0 + 64 * e < p.budget;
+    const bool is_open = ok && key[e] >> 21 == digit, above = ok && key[e] >> 21 > digit;
+    if (is_open) open[at + evict_rank(is_open)] = key[e];
+    at += evict_count(is_open);
+    cnt[0] += evict_count(above && low);
+    cnt[1] += evict_count(above && !low);
+    cnt[2] += evict_count(is_open && low);
+    cnt[3] += evict_count(is_open && !low);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane == 0) atomicAdd(&sums[i], cnt[i]);
+  __syncthreads();
+  int32_t* const info = p.info + (int64_t(g) * p.nch + c) * EVICT_INFO;
+  if (t < 4) info[1 + t] = sums[t];
+  if (c == 0 && t == 0) {
+    p.least[2 * g] = int32_t(digit);
+    p.least[2 * g + 1] = need;
   }
 }
 
-// The free places and moving rows of a segment, and the rows that stay.
-__global__ __launch_bounds__(256) void evict_list_kernel(EvictParams p) {
-  __shared__ int red[4], red2[4], red3[4];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, g = blockIdx.y, seg = blockIdx.x;
-  const int32_t* h = p.head + 4 * g;
-  const int64_t old = int64_t((uint64_t(uint32_t(h[1])) << 32) | uint32_t(h[0]));
-  const uint32_t least = uint32_t(h[2]);
-  const int need = h[3], budget = p.budget;
-  const int32_t* bf = p.before + (int64_t(g) * p.nseg + seg) * 3;
-  const int j = seg % p.nsub, run = p.steps * 64;
-  const int first = (seg / p.nsub) * run + j * EVICT_SEG;
-  const int end = min(first + min(EVICT_SEG, run - j * EVICT_SEG), p.n);  // one past the segment's rows
-  const float* w = p.w + int64_t(g) * p.whs;
-  const int32_t* pos = p.pos + int64_t(g) * p.phs;
-  const int row0 = first + wave * 256 + lane;
-  float wv[4];
-  int32_t pv[4];
+__global__ __launch_bounds__(1024) void evict_least_kernel(EvictParams p) {
+  __shared__ uint32_t hist[2048];
+  __shared__ int red[EVICT_NW];
+  __shared__ uint32_t digit_s;
+  __shared__ int need_s;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, g = blockIdx.x;
+  int32_t* const info = p.info + int64_t(g) * p.nch * EVICT_INFO;
+  const uint32_t* const open = p.open + int64_t(g) * p.nch * EVICT_CHUNK;
+  uint32_t prefix = uint32_t(p.least[2 * g]) << 21, digit;
+  int need = p.least[2 * g + 1];
+  hist[t] = 0u;
+  hist[t + 1024] = 0u;
+  __syncthreads();
+#pragma unroll 1
+  for (int d = 1; d < 3; ++d) {
+    const int shift = d == 1 ? 10 : 0;
+    const uint32_t mask = d == 1 ? 0u : 0x001ffc00u, digits = d == 1 ? 2047u : 1023u;
+    for (int c = wave; c < p.nch; c += EVICT_NW) {  // a wave per chunk
+      const int m = info[c * EVICT_INFO + 3] + info[c * EVICT_INFO + 4];
+#pragma unroll 4
+      for (int i = lane; i < m; i += 64) {
+        const uint32_t k = open[int64_t(c) * EVICT_CHUNK + i];
+        if ((k & mask) == (prefix & mask)) atomicAdd(&hist[(k >> shift) & digits], 1u);
+      }
+    }
+    __syncthreads();
+    const int hi = 2047 - 2 * t, c0 = int(hist[hi]), c1 = int(hist[hi - 1]);
+    hist[hi] = 0u;
+    hist[hi - 1] = 0u;
+    evict_pick(c0, c1, red, &digit_s, &need_s, digit, need);
+    prefix |= digit << shift;
+    __syncthreads();
+  }
+  // of each chunk: kept rows below the budget and from it on but for the equal ones, and those
+  for (int c = wave; c < p.nch; c += EVICT_NW) {
+    int32_t* const x = info + c * EVICT_INFO;
+    const int nlow = x[3], m = nlow + x[4];
+    int gl = 0, gh = 0, el = 0, eh = 0;
+#pragma unroll 4
+    for (int i0 = 0; i0 < m; i0 += 64) {
+      const int i = i0 + lane;
+      const uint32_t k = i < m ? open[int64_t(c) * EVICT_CHUNK + i] : 0u;
+      const bool low = i < nlow, gt = i < m && k > prefix, eq = i < m && k == prefix;
+      gl += evict_count(gt && low);
+      gh += evict_count(gt && !low);
+      el += evict_count(eq && low);
+      eh += evict_count(eq && !low);
+    }
+    if (lane == 0) x[1] += gl, x[2] += gh, x[3] = el, x[4] = eh;
+  }
+  __threadfence_block();
+  __syncthreads();
+  // what is before each chunk: one thread, over the chunks (their counts asked for eight at a time)
+  if (t != 0) return;
+  int eq = 0, hole = 0, move = 0;
+  for (int c0 = 0; c0 < p.nch; c0 += 8) {
+    int x[8][4];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[u][i] = c0 + u < p.nch ? info[(c0 + u) * EVICT_INFO + 1 + i] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int c = c0 + u;
+      if (c >= p.nch) break;
+      const int first = c * EVICT_CHUNK, rows = min(EVICT_CHUNK, p.n - first), low = max(0, min(rows, p.budget - first));
+      int32_t* const o = info + c * EVICT_INFO;
+      o[3] = eq;
+      o[4] = hole;
+      o[5] = move;
+      const int take_low = max(0, min(x[u][2], need - eq));
+      eq += x[u][2];
+      const int take_high = max(0, min(x[u][3], need - eq));
+      eq += x[u][3];
+      hole += low - x[u][0] - take_low;
+      move += x[u][1] + take_high;
+    }
+  }
+  p.least[2 * g] = int32_t(prefix);
+  p.least[2 * g + 1] = need;
+  p.count[g] = hole;
+}
+
+__global__ __launch_bounds__(1024) void evict_list_kernel(EvictParams p) {
+  __shared__ int red[EVICT_NW], red2[EVICT_NW], red3[EVICT_NW], red4[EVICT_NW];
+  const int c = blockIdx.x, g = blockIdx.y, budget = p.budget;
+  const EvictRows x = evict_rows(p, g, c);
+  const int64_t old = evict_old(p, g, red);
+  const uint32_t least = uint32_t(p.least[2 * g]);
+  const int need = p.least[2 * g + 1];
+  const int32_t* const info = p.info + (int64_t(g) * p.nch + c) * EVICT_INFO;
   uint32_t key[4];
   int neq = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int r = row0 + 64 * e;
-    wv[e] = r < end ? w[r] : 0.0f;
-    pv[e] = r < end ? pos[r] : 0;
+    const bool ok = x.row0 + 64 * e < p.n;
+    key[e] = ok ? evict_key(x.w[e], x.pos[e], old) : 0u;
+    neq += evict_count(ok && key[e] == least);
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const bool ok = row0 + 64 * e < end;
-    key[e] = ok ? evict_key(wv[e], pv[e], old) : 0u;
-    neq += __popcll(__builtin_amdgcn_ballot_w64(ok && key[e] == least));
-  }
-  if (lane == 0) red[wave] = neq;
-  __syncthreads();
-  int seen = bf[0];
-  for (int x = 0; x < wave; ++x) seen += red[x];
-  const uint64_t below = (1ull << lane) - 1ull;
+  int seen = info[3] + evict_before(neq, red2);
   bool keep[4];
   int nhole = 0, nmove = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int r = row0 + 64 * e;
-    const bool ok = r < end, low = r < budget;
-    const uint64_t b = __builtin_amdgcn_ballot_w64(ok && key[e] == least);
-    keep[e] = ok && (key[e] > least || (key[e] == least && seen + __popcll(b & below) < need));
-    seen += __popcll(b);
-    nhole += __popcll(__builtin_amdgcn_ballot_w64(ok && low && !keep[e]));
-    nmove += __popcll(__builtin_amdgcn_ballot_w64(!low && keep[e]));
+    const int r = x.row0 + 64 * e;
+    const bool ok = r < p.n, eq = ok && key[e] == least, low = r < budget;
+    keep[e] = ok && (key[e] > least || (eq && seen + evict_rank(eq) < need));
+    seen += evict_count(eq);
+    nhole += evict_count(low && !keep[e]);
+    nmove += evict_count(!low && keep[e]);
   }
-  if (lane == 0) red2[wave] = nhole, red3[wave] = nmove;
-  __syncthreads();
-  int hole = bf[1], move = bf[2];
-  for (int x = 0; x < wave; ++x) hole += red2[x], move += red3[x];
+  int hole = info[4] + evict_before(nhole, red3), move = info[5] + evict_before(nmove, red4);
   int32_t* const holes = p.hole + int64_t(g) * p.most;
   int32_t* const movers = p.mover + int64_t(g) * p.most;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int r = row0 + 64 * e;
-    const bool ok = r < end, low = r < budget;
-    const uint64_t bh = __builtin_amdgcn_ballot_w64(ok && low && !keep[e]), bm = __builtin_amdgcn_ballot_w64(!low && keep[e]);
-    if (ok && low && !keep[e]) holes[hole + __popcll(bh & below)] = r;
-    if (!low && keep[e]) movers[move + __popcll(bm & below)] = r;
-    hole += __popcll(bh);
-    move += __popcll(bm);
+    const int r = x.row0 + 64 * e;
+    const bool low = r < budget, is_hole = low && !keep[e], is_move = !low && keep[e];
+    if (is_hole) holes[hole + evict_rank(is_hole)] = r;
+    if (is_move) movers[move + evict_rank(is_move)] = r;
+    hole += evict_count(is_hole);
+    move += evict_count(is_move);
     if (low && keep[e]) {
       p.kept[int64_t(g) * p.khs + r] = r;
-      p.w_out[int64_t(g) * p.wos + r] = wv[e];
-      p.pos_out[int64_t(g) * p.pos_os + r] = pv[e];
+      p.w_out[int64_t(g) * p.wos + r] = x.w[e];
+      p.pos_out[int64_t(g) * p.pos_os + r] = x.pos[e];
     }
   }
 }
@@ -424,13 +537,13 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
 
 using namespace w8a8;
 
+// (No kernel of 8 rows: the compiler makes a path for every set of rows that move, at 222 registers, and the 16
+// rows' kernel is faster: 8 beams of 8191 rows, four layers, 204 -> 158 us.)
 template <class C>
 static void reorder_launch(const ReorderParams& p, int64_t blocks, hipStream_t stream) {
   const dim3 grid{unsigned(blocks), unsigned(p.nouter), 1};
   if (p.n <= 4)
     reorder_kernel<C, 4><<<grid, 256, 0, stream>>>(p);
-  else if (p.n <= 8)
-    reorder_kernel<C, 8><<<grid, 256, 0, stream>>>(p);
   else if (p.n <= 16)
     reorder_kernel<C, 16><<<grid, 256, 0, stream>>>(p);
   else if (p.n <= 32)
@@ -477,7 +590,7 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
       d.axis = r.axis_stride; d.outer = r.outer_stride; d.inner = r.run_stride;
       d.run = r.run_bytes / align; d.ninner = int(r.runs);
       const int64_t b = (d.run * d.ninner + 255) / 256;
-      if (b > INT32_MAX / 2) return fail(W8A8_ENOTSUP, "%s: tensor %lld too large", what, (long long)i0);
+      if (d.run * d.ninner > INT32_MAX) return fail(W8A8_ENOTSUP, "%s: tensor %lld too large", what, (long long)i0);
       if (blocks + b > INT32_MAX / 2) break;
       d.block0 = int(blocks);
       blocks += b;
@@ -494,15 +607,12 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
   return check_launch(what);
 }
 
-// Steps of 64 rows that each wave of the selection owns, and segments of the lists.
-static int evict_steps(int64_t n) { return int((n + 64 * EVICT_NW - 1) / (64 * EVICT_NW)); }
-static int evict_segments(int64_t n) {
-  return n <= EVICT_FUSED ? 0 : EVICT_NW * ((evict_steps(n) * 64 + EVICT_SEG - 1) / EVICT_SEG);
-}
+// Chunks of a head's rows (0: one workgroup chooses).
+static int64_t evict_chunks(int64_t n) { return n <= EVICT_ONE ? 0 : (n + EVICT_CHUNK - 1) / EVICT_CHUNK; }
 
 extern "C" int64_t w8a8_evict_workspace_bytes(int64_t KV, int64_t n, int64_t budget) {
   if (KV < 1 || KV > 65535 || n < 1 || n > INT32_MAX / 2 || budget < 1 || budget > n) return -1;
-  return KV * (5 + 2 * std::min(budget, n - budget) + 3 * int64_t(evict_segments(n))) * 4;
+  return KV * (3 + 2 * std::min(budget, n - budget) + evict_chunks(n) * (EVICT_INFO + 1024 + EVICT_CHUNK)) * 4;
 }
 
 extern "C" int w8a8_evict(void* k, int64_t k_head_stride, int64_t k_row_stride, void* v, int64_t v_head_stride,
@@ -540,28 +650,27 @@ extern "C" int w8a8_evict(void* k, int64_t k_head_stride, int64_t k_row_stride, 
   p.kept = kept; p.khs = KV > 1 ? kept_stride : 0; p.w_out = weights_out; p.wos = KV > 1 ? weights_out_stride : 0;
   p.pos_out = positions_out; p.pos_os = KV > 1 ? positions_out_stride : 0;
   p.most = int(std::min(budget, n - budget));
-  p.steps = evict_steps(n);
-  p.nseg = evict_segments(n);
-  p.nsub = p.nseg / EVICT_NW;
+  p.nch = int(evict_chunks(n));
   p.count = static_cast<int32_t*>(workspace);
-  p.head = p.count + KV;
-  p.before = p.head + 4 * KV;
-  p.hole = p.before + 3 * KV * p.nseg;
+  p.least = p.count + KV;
+  p.hole = p.least + 2 * KV;
   p.mover = p.hole + KV * p.most;
+  p.info = p.mover + KV * p.most;
+  p.digit = reinterpret_cast<uint32_t*>(p.info + KV * p.nch * EVICT_INFO);
+  p.open = p.digit + KV * p.nch * 1024;
   p.k = static_cast<char*>(k); p.kh = k_head_stride; p.kr = k_row_stride;
   p.v = static_cast<char*>(v); p.vh = v_head_stride; p.vr = v_row_stride;
   p.row_cols = int(row_bytes / 16);
-  if (n <= 1024 * 4)
-    evict_select_kernel<4><<<unsigned(KV), 1024, 0, stream>>>(p);
-  else if (n <= 1024 * 8)
-    evict_select_kernel<8><<<unsigned(KV), 1024, 0, stream>>>(p);
-  else if (n <= EVICT_FUSED)
-    evict_select_kernel<16><<<unsigned(KV), 1024, 0, stream>>>(p);
-  else if (n <= 1024 * 64)
-    evict_select_kernel<64><<<unsigned(KV), 1024, 0, stream>>>(p);
-  else
-    evict_select_kernel<0><<<unsigned(KV), 1024, 0, stream>>>(p);
-  if (p.nseg > 0) evict_list_kernel<<<dim3{unsigned(p.nseg), unsigned(KV), 1}, 256, 0, stream>>>(p);
+  if (p.nch == 0) {
+    evict_select_kernel<<<unsigned(KV), 1024, 0, stream>>>(p);
+  } else {
+    const dim3 grid{unsigned(p.nch), unsigned(KV), 1};
+    evict_newest_kernel<<<grid, 1024, 0, stream>>>(p);
+    evict_digit_kernel<<<grid, 1024, 0, stream>>>(p);
+    evict_split_kernel<<<grid, 1024, 0, stream>>>(p);
+    evict_least_kernel<<<unsigned(KV), 1024, 0, stream>>>(p);
+    evict_list_kernel<<<grid, 1024, 0, stream>>>(p);
+  }
   if (p.most > 0) {
     const int64_t blocks = std::min<int64_t>((int64_t(p.most) * p.row_cols + 255) / 256, 2048);
     evict_move_kernel<<<dim3{unsigned(blocks), unsigned(KV), 1}, 256, 0, stream>>>(p);
