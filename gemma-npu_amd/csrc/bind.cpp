@@ -14,10 +14,12 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPFunctions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <string>
+#include <vector>
 
 #include "w8a8.h"
 
@@ -74,6 +76,8 @@ struct Call {
   Tensor make(at::IntArrayRef size, ScalarType dt) const {
     return at::empty(size, at::TensorOptions(dt).device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device))));
   }
+  // The call's device has to be the current one (the wrapper makes it so).
+  void here() const { need(c10::hip::current_device() == device); }
   hipStream_t stream() const {
     return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(static_cast<c10::DeviceIndex>(device)).stream();
   }
@@ -519,6 +523,191 @@ PyObject* decode(PyObject* const* a) {
   return wrap(o);
 }
 
+// q, k, v, parents, n_past, window, scale -> o
+PyObject* decode_tree(PyObject* const* a) {
+  Call c;
+  const Heads q = heads(c, a[0]), k = heads(c, a[1]), v = heads(c, a[2]);
+  const Tensor& parents = c.vec(a[3], at::kInt);
+  c.here();
+  const int64_t H = q.t->size(0), N = q.t->size(1), D = q.t->size(2), KV = k.t->size(0), Tk = k.t->size(1);
+  const int64_t M = parents.size(0);
+  need(k.t->size(2) == D && v.t->sizes() == k.t->sizes() && N >= 1 && N <= M);
+  const int32_t* dev = nullptr;
+  int64_t past = -1;
+  if (THPVariable_CheckExact(a[4])) {
+    const Tensor& t = THPVariable_Unpack(a[4]);
+    need(t.is_cuda() && t.get_device() == c.device && t.scalar_type() == at::kInt && t.numel() == 1 && t.has_storage());
+    dev = static_cast<const int32_t*>(t.data_ptr());
+  } else {
+    past = integer(a[4]);
+    need(past >= 0);
+  }
+  const int64_t window = integer(a[5]);
+  const float scale = real(a[6]);
+  const int64_t bytes = w8a8_attention_tree_workspace_bytes(H, KV, N, M, Tk, D, past, window);
+  need(bytes >= 0);
+  const Tensor o = c.make({H, N, D}, at::kBFloat16), ws = bytes ? c.make({bytes}, at::kByte) : Tensor();
+  const hipStream_t st = c.stream();
+  launch("w8a8_attention_tree_bf16", [&] {
+    return w8a8_attention_tree_bf16(bf(*q.t), q.hs, q.rs, bf(*k.t), k.hs, k.rs, bf(*v.t), v.hs, v.rs, H, KV, N, M, Tk, D,
+                                    static_cast<const int32_t*>(parents.data_ptr()), past, dev, window, scale, bfo(o), N * D,
+                                    D, nullptr, bytes ? ws.data_ptr() : nullptr, bytes, st);
+  });
+  return wrap(o);
+}
+
+// q [H, Tq, D] or [H, D], k, lse, weights, q_start, window, scale -> True
+PyObject* add_key_weights(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[0]));
+  const bool one = THPVariable_Unpack(a[0]).dim() == 2;
+  const Tensor& qt = one ? c.rows(a[0], at::kBFloat16) : c.tensor(a[0], at::kBFloat16, 3);
+  const int64_t H = qt.size(0), Tq = one ? 1 : qt.size(1), D = qt.size(one ? 1 : 2);
+  need(one || D <= 1 || qt.stride(2) == 1);
+  const int64_t qrs = one || Tq <= 1 ? D : qt.stride(1), qhs = H > 1 ? qt.stride(0) : std::max<int64_t>(Tq, 1) * qrs;
+  const Heads k = heads(c, a[1]);
+  const int64_t KV = k.t->size(0), Tk = k.t->size(1);
+  need(k.t->size(2) == D && THPVariable_CheckExact(a[2]));
+  const bool vec = one && THPVariable_Unpack(a[2]).dim() == 1;
+  const Tensor& lse = vec ? c.tensor(a[2], at::kFloat, 1) : c.rows(a[2], at::kFloat);
+  need(lse.size(0) == H && (vec || lse.size(1) == Tq));
+  const Tensor& w = c.rows(a[3], at::kFloat);
+  need(w.size(0) == KV && w.size(1) == Tk);
+  c.here();
+  const int32_t* dev = nullptr;
+  int64_t start = -1;
+  if (THPVariable_CheckExact(a[4])) {
+    const Tensor& t = THPVariable_Unpack(a[4]);
+    need(t.is_cuda() && t.get_device() == c.device && t.scalar_type() == at::kInt && t.numel() == 1 && t.has_storage());
+    dev = static_cast<const int32_t*>(t.data_ptr());
+  } else {
+    start = integer(a[4]);
+    need(start >= 0);
+  }
+  const int64_t window = integer(a[5]);
+  const float scale = real(a[6]);
+  const int64_t bytes = w8a8_attention_key_weights_workspace_bytes(H, KV, Tq, Tk, D, start, window);
+  need(bytes >= 0);
+  const Tensor ws = bytes ? c.make({bytes}, at::kByte) : Tensor();
+  const hipStream_t st = c.stream();
+  launch("w8a8_attention_key_weights", [&] {
+    return w8a8_attention_key_weights(bf(qt), qhs, qrs, bf(*k.t), k.hs, k.rs, f32(lse), H > 1 ? lse.stride(0) : Tq, H, KV, Tq,
+                                      Tk, D, start, dev, window, scale, f32(w), KV > 1 ? w.stride(0) : Tk,
+                                      bytes ? ws.data_ptr() : nullptr, bytes, st);
+  });
+  Py_RETURN_TRUE;
+}
+
+// logits, scores, k -> (scores, beams, tokens)
+PyObject* beam_select(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[0]) && THPVariable_CheckExact(a[1]));
+  const ScalarType dt = THPVariable_Unpack(a[0]).scalar_type();
+  need(dt == at::kBFloat16 || dt == at::kFloat);
+  const int64_t dim = THPVariable_Unpack(a[0]).dim();
+  need(dim == 2 || dim == 3);
+  const Tensor &x = c.tensor(a[0], dt, dim), &s = c.tensor(a[1], at::kFloat, dim - 1);
+  c.here();
+  const int64_t B = dim == 3 ? x.size(0) : 1, nb = x.size(dim - 2), V = x.size(dim - 1), k = integer(a[2]);
+  need(s.size(dim - 2) == nb && (dim == 2 || s.size(0) == B));
+  need((V <= 1 || x.stride(dim - 1) == 1) && (nb <= 1 || s.stride(dim - 2) == 1));
+  const int64_t bytes = w8a8_beam_select_workspace_bytes(B, nb, V, k);
+  need(bytes > 0);
+  const std::vector<int64_t> size = dim == 3 ? std::vector<int64_t>{B, k} : std::vector<int64_t>{k};
+  const Tensor value = c.make(size, at::kFloat), beam = c.make(size, at::kLong), token = c.make(size, at::kLong),
+               ws = c.make({bytes}, at::kByte);
+  const hipStream_t st = c.stream();
+  launch("w8a8_beam_select", [&] {
+    return w8a8_beam_select(x.data_ptr(), dt == at::kFloat ? 1 : 0, B > 1 ? x.stride(0) : nb * V,
+                            nb > 1 ? x.stride(dim - 2) : V, f32(s), B > 1 ? s.stride(0) : nb, B, nb, V, k, f32(value),
+                            static_cast<int64_t*>(beam.data_ptr()), static_cast<int64_t*>(token.data_ptr()), ws.data_ptr(),
+                            bytes, st);
+  });
+  return tuple(value, beam, token);
+}
+
+// tensors (a list or tuple), index, dim -> True
+PyObject* reorder(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[1]));
+  const Tensor& index = c.tensor(a[1], at::kLong, THPVariable_Unpack(a[1]).dim() == 2 ? 2 : 1);
+  c.here();
+  const int64_t n = index.size(index.dim() - 1);
+  need(n >= 1 && n <= 64 && (n == 1 || index.stride(index.dim() - 1) == 1));
+  need(PyList_CheckExact(a[0]) || PyTuple_CheckExact(a[0]));
+  const int64_t count = PySequence_Fast_GET_SIZE(a[0]), dim0 = integer(a[2]);
+  std::vector<w8a8_rows> rows;
+  int64_t size = -1, entries = -1;
+  for (int64_t i = 0; i < count; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(a[0], i);
+    need(THPVariable_CheckExact(o));
+    const Tensor& t = THPVariable_Unpack(o);
+    need(t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && t.get_device() == c.device && t.numel() > 0);
+    const int64_t es = t.element_size(), nd = t.dim(), d = dim0 < 0 ? dim0 + nd : dim0;
+    need(d >= 0 && d < nd);
+    for (int64_t x = 0; x < nd; ++x) need(t.size(x) == 1 || t.stride(x) > 0);
+    int64_t outer = 1, outer_stride = 0, run = 1, runs = 1, run_stride = 0;
+    for (int64_t x = d - 1; x >= 0; --x) {
+      if (t.size(x) == 1) continue;
+      if (outer == 1)
+        outer_stride = t.stride(x);
+      else
+        need(t.stride(x) == outer * outer_stride);
+      outer *= t.size(x);
+    }
+    for (int64_t x = nd - 1; x > d; --x) {
+      if (t.size(x) == 1) continue;
+      if (runs == 1 && t.stride(x) == run)
+        run *= t.size(x);
+      else if (runs == 1)
+        runs = t.size(x), run_stride = t.stride(x);
+      else {
+        need(t.stride(x) == runs * run_stride);
+        runs *= t.size(x);
+      }
+    }
+    need(size < 0 || (t.size(d) == size && outer == entries));
+    size = t.size(d);
+    entries = outer;
+    rows.push_back({t.data_ptr(), outer_stride * es, t.stride(d) * es, run_stride * es, runs, run * es});
+  }
+  need(count > 0 && n <= size && (index.dim() == 1 || index.size(0) == entries));
+  const hipStream_t st = c.stream();
+  launch("w8a8_reorder_rows", [&] {
+    return w8a8_reorder_rows(rows.data(), count, static_cast<const int64_t*>(index.data_ptr()),
+                             index.dim() == 2 && entries > 1 ? index.stride(0) : 0, n, size, entries, st);
+  });
+  Py_RETURN_TRUE;
+}
+
+// k, v, weights, positions, n, budget, recent -> (kept, weights, positions)
+PyObject* evict(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[0]));
+  const ScalarType dt = THPVariable_Unpack(a[0]).scalar_type();
+  const Tensor &k = c.tensor(a[0], dt, 3), &v = c.tensor(a[1], dt, 3);
+  need(k.sizes() == v.sizes() && (k.size(2) <= 1 || (k.stride(2) == 1 && v.stride(2) == 1)));
+  const int64_t KV = k.size(0), Tk = k.size(1), D = k.size(2), es = k.element_size();
+  const Tensor &w = c.rows(a[2], at::kFloat), &pos = c.rows(a[3], at::kInt);
+  c.here();
+  const int64_t n = integer(a[4]), budget = integer(a[5]), recent = integer(a[6]);
+  need(w.size(0) == KV && pos.size(0) == KV && w.size(1) >= n && pos.size(1) >= n);
+  need(budget >= 1 && budget <= n && n <= Tk && recent >= 0 && recent <= budget);
+  const int64_t bytes = w8a8_evict_workspace_bytes(KV, n, budget);
+  need(bytes > 0);
+  const Tensor kept = c.make({KV, budget}, at::kInt), wo = c.make({KV, budget}, at::kFloat),
+               po = c.make({KV, budget}, at::kInt), ws = c.make({bytes}, at::kByte);
+  const hipStream_t st = c.stream();
+  launch("w8a8_evict", [&] {
+    return w8a8_evict(k.data_ptr(), KV > 1 ? k.stride(0) * es : 0, Tk > 1 ? k.stride(1) * es : D * es, v.data_ptr(),
+                      KV > 1 ? v.stride(0) * es : 0, Tk > 1 ? v.stride(1) * es : D * es, D * es, KV, n, f32(w),
+                      KV > 1 ? w.stride(0) : w.size(1), static_cast<const int32_t*>(pos.data_ptr()),
+                      KV > 1 ? pos.stride(0) : pos.size(1), budget, recent, static_cast<int32_t*>(kept.data_ptr()), budget,
+                      f32(wo), budget, static_cast<int32_t*>(po.data_ptr()), budget, ws.data_ptr(), bytes, st);
+  });
+  return tuple(kept, wo, po);
+}
+
 // Waits for torch's current stream of tensor t's device; True when it is done, None without waiting if t is
 // no GPU tensor.
 PyObject* wait_stream(PyObject* const* a) {
@@ -572,7 +761,8 @@ PyMethodDef methods[] = {
     W8A8_ENTRY(quant_packed, 1), W8A8_ENTRY(k_in, 3),           W8A8_ENTRY(k_post_attn, 7), W8A8_ENTRY(k_post_ff, 6),
     W8A8_ENTRY(k_ple_gate, 4),  W8A8_ENTRY(k_ple_out_k_in, 8),  W8A8_ENTRY(k_qkv, 12),    W8A8_ENTRY(attention, 7),
     W8A8_ENTRY(attention_quant, 7), W8A8_ENTRY(decode, 7),      W8A8_ENTRY(wait_stream, 1),
-    W8A8_ENTRY(settle, 2),
+    W8A8_ENTRY(settle, 2),      W8A8_ENTRY(decode_tree, 7),     W8A8_ENTRY(add_key_weights, 7), W8A8_ENTRY(beam_select, 3),
+    W8A8_ENTRY(reorder, 3),     W8A8_ENTRY(evict, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "The wrappers' launch path in native code.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

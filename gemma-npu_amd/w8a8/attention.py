@@ -350,6 +350,10 @@ def decode_tree(q, k, v, parents, n_past, window=0, scale=1.0, out=None, return_
     Returns o [H, N, D] (into `out` if given, any strides with a contiguous last dimension), and with
     return_lse the fp32 [H, N] logsumexp.  workspace: a device uint8 tensor of at least
     decode_tree_workspace_bytes(...); by default one from torch's allocator."""
+    if _native is not None and out is None and workspace is None and not return_lse:
+        o = _native.decode_tree(q, k, v, parents, n_past, window, scale)
+        if o is not None:
+            return o
     _check3(q, "q")
     _check3(k, "k")
     _check3(v, "v")
@@ -404,6 +408,8 @@ def add_key_weights(q, k, lse, weights, q_start=0, window=0, scale=1.0, workspac
     weights: fp32 [KV, Tk], changed in place and returned.  Keys are seen as in attention().  q_start: an int,
     or with few rows (Tq * H // KV <= 32) an int32 GPU tensor of one element, so that a captured decode step
     adds at each new position.  A query with an lse of -inf adds nothing.  Deterministic."""
+    if _native is not None and workspace is None and _native.add_key_weights(q, k, lse, weights, q_start, window, scale):
+        return weights
     if isinstance(q, torch.Tensor) and q.dim() == 2:
         q = q[:, None]
         lse = lse[:, None] if isinstance(lse, torch.Tensor) and lse.dim() == 1 else lse

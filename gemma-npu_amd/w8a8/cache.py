@@ -11,7 +11,7 @@ weights).  Everything runs on torch's current stream of the tensors' device; the
 import torch
 
 from ._lib import Rows, call_on, lib
-from .ops import _stream
+from .ops import _native, _stream
 
 
 def _runs(t, dim, name):
@@ -55,6 +55,8 @@ def reorder(tensors, index, dim=0):
     rows may be exchanged, repeated and dropped.  An index outside the dimension leaves its row as it is.
     Views are taken as they are, so k[:, :, :length] moves the live rows only; the tensors must not overlap."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if _native is not None and _native.reorder(tensors, index, dim):
+        return
     if not isinstance(index, torch.Tensor) or index.dtype != torch.int64 or index.dim() not in (1, 2):
         raise TypeError("reorder: index must be an int64 GPU tensor [n] or [outer, n]")
     if index.device.type != "cuda":
@@ -107,6 +109,10 @@ def evict(k, v, weights, positions, n, budget, recent=0, out=None, workspace=Non
     on their order.  Returns (kept int32, weights fp32, positions int32), each [KV, budget]: the row that each
     row came from, and its weight and position; out: the three tensors to write them to, of which the
     latter two may be weights[:, :budget] and positions[:, :budget] themselves."""
+    if _native is not None and out is None and workspace is None:
+        r = _native.evict(k, v, weights, positions, n, budget, recent)
+        if r is not None:
+            return r
     n, budget, recent = int(n), int(budget), int(recent)
     for t, name in ((k, "k"), (v, "v")):
         if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dim() != 3:

@@ -484,6 +484,10 @@ def beam_select(logits, scores, k, workspace=None):
     and values in order.  -inf logits are tokens that cannot follow; a NaN or +inf logit makes its beam's
     scores NaN, which rank first, as torch.topk has it.  k <= 64, nb <= 256.  workspace: a device uint8
     tensor of beam_select_workspace_bytes(...); by default one from torch's allocator."""
+    if _native is not None and workspace is None:
+        r = _native.beam_select(logits, scores, k)
+        if r is not None:
+            return r
     if not isinstance(logits, torch.Tensor) or not isinstance(scores, torch.Tensor):
         raise TypeError("beam_select: logits and scores must be tensors")
     if logits.device.type != "cuda" or scores.device != logits.device:
