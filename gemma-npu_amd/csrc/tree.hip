@@ -18,11 +18,11 @@
 //
 // Within a workgroup the key blocks pass through a two-slot LDS ring (buffer_load ... lds, K one block
 // further ahead than V), one barrier per block: iteration n makes S^T = K Q^T and the softmax of block
-// n + 1 and multiplies P V of block n.  Each wave owns 16 rows' S phase (with fewer row tiles than waves
-// several waves make the same one: the keys' way through memory is what bounds those) and D / NW columns
-// of O^T in the P V phase, its V^T operand read from the row-major V rows with ds_read_b64_tr_b16.
+// n + 1 and multiplies P V of block n.  The first RT waves own 16 rows' S phase each (the others wait: the
+// keys' way through memory is what bounds small tiles), every wave D / NW columns of O^T in the P V phase,
+// its V^T operand read from the row-major V rows with ds_read_b64_tr_b16.
 // Scores, softmax and sums are fp32; the softmax weights are rounded to bf16 for the second product, at
-// most 2^-9 of each weight, as the other attention kernels do.
+// most 2^-8 of each weight, as the other attention kernels do.
 //
 // Values a row does not see never reach it: in the blocks that some row sees only in part (those at the
 // window's edge and the tree's own) infinities and NaN in V are replaced by zeros before the MFMA, whose
@@ -69,11 +69,13 @@ __device__ __forceinline__ TreeGeom tree_geom(const TreeParams& p) {
   return t;
 }
 
-constexpr int tree_waves(int rt) { return rt > 4 ? 8 : 4; }
+// Waves of a workgroup.  At head_dim 512 a tile of 64 rows has eight too, four of which have no rows of their own in
+// the S phase: half of O^T per wave leaves the registers for a variable per slot (64 nodes over 32749 rows 91 -> 75 us).
+constexpr int tree_waves(int rt, int d) { return rt > 4 || (d == 512 && rt == 4) ? 8 : 4; }
 
 template <int D, int RT>
 struct TreeShape {
-  static constexpr int NW = tree_waves(RT);
+  static constexpr int NW = tree_waves(RT, D);
   static constexpr int NT = NW * 64;
   static constexpr int BN = D == 128 ? 64 : 32;      // keys per block
   static constexpr int R = RT * 16;                  // rows per tile
@@ -88,7 +90,7 @@ struct TreeShape {
   static constexpr int AUX = B_OFF + TREE_MAX_NODES * (TREE_WORDS + 2) * 4;
   static constexpr int NDW = D / NW / 16;            // 16-wide d tiles of O^T per wave
   static constexpr int KR = 3;                       // K fragments in flight
-  static constexpr bool SPLIT = D < 512 || RT < 4;   // a variable per slot (the others would spill)
+  static constexpr bool SPLIT = D < 512 || RT < 5;   // a variable per slot (the others would spill)
 };
 
 // The nodes' views of the tree into LDS: bits[m] = the nodes on m's chain (none: unused), depth[m].  Every
@@ -139,7 +141,7 @@ __device__ __forceinline__ void tree_resolve(const int32_t* parents, int M, uint
 }
 
 template <int D, int RT>
-__global__ __launch_bounds__(tree_waves(RT) * 64, 1) void attn_tree_kernel(TreeParams p) {
+__global__ __launch_bounds__(tree_waves(RT, D) * 64, 1) void attn_tree_kernel(TreeParams p) {
   using S = TreeShape<D, RT>;
   constexpr int NW = S::NW, NT = S::NT, BN = S::BN, R = S::R, KCH = S::KCH, ROW = S::ROW, PLD = S::PLD, NDW = S::NDW;
   constexpr int NKC = BN / 32;              // 32-key chunks per block
@@ -629,12 +631,12 @@ static TreePlan tree_plan(int64_t H, int64_t KV, int64_t N, int64_t M, int64_t T
   // through memory, the tile's store, and the parts written and read back.  The times of a block
   // (64 KiB of K and V at head_dim 512, 32 KiB else) are fitted to calls of 8 to 1024 rows over 700 to
   // 65521 keys; small tiles read the keys more often, large ones leave more to be joined.  us at 16 / 32 /
-  // 64 / 80 / 96 / 128 rows a tile: 8 heads of 512, 16 nodes over 3658 rows 20 / 22 / 25 / 26 / 27 / 31, over
-  // 32749 rows 57 / 42 / 39 / 39 / 39 / 45, 64 nodes over 32749 rows 194 / 121 / 92 / - / - / 71; 32 heads of
+  // 64 / 80 / 96 / 128 rows a tile: 8 heads of 512, 16 nodes over 3658 rows 20 / 22 / 26 / 26 / 27 / 31, over
+  // 32749 rows 57 / 42 / 36 / 39 / 39 / 45, 64 nodes over 32749 rows 194 / 121 / 75 / - / - / 72; 32 heads of
   // 128 on 8, 33 nodes over 65521 rows 163 / 114 / 131 / 96 / 103 / 112.
   static const int tiles[6] = {1, 2, 4, 5, 6, 8};
   static const double block[3][6] = {{0.63, 0.75, 1.2, 1.27, 1.4, 1.6}, {0.55, 0.8, 1.15, 1.3, 1.45, 1.75},
-                                     {1.45, 1.7, 2.3, 2.4, 2.5, 2.9}};
+                                     {1.45, 1.7, 1.8, 2.4, 2.5, 2.9}};
   const int di = D == 128 ? 0 : D == 256 ? 1 : 2;
   const int64_t xcd_cus = std::max(1, attn_cu_count() / 8);
   double least = 0.0;

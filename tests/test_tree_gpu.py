@@ -305,8 +305,8 @@ PLANS = [
     (512, 32, 64, 0, 128, 128, False), (16, 1, 128, 0, 128, 64, True), (16, 1, 33, 2000, 128, 80, True), (10, 2, 33, 8000, 128, 96, True),
     (256, 16, 33, 500, 128, 128, True), (32, 2, 33, 100, 256, 32, True), (16, 16, 33, 2000, 256, 64, True), (16, 1, 33, 2000, 256, 80, True),
     (10, 2, 33, 8000, 256, 96, True), (24, 8, 33, 8000, 256, 128, True), (512, 32, 64, 0, 256, 128, False), (16, 1, 33, 0, 512, 32, True),
-    (1024, 64, 10, 0, 512, 64, False), (16, 1, 128, 0, 512, 64, True), (6, 1, 128, 2000, 512, 80, True), (10, 2, 33, 8000, 512, 96, True),
-    (24, 4, 33, 8000, 512, 128, True), (512, 32, 64, 0, 512, 128, False),
+    (1024, 64, 10, 0, 512, 64, False), (16, 1, 128, 0, 512, 64, True), (16, 4, 33, 8000, 512, 80, True), (64, 8, 12, 8000, 512, 96, True),
+    (96, 16, 64, 2000, 512, 128, True), (256, 16, 128, 0, 512, 128, False),
 ]
 
 
