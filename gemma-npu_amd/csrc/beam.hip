@@ -366,9 +366,10 @@ static int64_t beam_chunks(int64_t rows, int64_t V) {
   return (V + chunk - 1) / chunk;
 }
 
+// (Launches of less than 2^32 threads.)
 static bool beam_shape_ok(int64_t B, int64_t nb, int64_t V, int64_t k) {
-  return B >= 1 && B <= INT32_MAX && nb >= 1 && nb <= BEAM_MAX_BEAMS && V >= 1 && V <= INT32_MAX / 2 && k >= 1 &&
-         k <= BEAM_MAX_K && k <= nb * V && B * nb <= INT32_MAX / (beam_chunks(B * nb, V) * BEAM_MAX_K);
+  return B >= 1 && B < (1 << 22) && nb >= 1 && nb <= BEAM_MAX_BEAMS && V >= 1 && V <= INT32_MAX / 2 && k >= 1 &&
+         k <= BEAM_MAX_K && k <= nb * V && B * nb * beam_chunks(B * nb, V) < (1 << 24);
 }
 
 extern "C" int64_t w8a8_beam_select_workspace_bytes(int64_t B, int64_t nb, int64_t V, int64_t k) {

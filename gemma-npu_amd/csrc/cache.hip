@@ -16,6 +16,7 @@ namespace w8a8 {
 
 constexpr int REORDER_MAX = 64;       // rows of the axis that change
 constexpr int REORDER_TENSORS = 48;   // tensors of a launch
+constexpr int64_t REORDER_BLOCKS = (int64_t(1) << 24) - 1;  // workgroups of a launch's x: 2^32 threads are too many
 
 struct ReorderTensor {
   char* base;
@@ -574,6 +575,10 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
     if ((size > 1 && r.axis_stride <= 0) || (outer > 1 && r.outer_stride <= 0) || (r.runs > 1 && r.run_stride < r.run_bytes) ||
         (size > 1 && r.axis_stride < r.run_bytes))
       return fail(W8A8_EINVAL, "%s: tensor %lld: strides must be positive and rows must not overlap", what, (long long)i);
+    // the same memory twice (a cache that two layers share) would be read and written by two workgroups
+    for (int64_t j = 0; j < i; ++j)
+      if (tensors[j].data == r.data && tensors[j].runs > 0 && tensors[j].run_bytes > 0)
+        return fail(W8A8_EINVAL, "%s: tensors %lld and %lld are the same memory", what, (long long)j, (long long)i);
     for (int64_t x : {int64_t(reinterpret_cast<uintptr_t>(r.data)), size > 1 ? r.axis_stride : 0, outer > 1 ? r.outer_stride : 0,
                       r.runs > 1 ? r.run_stride : 0, r.run_bytes})
       while (x % align != 0) align = align == 16 ? 4 : 1;
@@ -591,7 +596,7 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
       d.run = r.run_bytes / align; d.ninner = int(r.runs);
       const int64_t b = (d.run * d.ninner + 255) / 256;
       if (d.run * d.ninner > INT32_MAX) return fail(W8A8_ENOTSUP, "%s: tensor %lld too large", what, (long long)i0);
-      if (blocks + b > INT32_MAX / 2) break;
+      if (blocks + b > REORDER_BLOCKS) break;  // (one tensor never has so many)
       d.block0 = int(blocks);
       blocks += b;
       ++p.ntensors;

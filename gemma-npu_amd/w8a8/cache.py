@@ -53,7 +53,8 @@ def reorder(tensors, index, dim=0):
     index: int64 GPU tensor [n], n <= 64 and at most the size of dim (rows past n are left as they are), or
     [outer, n] with one row per entry of the dimensions before dim.  Every row is read before any is written:
     rows may be exchanged, repeated and dropped.  An index outside the dimension leaves its row as it is.
-    Views are taken as they are, so k[:, :, :length] moves the live rows only; the tensors must not overlap."""
+    Views are taken as they are, so k[:, :, :length] moves the live rows only; the tensors must not overlap
+    (one given twice, as a cache that two layers share, is refused)."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if _native is not None and _native.reorder(tensors, index, dim):
         return

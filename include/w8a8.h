@@ -635,7 +635,8 @@ typedef struct {
  * of an accepted path of drafted tokens moved up.  index int64 [n] in device memory, for all `outer`
  * entries, or with index_stride > 0 [outer, n] of that row stride.  Rows 0 .. size - 1 can be taken, the
  * first n <= 64 change; every row is read before any is written, so rows may be exchanged, repeated and
- * dropped; an index outside 0 .. size - 1 leaves its row as it is.  Tensors must not overlap each other. */
+ * dropped; an index outside 0 .. size - 1 leaves its row as it is.  Tensors must not overlap each other (the
+ * same address twice is refused); outer <= 65535. */
 int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const int64_t *index, int64_t index_stride, int64_t n,
                       int64_t size, int64_t outer, hipStream_t stream);
 
@@ -645,8 +646,9 @@ int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const int64_t *in
  * Sums and ranking in 64 bits.  -inf logits are tokens that cannot follow; a beam whose score minus
  * logsumexp is not finite (a score of -inf: a beam that is out; a NaN or +inf logit: NaN) gives that value
  * to all its tokens, all -inf logits give -inf; NaN ranks first, as torch.topk has it.
- * nb <= 256, k <= 64, k <= nb * V.  workspace: w8a8_beam_select_workspace_bytes(...) bytes (-1: invalid),
- * 8-byte aligned, scratch.  Two launches, deterministic. */
+ * nb <= 256, k <= 64, k <= nb * V, B < 2^22, less than 2^24 chunks (of 4096 logits of a beam, or 8192 where
+ * there are many).  workspace: w8a8_beam_select_workspace_bytes(...) bytes (-1: invalid), 8-byte aligned,
+ * scratch.  Two launches, deterministic. */
 int64_t w8a8_beam_select_workspace_bytes(int64_t B, int64_t nb, int64_t V, int64_t k);
 int w8a8_beam_select(const void *logits, int logits_are_f32, int64_t group_stride, int64_t row_stride,
                      const float *scores, int64_t score_stride, int64_t B, int64_t nb, int64_t V, int64_t k,

@@ -127,6 +127,9 @@ def test_reorder_refusals():
     ]:
         with pytest.raises(error):
             cache.reorder(*args)
+    for args in (([t, t + 1, t], i), ([t, t[:, :2]], i)):                           # the same memory twice
+        with pytest.raises(W8A8Error, match="same memory"):
+            cache.reorder(*args)
     cache.reorder([], i)
     cache.reorder(t, i[:0])
     cache.reorder(torch.zeros(4, 0, device=DEV), i)

@@ -60,6 +60,7 @@ def test_key_weights():
         (dict(krs=128), EINVAL, "strides"), (dict(qrs=260), EALIGN, "strides"), (dict(lhs=19), EINVAL, "lse"),
         (dict(whs=99), EINVAL, "weights"), (dict(q=ODD), EALIGN, "aligned"), (dict(w=ODD), EALIGN, "aligned"),
         (dict(krs=1 << 31), ENOTSUP, "stride"),
+        (dict(H=1 << 16, KV=1 << 16), EINVAL, "KV=65536"),                                    # past a launch's second dimension
     ])
     size = _lib.lib().w8a8_attention_key_weights_workspace_bytes
     assert size(8, 1, 1, 5000, 512, 4999, 0) == 0 and size(8, 1, 1, 5000, 512, -1, 0) == 0
@@ -97,6 +98,8 @@ def test_reorder():
         (dict(tensors=rows(runs=2, run_stride=100)), EINVAL, "overlap"), (dict(tensors=rows(data=None)), EINVAL, "tensor 0"),
         (dict(tensors=rows(runs=-1)), EINVAL, "tensor 0"),
     ])
+    twice = (_lib.Rows * 3)(rows()[0], rows(data=0x900000)[0], rows()[0])
+    refused("w8a8_reorder_rows", ok, [(dict(tensors=twice, count=3), EINVAL, "0 and 2 are the same memory")])
     assert status("w8a8_reorder_rows", {**ok, "count": 0})[0] == 0
     assert status("w8a8_reorder_rows", {**ok, "n": 0})[0] == 0
     assert status("w8a8_reorder_rows", {**ok, "tensors": rows(runs=0)})[0] == 0
@@ -109,6 +112,7 @@ def test_beams():
         (dict(V=0), EINVAL, "V=0"), (dict(B=0), EINVAL, "B=0"), (dict(x=None), EINVAL, "null"), (dict(ot=None), EINVAL, "null"),
         (dict(rs=99), EINVAL, "strides"), (dict(ss=3), EINVAL, "strides"), (dict(wsb=8), EINVAL, "workspace"), (dict(x=ODD), EALIGN, "aligned"),
         (dict(ob=ODD), EALIGN, "aligned"), (dict(B=1 << 30), EINVAL, "B="),
+        (dict(B=1 << 22), EINVAL, "B="), (dict(B=70000, nb=256, ss=256), EINVAL, "B=70000"),   # launches past 2^32 threads
     ])
     size = _lib.lib().w8a8_beam_select_workspace_bytes
     assert size(1, 4, 262144, 8) > 0 and size(1, 4, 262144, 65) == -1 and size(1, 2, 3, 7) == -1
