@@ -79,7 +79,8 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
 //                        counted, the keys of that digit listed, in row order
 //   evict_least_kernel   one workgroup per KV head finds the key among those, and what is before each chunk
 //   evict_list_kernel    the lists of free places and moving rows, chunk by chunk
-// and evict_move_kernel copies the rows.  Loops are not unrolled over a thread's rows: a workgroup runs
+// and evict_move_kernel copies the rows.  A cache that is cut by a few rows (EVICT_FEW, as at every step of a
+// cache that is full) is one launch of evict_few_kernel, which takes the rows that go one by one.  Loops are not unrolled over a thread's rows: a workgroup runs
 // through such code once, and fetching it took longer than the work (65521 rows of 8 heads with the keys in
 // registers 84 us for the select alone, 242 us reading them again at each step; in chunks 34).
 
@@ -87,6 +88,8 @@ constexpr int EVICT_NW = 16;
 constexpr int EVICT_ONE = 16384;           // most rows of evict_select_kernel
 constexpr int EVICT_CHUNK = 4096;          // rows per workgroup of the others
 constexpr int EVICT_INFO = 6;              // words of a chunk's counts
+constexpr int EVICT_FEW = 6;               // most rows that evict_few_kernel takes out
+constexpr int EVICT_FEW_COLS = 2048;       // and most 16-byte columns of k (and of v) that its workgroup moves
 
 struct EvictParams {
   const float* w; int64_t whs;          // fp32 [KV, n]
@@ -268,6 +271,90 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams p) {
     }
   }
   if (wave == EVICT_NW - 1 && lane == 0) p.count[g] = hole;
+}
+
+// One workgroup per KV head and a launch for everything, where at most EVICT_FEW rows go.  A thread holds E rows
+// in registers; the row of the least key (ties: the highest) goes, as often as rows have to.  Each choice is a
+// minimum over the workgroup, which bounds it (1.2 us): of 4097 rows of head_dim 512 one goes in 5.3 us, four in
+// 9.1, eight would in 13.9; the radix select and the launch that moves the rows take 13.8 whatever goes (of 512
+// rows 9.4 against 7.7 for four and 11.8 for eight, of 16384 28 against 13 and 19).
+template <int E>
+__global__ __launch_bounds__(1024) void evict_few_kernel(EvictParams p) {
+  __shared__ uint64_t least[2][EVICT_NW];
+  __shared__ int red[EVICT_NW], out[EVICT_FEW], hole[EVICT_FEW], mover[EVICT_FEW];
+  const int t = threadIdx.x, wave = t >> 6, g = blockIdx.x, n = p.n, budget = p.budget, drop = n - budget;
+  const float* w = p.w + int64_t(g) * p.whs;
+  const int32_t* pos = p.pos + int64_t(g) * p.phs;
+  float x[E];
+  int32_t y[E];
+  int newest = INT32_MIN;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int r = t + 1024 * e;
+    x[e] = r < n ? w[r] : 0.0f;
+    y[e] = r < n ? pos[r] : INT32_MIN;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) newest = max(newest, y[e]);
+  const int64_t old = int64_t(evict_max(newest, red)) - p.recent;
+  uint32_t key[E], gone = 0;  // and this thread's rows that are not there
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    key[e] = evict_key(x[e], y[e], old);
+    gone |= t + 1024 * e < n ? 0u : 1u << e;
+  }
+#pragma unroll 1
+  for (int j = 0; j < drop; ++j) {
+    // the least key and, less for higher rows, its place (at least two rows are left: none is ~0 but the last)
+    uint64_t m = ~0ull;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (!(gone >> e & 1u)) m = min(m, uint64_t(key[e]) << 32 | uint32_t(~(t + 1024 * e)));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = min(m, uint64_t(__shfl_xor(m, o, 64)));
+    if ((t & 63) == 0) least[j & 1][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EVICT_NW; ++i) m = min(m, least[j & 1][i]);
+    const int r = int(~uint32_t(m));
+    if ((r & 1023) == t) gone |= 1u << (r >> 10);
+    if (t == 0) out[j] = r;
+  }
+  __syncthreads();
+  // free places and the rows that fill them, both in row order: thread j < drop ranks out[j] and row budget + j
+  int nhole = 0;
+  for (int j = 0; j < drop; ++j) nhole += out[j] < budget ? 1 : 0;
+  if (t < drop) {
+    int before = 0, moves = 0;
+    bool stays = true;  // row budget + t
+    for (int i = 0; i < drop; ++i) {
+      before += out[i] < out[t] ? 1 : 0;
+      moves += out[i] >= budget && out[i] < budget + t ? 1 : 0;
+      stays = stays && out[i] != budget + t;
+    }
+    if (out[t] < budget) hole[before] = out[t];
+    if (stays) mover[t - moves] = budget + t;
+  }
+  int32_t* const ko = p.kept + int64_t(g) * p.khs;
+  float* const wo = p.w_out + int64_t(g) * p.wos;
+  int32_t* const po = p.pos_out + int64_t(g) * p.pos_os;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int r = t + 1024 * e;
+    if (r < budget && !(gone >> e & 1u)) ko[r] = r, wo[r] = x[e], po[r] = y[e];
+  }
+  __syncthreads();
+  char* const k = p.k + int64_t(g) * p.kh;
+  char* const v = p.v + int64_t(g) * p.vh;
+  for (int i = t; i < nhole * p.row_cols; i += 1024) {
+    const int m = i / p.row_cols, col = i % p.row_cols;
+    const int64_t dst = hole[m], src = mover[m], c = int64_t(col) * 16;
+    const v4u a = *reinterpret_cast<const v4u*>(k + src * p.kr + c);
+    const v4u b = *reinterpret_cast<const v4u*>(v + src * p.vr + c);
+    *reinterpret_cast<v4u*>(k + dst * p.kr + c) = a;
+    *reinterpret_cast<v4u*>(v + dst * p.vr + c) = b;
+    if (col == 0) ko[dst] = int32_t(src), wo[dst] = w[src], po[dst] = pos[src];
+  }
 }
 
 // A chunk's rows of thread t: chunk * 4096 + 256 (t / 64) + t % 64, + 64, + 128, + 192.
@@ -666,6 +753,15 @@ extern "C" int w8a8_evict(void* k, int64_t k_head_stride, int64_t k_row_stride, 
   p.k = static_cast<char*>(k); p.kh = k_head_stride; p.kr = k_row_stride;
   p.v = static_cast<char*>(v); p.vh = v_head_stride; p.vr = v_row_stride;
   p.row_cols = int(row_bytes / 16);
+  if (p.nch == 0 && n > budget && n - budget <= EVICT_FEW && (n - budget) * p.row_cols <= EVICT_FEW_COLS) {
+    if (n <= 4 * 1024)
+      evict_few_kernel<4><<<unsigned(KV), 1024, 0, stream>>>(p);
+    else if (n <= 8 * 1024)
+      evict_few_kernel<8><<<unsigned(KV), 1024, 0, stream>>>(p);
+    else
+      evict_few_kernel<16><<<unsigned(KV), 1024, 0, stream>>>(p);
+    return check_launch(what);
+  }
   if (p.nch == 0) {
     evict_select_kernel<<<unsigned(KV), 1024, 0, stream>>>(p);
   } else {

@@ -173,6 +173,10 @@ def run_evict(k, v, w, pos, n, budget, recent, **kw):
     (1, 1, 1, 128, 1, 0), (1, 2, 2, 128, 1, 1), (1, 2, 2, 128, 1, 0), (3, 10, 7, 64, 4, 2), (1, 64, 64, 256, 64, 5),
     (2, 65, 65, 128, 64, 64), (1, 1025, 1024, 512, 100, 10), (1, 4097, 4097, 512, 4096, 1024), (2, 5000, 4096, 128, 17, 0),
     (1, 16384, 16384, 64, 9000, 3000), (2, 16385, 16385, 64, 16384, 100), (1, 40000, 33333, 128, 1, 1), (4, 3001, 3001, 128, 1500, 1500),
+    # few rows go
+    (1, 3, 3, 128, 1, 1), (2, 9, 9, 64, 1, 0), (1, 10, 10, 64, 1, 1), (1, 16, 12, 64, 7, 3), (3, 1000, 1000, 128, 995, 64), (1, 4096, 4096, 64, 4095, 0),
+    (2, 4100, 4097, 512, 4089, 1024), (1, 8192, 8192, 128, 8190, 8190), (2, 8193, 8193, 64, 8186, 100), (1, 16384, 16384, 128, 16383, 17),
+    (1, 500, 500, 4096, 497, 5), (1, 500, 500, 4096, 493, 5),
 ], ids=lambda c: "x".join(map(str, c)))
 def test_evict_matches_the_definition(case):
     KV, rows, n, D, budget, recent = case
@@ -195,6 +199,10 @@ def test_evict_special_weights():
     w[0, 3::7], w[0, 4::9], w[0, 5::11], w[1, ::2], w[1, 1::4] = math.nan, math.inf, -math.inf, 0.0, -0.0
     run_evict(k, v, w, pos, n, budget, 20)
     run_evict(k, v, torch.full((2, n), math.nan), pos, n, budget, 0)
+    for few in (n - 1, n - 6):
+        run_evict(k, v, w, pos, n, few, 20)
+        run_evict(k, v, torch.full((2, n), math.nan), pos, n, few, few)
+        run_evict(k, v, w, pos[:, :1].expand(2, n).contiguous(), n, few, 1)          # every row is the newest
     run_evict(k, v, torch.full((2, n), 1e-42), pos, n, budget, 5)      # subnormal, all equal
     extreme = pos.clone()
     extreme[:, 0], extreme[:, 1] = -2 ** 31, 2 ** 31 - 1
