@@ -13,7 +13,7 @@
 // the k best.  beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k
 // best of those lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and
 // the choice between them has to be right.  The logits' way through memory bounds large calls (64 beams of
-// 262144 fp32 logits: 43 -> 30 us, 67 MB), two kernels' starts and barriers small ones (4 beams of bf16: 20 -> 15 us).
+// 262144 fp32 logits: 43 -> 28 us, 67 MB), two kernels' starts and barriers small ones (4 beams of bf16: 20 -> 13.5 us).
 #include <algorithm>
 
 #include "w8a8_common.h"
@@ -211,8 +211,8 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
 
 __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
   __shared__ double base_s[BEAM_MAX_BEAMS];
-  __shared__ uint64_t lv[BEAM_LIST], gmax[64], bound_s;
-  __shared__ uint32_t li[BEAM_LIST];
+  __shared__ uint64_t lv[BEAM_LIST], la[BEAM_LIST];  // candidates: score's order bits, beam << 32 | token
+  __shared__ uint32_t gmax[64], bound_s;
   __shared__ int count;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int grp = blockIdx.x;
@@ -244,10 +244,14 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     if (lane == 0) base_s[i] = b;
   }
   __syncthreads();
-  // a candidate's score's order bits and i V + v; false where there is none.  A beam whose base is not finite
-  // has that score for every token: its first tokens stand for it.
+  // A candidate's score's order bits and place; false where there is none.  A beam whose base is not finite
+  // has that score for every token: its first tokens stand for it.  (j / per, less than 256, from a product
+  // that is off by at most one: an integer division is most of the work otherwise.)
+  const float rper = 1.0f / float(per);
   auto score = [&](int j, uint2 a, uint64_t& o, uint64_t& at) __attribute__((always_inline)) {
-    const int i = j / per, c = j % per;
+    int i = int(float(j) * rper), c = j - i * per;
+    if (c < 0) --i, c += per;
+    if (c >= per) ++i, c -= per;
     const double b = base_s[i];
     uint32_t tok = a.y;
     double sc = b + double(__uint_as_float(a.x));
@@ -256,101 +260,90 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
       tok = c < p.k && c < p.V ? uint32_t(c) : 0xffffffffu;
     }
     o = order_bits(sc);
-    at = uint64_t(i) * uint64_t(p.V) + tok;
+    at = uint64_t(uint32_t(i)) << 32 | tok;
     return tok != 0xffffffffu;
   };
-  auto get = [&](int j, uint64_t& o, uint64_t& at) __attribute__((always_inline)) { return score(j, cand[j], o, at); };
-  uint64_t bits[BEAM_HELD], top = 0;  // (0, below every score: none)
+  uint64_t bits[BEAM_HELD], place[BEAM_HELD], top = 0;  // (0, below every score: none)
 #pragma unroll
   for (int u = 0; u < BEAM_HELD; ++u) {
-    uint64_t o = 0, at;
+    bits[u] = 0;
+    if (1024 * u >= total) break;
     const int j = t + 1024 * u;
-    bits[u] = j < total && score(j, held[u], o, at) ? o : 0;
+    if (j < total && !score(j, held[u], bits[u], place[u])) bits[u] = 0;
     top = max(top, bits[u]);
   }
   for (int j = t + 1024 * BEAM_HELD; j < total; j += 1024) {
     uint64_t o, at;
-    if (get(j, o, at)) top = max(top, o);
+    if (score(j, cand[j], o, at)) top = max(top, o);
   }
+  // the bound: of the scores' upper halves
+  uint32_t high = uint32_t(top >> 32);
 #pragma unroll
-  for (int x = 8; x > 0; x >>= 1) {
-    const uint64_t o = __shfl_xor(top, x, 64);
-    top = max(top, o);
-  }
-  if ((t & 15) == 0) gmax[t >> 4] = top;
+  for (int x = 8; x > 0; x >>= 1) high = max(high, uint32_t(__shfl_xor(high, x, 64)));
+  if ((t & 15) == 0) gmax[t >> 4] = high;
   __syncthreads();
   if (wave == 0) {
-    const uint64_t b = wave_kth(gmax[lane], p.k);
+    const uint32_t b = wave_kth(gmax[lane], p.k);
     if (lane == 0) bound_s = b;
   }
   __syncthreads();
-  const uint64_t bound = max(bound_s, uint64_t(1));
-  auto list = [&](uint64_t o, int j) __attribute__((always_inline)) {
+  const uint64_t bound = max(uint64_t(bound_s) << 32, uint64_t(1));
+  auto list = [&](uint64_t o, uint64_t at) __attribute__((always_inline)) {
     const int c = atomicAdd(&count, 1);
-    if (c < BEAM_LIST) lv[c] = o, li[c] = uint32_t(j);
+    if (c < BEAM_LIST) lv[c] = o, la[c] = at;
   };
 #pragma unroll
-  for (int u = 0; u < BEAM_HELD; ++u)
-    if (bits[u] >= bound) list(bits[u], t + 1024 * u);
+  for (int u = 0; u < BEAM_HELD; ++u) {
+    if (1024 * u >= total) break;
+    if (bits[u] >= bound) list(bits[u], place[u]);
+  }
   for (int j = t + 1024 * BEAM_HELD; j < total; j += 1024) {
     uint64_t o, at;
-    if (get(j, o, at) && o >= bound) list(o, j);
+    if (score(j, cand[j], o, at) && o >= bound) list(o, at);
   }
   __syncthreads();
-  auto store = [&](int r, int j) __attribute__((always_inline)) {
-    uint64_t o, at;
-    get(j, o, at);
-    const int i = j / per;
+  auto store = [&](int r, uint64_t o, uint64_t at) __attribute__((always_inline)) {
     const uint64_t b = o == ~0ull ? 0x7ff8000000000000ull : (o >> 63 ? o & 0x7fffffffffffffffull : ~o);
     p.out_score[int64_t(grp) * p.k + r] = float(__longlong_as_double((long long)b));
-    p.out_beam[int64_t(grp) * p.k + r] = i;
-    p.out_tok[int64_t(grp) * p.k + r] = int64_t(at - uint64_t(i) * uint64_t(p.V));
+    p.out_beam[int64_t(grp) * p.k + r] = int64_t(at >> 32);
+    p.out_tok[int64_t(grp) * p.k + r] = int64_t(uint32_t(at));
   };
   const int nc = count;
   if (nc <= BEAM_LIST) {
     for (int a = t; a < nc; a += 1024) {
-      uint64_t o, at;
-      get(int(li[a]), o, at);
+      const uint64_t o = lv[a], at = la[a];
       int rank = 0;
       for (int c = 0; c < nc; ++c) {
-        bool first = lv[c] > o;
-        if (lv[c] == o && c != a) {
-          uint64_t oo, oat;
-          get(int(li[c]), oo, oat);
-          first = oat < at;
-        }
-        rank += first ? 1 : 0;
+        const uint64_t oc = lv[c], ac = la[c];
+        rank += (oc > o || (oc == o && ac < at)) ? 1 : 0;
       }
-      if (rank < p.k) store(rank, int(li[a]));
+      if (rank < p.k) store(rank, o, at);
     }
     return;
   }
   // one by one: the best after the last one taken
   __shared__ uint64_t sv[16], sa[16];
-  __shared__ int sj[16];
   uint64_t last = 0, lastat = 0;
   for (int r = 0; r < p.k; ++r) {
-    uint64_t b = 0, ba = ~0ull;
-    int bj = -1;
+    uint64_t b = 0, ba = ~0ull;  // (below every candidate)
     for (int j = t; j < total; j += 1024) {
       uint64_t o, at;
-      if (!get(j, o, at)) continue;
+      if (!score(j, cand[j], o, at)) continue;
       if (r > 0 && !(o < last || (o == last && at > lastat))) continue;
-      if (bj < 0 || o > b || (o == b && at < ba)) b = o, ba = at, bj = j;
+      if (o > b || (o == b && at < ba)) b = o, ba = at;
     }
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) {
       const uint64_t ob = __shfl_xor(b, x, 64), oa = __shfl_xor(ba, x, 64);
-      const int oj = __shfl_xor(bj, x, 64);
-      if (oj >= 0 && (bj < 0 || ob > b || (ob == b && oa < ba))) b = ob, ba = oa, bj = oj;
+      if (ob > b || (ob == b && oa < ba)) b = ob, ba = oa;
     }
     __syncthreads();
-    if (lane == 0) sv[wave] = b, sa[wave] = ba, sj[wave] = bj;
+    if (lane == 0) sv[wave] = b, sa[wave] = ba;
     __syncthreads();
-    b = sv[0], ba = sa[0], bj = sj[0];
+    b = sv[0], ba = sa[0];
     for (int w = 1; w < 16; ++w)
-      if (sj[w] >= 0 && (bj < 0 || sv[w] > b || (sv[w] == b && sa[w] < ba))) b = sv[w], ba = sa[w], bj = sj[w];
-    if (t == 0) store(r, bj);
+      if (sv[w] > b || (sv[w] == b && sa[w] < ba)) b = sv[w], ba = sa[w];
+    if (t == 0) store(r, b, ba);
     last = b, lastat = ba;
   }
 }
