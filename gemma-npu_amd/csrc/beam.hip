@@ -50,9 +50,6 @@ __device__ __forceinline__ uint64_t order_bits(double x) {
 
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int j) { return uint32_t(__builtin_amdgcn_readlane(int(v), j)); }
 __device__ __forceinline__ float lane_value(float v, int j) { return __uint_as_float(lane_value(__float_as_uint(v), j)); }
-__device__ __forceinline__ uint64_t lane_value(uint64_t v, int j) {
-  return uint64_t(lane_value(uint32_t(v), j)) | (uint64_t(lane_value(uint32_t(v >> 32), j)) << 32);
-}
 
 // The k-th largest of 64 lanes' values (k <= 64, none of them NaN): the value whose rank, ties by lane, is k - 1.
 template <class T>
