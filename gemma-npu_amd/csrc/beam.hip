@@ -8,12 +8,14 @@
 // beam_chunk_kernel reads the logits once.  A workgroup takes a run of 256 E logits of one beam into registers,
 // makes their maximum and sum of exponentials, and finds its k largest: the k-th largest of the maxima of 64
 // lane groups is a bound that at least k logits reach and few more do, so those are listed and ranked by
-// counting.  Where too many reach it (equal logits, as a grammar's -inf), or there is a NaN, the k are taken
-// one by one instead.  Within a beam the order of logits is the order of scores, so nothing else can be among
-// the k best.  beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k
-// best of those lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and
-// the choice between them has to be right.  The logits' way through memory bounds large calls (64 beams of
-// 262144 fp32 logits: 43 -> 28 us, 67 MB), two kernels' starts and barriers small ones (4 beams of bf16: 20 -> 13.5 us).
+// counting.  Where too many reach it (equal logits), or there is a NaN, the k are taken one by one instead.
+// Within a beam the order of logits is the order of scores, so nothing else can be among the k best.
+// beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k best of those
+// lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and the choice
+// between them has to be right.  Where too many reach its bound (k near 64, beams far apart) the listed ones
+// give a tighter one: 64 of 64 beams of 32000 one by one 1189 us, so 148.  The logits' way through memory bounds
+// large calls (64 beams of 262144 fp32 logits: 43 -> 29 us, 67 MB), two kernels' starts and barriers small ones
+// (4 beams of bf16: 20 -> 14 us).
 #include <algorithm>
 
 #include "w8a8_common.h"
@@ -22,7 +24,8 @@ namespace w8a8 {
 
 constexpr int BEAM_MAX_K = 64;
 constexpr int BEAM_MAX_BEAMS = 256;
-constexpr int BEAM_LIST = 512;              // most candidates that are ranked by counting
+constexpr int BEAM_LIST = 1024;             // most candidates that are ranked by counting
+constexpr int BEAM_ROUNDS = 8;              // most times that the join tightens its bound
 constexpr int BEAM_HELD = 8;                // candidates that a thread of the join keeps in registers
 
 struct BeamParams {
@@ -163,20 +166,28 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
   s = (red2[0] + red2[1]) + (red2[2] + red2[3]);  // NaN with a NaN or +inf among the logits
   // the sum against exp2(mref), a rounded exponent: against the maximum itself
   const float scale = __builtin_amdgcn_exp2f(__builtin_fmaf(-top, l2e, mref));
-  const float bound = bound_s;  // (-inf where fewer than k groups hold any)
-  const bool plain = s == s && bound > -__builtin_inff();
-  if (plain && m >= bound) {
+  const float bound = bound_s;
+  const bool plain = s == s;
+  auto list = [&](int e) __attribute__((always_inline)) {
+    const int at = atomicAdd(&count, 1);
+    if (at < BEAM_LIST) lv[at] = order_bits(v[e]), li[at] = index(e);
+  };
+  if (plain && bound > -__builtin_inff()) {
+    if (m >= bound)
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (v[e] >= bound) {
-        const int at = atomicAdd(&count, 1);
-        if (at < BEAM_LIST) lv[at] = order_bits(v[e]), li[at] = index(e);
-      }
+      for (int e = 0; e < E; ++e)
+        if (v[e] >= bound) list(e);
+  } else if (plain) {
+    // fewer than k groups hold more than -inf (a grammar's mask, a short vocabulary): all that is above it, and
+    // of the rest the first k logits hold as many as can be among the best
+    if (m > -__builtin_inff() || 8 * t < p.k)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (v[e] > -__builtin_inff() || (valid(e) && int(index(e)) - base < p.k)) list(e);
   }
   __syncthreads();
-  const int64_t slot = int64_t(row) * p.nch + ch;
-  if (t == 0) p.stat[slot] = make_float2(top, top == -__builtin_inff() ? s : s * scale);
-  uint2* out = p.cand + slot * p.k;
+  if (t == 0) p.stat[int64_t(row) * p.nch + ch] = make_float2(top, top == -__builtin_inff() ? s : s * scale);
+  uint2* out = p.cand + (int64_t(row) * p.nch + ch) * p.k;
   const int nc = count;
   auto value = [&](uint32_t o) __attribute__((always_inline)) {  // the logit's bits again (NaN: the quiet one)
     return o == 0xffffffffu ? 0x7fc00000u : (o & 0x80000000u ? o & 0x7fffffffu : ~o);
@@ -188,6 +199,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
       for (int c = 0; c < nc; ++c) rank += before(lv[c], li[c], a, ai) ? 1 : 0;
       if (rank < p.k) out[rank] = make_uint2(value(a), ai);
     }
+    for (int j = nc + t; j < p.k; j += 256) out[j] = make_uint2(0x7fc00000u, 0xffffffffu);  // (none left)
     return;
   }
   // one by one: the best after the last one taken
@@ -214,7 +226,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int grp = blockIdx.x;
   const int per = p.nch * p.k, total = p.nb * per;
-  const uint2* cand = p.cand + int64_t(grp) * p.nb * per;
+  const uint2* cand = p.cand + int64_t(grp) * total;
   // the first candidates are asked for before the beams' sums are made
   uint2 held[BEAM_HELD];
 #pragma unroll
@@ -273,7 +285,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     uint64_t o, at;
     if (score(j, cand[j], o, at)) top = max(top, o);
   }
-  // the bound: of the scores' upper halves
+  // the bound: of the upper halves of the best scores of 64 groups
   uint32_t high = uint32_t(top >> 32);
 #pragma unroll
   for (int x = 8; x > 0; x >>= 1) high = max(high, uint32_t(__shfl_xor(high, x, 64)));
@@ -284,28 +296,43 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     if (lane == 0) bound_s = b;
   }
   __syncthreads();
-  const uint64_t bound = max(uint64_t(bound_s) << 32, uint64_t(1));
+  uint64_t bound = max(uint64_t(bound_s) << 32, uint64_t(1));
   auto list = [&](uint64_t o, uint64_t at) __attribute__((always_inline)) {
     const int c = atomicAdd(&count, 1);
     if (c < BEAM_LIST) lv[c] = o, la[c] = at;
   };
+  int nc;
+  for (int round = 0;; ++round) {
 #pragma unroll
-  for (int u = 0; u < BEAM_HELD; ++u) {
-    if (1024 * u >= total) break;
-    if (bits[u] >= bound) list(bits[u], place[u]);
+    for (int u = 0; u < BEAM_HELD; ++u) {
+      if (1024 * u >= total) break;
+      if (bits[u] >= bound) list(bits[u], place[u]);
+    }
+    for (int j = t + 1024 * BEAM_HELD; j < total; j += 1024) {
+      uint64_t o, at;
+      if (score(j, cand[j], o, at) && o >= bound) list(o, at);
+    }
+    __syncthreads();
+    nc = count;
+    if (nc <= BEAM_LIST || round == BEAM_ROUNDS) break;
+    // too many (a group without any of the best beams): the same bound of those that were listed
+    if (wave == 0) {
+      uint32_t high = 0;
+      for (int c = lane; c < BEAM_LIST; c += 64) high = max(high, uint32_t(lv[c] >> 32));
+      const uint32_t b = wave_kth(high, p.k);
+      if (lane == 0) bound_s = b, count = 0;
+    }
+    __syncthreads();
+    const uint64_t tighter = uint64_t(bound_s) << 32;
+    if (tighter <= bound) break;  // (equal scores)
+    bound = tighter;
   }
-  for (int j = t + 1024 * BEAM_HELD; j < total; j += 1024) {
-    uint64_t o, at;
-    if (score(j, cand[j], o, at) && o >= bound) list(o, at);
-  }
-  __syncthreads();
   auto store = [&](int r, uint64_t o, uint64_t at) __attribute__((always_inline)) {
     const uint64_t b = o == ~0ull ? 0x7ff8000000000000ull : (o >> 63 ? o & 0x7fffffffffffffffull : ~o);
     p.out_score[int64_t(grp) * p.k + r] = float(__longlong_as_double((long long)b));
     p.out_beam[int64_t(grp) * p.k + r] = int64_t(at >> 32);
     p.out_tok[int64_t(grp) * p.k + r] = int64_t(uint32_t(at));
   };
-  const int nc = count;
   if (nc <= BEAM_LIST) {
     for (int a = t; a < nc; a += 1024) {
       const uint64_t o = lv[a], at = la[a];

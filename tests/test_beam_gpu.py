@@ -60,6 +60,7 @@ def make(B, nb, V, dtype, seed, spread=3.0):
     # B, nb, V, k
     (1, 1, 1, 1), (1, 1, 7, 7), (1, 2, 5, 10), (1, 4, 1000, 8), (3, 5, 8192, 16), (2, 3, 8193, 64), (1, 16, 20001, 64),
     (1, 4, 262144, 8), (2, 8, 32003, 16), (5, 1, 4096, 5), (1, 64, 3001, 32), (1, 200, 100, 64), (1, 3, 65537, 1),
+    (1, 64, 32000, 64), (2, 256, 2000, 64), (1, 8, 262144, 64), (1, 100, 12345, 40),
 ], ids=lambda s: "x".join(map(str, s)))
 def test_matches_the_definition(shape, dtype):
     B, nb, V, k = shape
@@ -103,6 +104,19 @@ def test_masked_tokens_and_beams(V, dtype):
     y = x.clone()
     y[:, :, ::2] = torch.finfo(torch.bfloat16 if dtype == "bf16" else torch.float32).min
     check(cast(y), s, 12, "lowest value")
+
+
+@pytest.mark.parametrize("V,allowed", [(8192, 1), (8192, 7), (262144, 40), (70, 3)])
+def test_a_grammar_with_few_tokens(V, allowed):
+    """Less tokens than are asked for in each chunk, the allowed ones among the first or the last."""
+    for seed in range(3):
+        x, s = make(1, 3, V, "fp32", seed=V + seed)
+        at = torch.randperm(V, generator=torch.Generator().manual_seed(seed))[:allowed]
+        at = at if seed == 0 else at % 64 if seed == 1 else V - 1 - at % 64
+        y = torch.full_like(x, -math.inf)
+        y[:, :, at] = x[:, :, at]
+        for k in (1, 8, 64):
+            check(y, s, k, f"{V} {allowed} {seed} {k}")
 
 
 def test_nan_and_infinite_logits():
