@@ -13,9 +13,9 @@
 // beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k best of those
 // lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and the choice
 // between them has to be right.  Where too many reach its bound (k near 64, beams far apart) the listed ones
-// give a tighter one: 64 of 64 beams of 32000 one by one 1189 us, so 148.  The logits' way through memory bounds
-// large calls (64 beams of 262144 fp32 logits: 43 -> 29 us, 67 MB), two kernels' starts and barriers small ones
-// (4 beams of bf16: 20 -> 14 us).
+// give a tighter one: 64 of 64 beams of 32000 one by one 1189 us, so 125.  The logits' way through memory bounds
+// large calls (64 beams of 262144 fp32 logits: 43 -> 28 us, 67 MB), two kernels' starts and barriers small ones
+// (4 beams of bf16: 20 -> 13 us).
 #include <algorithm>
 
 #include "w8a8_common.h"
@@ -71,7 +71,7 @@ __device__ __forceinline__ T wave_kth(T v, int k) {
 // A candidate before another: larger, or equal and of the lower index.
 template <class T>
 __device__ __forceinline__ bool before(T a, uint32_t ai, T b, uint32_t bi) {
-  return a > b || (a == b && ai < bi);
+  return (a > b) | ((a == b) & (ai < bi));  // (no branch: both are read at once)
 }
 
 // The best of a workgroup's candidates, given to every thread.
@@ -104,14 +104,17 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
   const int row = blockIdx.x / p.nch, ch = blockIdx.x % p.nch;
   const X* xp = static_cast<const X*>(p.x) + int64_t(row / p.nb) * p.gs + int64_t(row % p.nb) * p.rs;
   const int base = ch * CHUNK, n = min(CHUNK, p.V - base);
-  // element e of thread t is logit base + 8 (t + 256 (e / 8)) + e % 8; past the last one -inf
+  // element e of thread t is logit base + 8 (t + 256 (e / 8)) + e % 8, or where that leaves lane groups without
+  // any base + t + 256 e; past the last one -inf
   float v[E];
+  const bool thin = n <= 2048;
   const bool wide = (reinterpret_cast<uintptr_t>(xp) & 15) == 0;
+  auto local = [&](int e) __attribute__((always_inline)) { return thin ? t + 256 * e : 8 * (t + 256 * (e >> 3)) + (e & 7); };
 #pragma unroll
   for (int c = 0; c < E / 8; ++c) {
     const int at = 8 * (t + 256 * c);
     const X* src = xp + base + at;
-    if (wide && at + 8 <= n) {
+    if (!thin && wide && at + 8 <= n) {
       if constexpr (sizeof(X) == 2) {
         float f[8];
         unpack8(*reinterpret_cast<const v4u*>(src), f);
@@ -126,18 +129,19 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float f = -__builtin_inff();
-        if (at + e < n) {
+        const int i = local(8 * c + e);
+        if (i < n) {
           if constexpr (sizeof(X) == 2)
-            f = bf16_to_f32(src[e]);
+            f = bf16_to_f32(xp[base + i]);
           else
-            f = src[e];
+            f = xp[base + i];
         }
         v[8 * c + e] = f;
       }
     }
   }
-  auto valid = [&](int e) __attribute__((always_inline)) { return 8 * (t + 256 * (e >> 3)) + (e & 7) < n; };
-  auto index = [&](int e) __attribute__((always_inline)) { return uint32_t(base + 8 * (t + 256 * (e >> 3)) + (e & 7)); };
+  auto valid = [&](int e) __attribute__((always_inline)) { return local(e) < n; };
+  auto index = [&](int e) __attribute__((always_inline)) { return uint32_t(base + local(e)); };
 
   // the maximum (fmaxf passes NaN over), and those of groups of four lanes
   float m = -__builtin_inff();
@@ -180,10 +184,10 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
   } else if (plain) {
     // fewer than k groups hold more than -inf (a grammar's mask, a short vocabulary): all that is above it, and
     // of the rest the first k logits hold as many as can be among the best
-    if (m > -__builtin_inff() || 8 * t < p.k)
+    if (m > -__builtin_inff() || t < p.k)
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (v[e] > -__builtin_inff() || (valid(e) && int(index(e)) - base < p.k)) list(e);
+        if (v[e] > -__builtin_inff() || (valid(e) && local(e) < p.k)) list(e);
   }
   __syncthreads();
   if (t == 0) p.stat[int64_t(row) * p.nch + ch] = make_float2(top, top == -__builtin_inff() ? s : s * scale);
@@ -196,7 +200,11 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
     for (int j = t; j < nc; j += 256) {
       int rank = 0;
       const uint32_t a = lv[j], ai = li[j];
-      for (int c = 0; c < nc; ++c) rank += before(lv[c], li[c], a, ai) ? 1 : 0;
+#pragma unroll 8
+      for (int c = 0; c < nc; ++c) {
+        const uint32_t o = lv[c], oi = li[c];
+        rank += before(o, oi, a, ai) ? 1 : 0;
+      }
       if (rank < p.k) out[rank] = make_uint2(value(a), ai);
     }
     for (int j = nc + t; j < p.k; j += 256) out[j] = make_uint2(0x7fc00000u, 0xffffffffu);  // (none left)
@@ -337,9 +345,10 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     for (int a = t; a < nc; a += 1024) {
       const uint64_t o = lv[a], at = la[a];
       int rank = 0;
+#pragma unroll 8
       for (int c = 0; c < nc; ++c) {
         const uint64_t oc = lv[c], ac = la[c];
-        rank += (oc > o || (oc == o && ac < at)) ? 1 : 0;
+        rank += (oc > o) | ((oc == o) & (ac < at)) ? 1 : 0;
       }
       if (rank < p.k) store(rank, o, at);
     }
