@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
 //   evict_least_kernel   one workgroup per KV head finds the key among those, and what is before each chunk
 //   evict_list_kernel    the lists of free places and moving rows, chunk by chunk
 // and evict_move_kernel copies the rows.  A cache that is cut by a few rows (EVICT_FEW, as at every step of a
-// cache that is full) is one launch of evict_few_kernel, which takes the rows that go one by one.  Loops are not unrolled over a thread's rows: a workgroup runs
+// cache that is full) goes without that: the rows that go are taken one by one (evict_few_kernel).  Loops are not unrolled over a thread's rows: a workgroup runs
 // through such code once, and fetching it took longer than the work (65521 rows of 8 heads with the keys in
 // registers 84 us for the select alone, 242 us reading them again at each step; in chunks 34).
 
@@ -273,54 +273,23 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictParams p) {
   if (wave == EVICT_NW - 1 && lane == 0) p.count[g] = hole;
 }
 
-// One workgroup per KV head and a launch for everything, where at most EVICT_FEW rows go.  A thread holds E rows
-// in registers; the row of the least key (ties: the highest) goes, as often as rows have to.  Each choice is a
-// minimum over the workgroup, which bounds it (1.2 us): of 4097 rows of head_dim 512 one goes in 5.3 us, four in
-// 9.1, eight would in 13.9; the radix select and the launch that moves the rows take 13.8 whatever goes (of 512
-// rows 9.4 against 7.7 for four and 11.8 for eight, of 16384 28 against 13 and 19).
-template <int E>
-__global__ __launch_bounds__(1024) void evict_few_kernel(EvictParams p) {
-  __shared__ uint64_t least[2][EVICT_NW];
-  __shared__ int red[EVICT_NW], out[EVICT_FEW], hole[EVICT_FEW], mover[EVICT_FEW];
-  const int t = threadIdx.x, wave = t >> 6, g = blockIdx.x, n = p.n, budget = p.budget, drop = n - budget;
-  const float* w = p.w + int64_t(g) * p.whs;
-  const int32_t* pos = p.pos + int64_t(g) * p.phs;
-  float x[E];
-  int32_t y[E];
-  int newest = INT32_MIN;
+// A row's key and, less for higher rows, its place: of equal keys the highest row goes first.
+__device__ __forceinline__ uint64_t evict_place(uint32_t key, int row) { return uint64_t(key) << 32 | uint32_t(~row); }
+
+// The least of v over the workgroup's 1024 threads (buf [16], not in use by others until the next barrier after).
+__device__ __forceinline__ uint64_t evict_min(uint64_t v, uint64_t* buf) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int r = t + 1024 * e;
-    x[e] = r < n ? w[r] : 0.0f;
-    y[e] = r < n ? pos[r] : INT32_MIN;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) newest = max(newest, y[e]);
-  const int64_t old = int64_t(evict_max(newest, red)) - p.recent;
-  uint32_t key[E], gone = 0;  // and this thread's rows that are not there
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    key[e] = evict_key(x[e], y[e], old);
-    gone |= t + 1024 * e < n ? 0u : 1u << e;
-  }
-#pragma unroll 1
-  for (int j = 0; j < drop; ++j) {
-    // the least key and, less for higher rows, its place (at least two rows are left: none is ~0 but the last)
-    uint64_t m = ~0ull;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (!(gone >> e & 1u)) m = min(m, uint64_t(key[e]) << 32 | uint32_t(~(t + 1024 * e)));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = min(m, uint64_t(__shfl_xor(m, o, 64)));
-    if ((t & 63) == 0) least[j & 1][wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < EVICT_NW; ++i) m = min(m, least[j & 1][i]);
-    const int r = int(~uint32_t(m));
-    if ((r & 1023) == t) gone |= 1u << (r >> 10);
-    if (t == 0) out[j] = r;
-  }
+  for (int o = 32; o > 0; o >>= 1) v = min(v, uint64_t(__shfl_xor(v, o, 64)));
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < EVICT_NW; ++i) v = min(v, buf[i]);
+  return v;
+}
+
+// With the rows that go (out [n - budget] in LDS): the rows that move, and where to.  Called by 1024 threads.
+__device__ __forceinline__ void evict_few_move(const EvictParams& p, int g, const int* out, int* hole, int* mover) {
+  const int t = threadIdx.x, budget = p.budget, drop = p.n - budget;
   // free places and the rows that fill them, both in row order: thread j < drop ranks out[j] and row budget + j
   int nhole = 0;
   for (int j = 0; j < drop; ++j) nhole += out[j] < budget ? 1 : 0;
@@ -335,14 +304,6 @@ __global__ __launch_bounds__(1024) void evict_few_kernel(EvictParams p) {
     if (out[t] < budget) hole[before] = out[t];
     if (stays) mover[t - moves] = budget + t;
   }
-  int32_t* const ko = p.kept + int64_t(g) * p.khs;
-  float* const wo = p.w_out + int64_t(g) * p.wos;
-  int32_t* const po = p.pos_out + int64_t(g) * p.pos_os;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int r = t + 1024 * e;
-    if (r < budget && !(gone >> e & 1u)) ko[r] = r, wo[r] = x[e], po[r] = y[e];
-  }
   __syncthreads();
   char* const k = p.k + int64_t(g) * p.kh;
   char* const v = p.v + int64_t(g) * p.vh;
@@ -353,8 +314,65 @@ __global__ __launch_bounds__(1024) void evict_few_kernel(EvictParams p) {
     const v4u b = *reinterpret_cast<const v4u*>(v + src * p.vr + c);
     *reinterpret_cast<v4u*>(k + dst * p.kr + c) = a;
     *reinterpret_cast<v4u*>(v + dst * p.vr + c) = b;
-    if (col == 0) ko[dst] = int32_t(src), wo[dst] = w[src], po[dst] = pos[src];
+    if (col == 0) {
+      p.kept[int64_t(g) * p.khs + dst] = int32_t(src);
+      p.w_out[int64_t(g) * p.wos + dst] = p.w[int64_t(g) * p.whs + src];
+      p.pos_out[int64_t(g) * p.pos_os + dst] = p.pos[int64_t(g) * p.phs + src];
+    }
   }
+}
+
+// One workgroup per KV head and a launch for everything, where at most EVICT_FEW rows go.  A thread holds E rows
+// in registers; the row of the least key (ties: the highest) goes, as often as rows have to.  Each choice is a
+// minimum over the workgroup, which bounds it (1.2 us): of 4097 rows of head_dim 512 one goes in 5.3 us, four in
+// 9.1, eight would in 13.9; the radix select and the launch that moves the rows take 13.8 whatever goes (of 512
+// rows 9.4 against 7.7 for four and 11.8 for eight, of 16384 28 against 13 and 19).
+template <int E>
+__global__ __launch_bounds__(1024) void evict_few_kernel(EvictParams p) {
+  __shared__ uint64_t least[2][EVICT_NW];
+  __shared__ int red[EVICT_NW], out[EVICT_FEW], hole[EVICT_FEW], mover[EVICT_FEW];
+  const int t = threadIdx.x, g = blockIdx.x, n = p.n, budget = p.budget, drop = n - budget;
+  const float* w = p.w + int64_t(g) * p.whs;
+  const int32_t* pos = p.pos + int64_t(g) * p.phs;
+  float x[E];
+  int32_t y[E];
+  int newest = INT32_MIN;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int r = t + 1024 * e;
+    x[e] = r < n ? w[r] : 0.0f;
+    y[e] = r < n ? pos[r] : INT32_MIN;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) newest = max(newest, y[e]);
+  const int64_t old = int64_t(evict_max(newest, red)) - p.recent;
+  uint32_t key[E], gone = 0;  // (this thread's rows that are not there)
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    key[e] = evict_key(x[e], y[e], old);
+    gone |= t + 1024 * e < n ? 0u : 1u << e;
+  }
+#pragma unroll 1
+  for (int j = 0; j < drop; ++j) {
+    uint64_t m = ~0ull;  // (at least two rows are left: none is ~0 but the last)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (!(gone >> e & 1u)) m = min(m, evict_place(key[e], t + 1024 * e));
+    const int r = int(~uint32_t(evict_min(m, least[j & 1])));
+    if ((r & 1023) == t) gone |= 1u << (r >> 10);
+    if (t == 0) out[j] = r;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int r = t + 1024 * e;
+    if (r < budget && !(gone >> e & 1u)) {
+      p.kept[int64_t(g) * p.khs + r] = r;
+      p.w_out[int64_t(g) * p.wos + r] = x[e];
+      p.pos_out[int64_t(g) * p.pos_os + r] = y[e];
+    }
+  }
+  __syncthreads();
+  evict_few_move(p, g, out, hole, mover);
 }
 
 // A chunk's rows of thread t: chunk * 4096 + 256 (t / 64) + t % 64, + 64, + 128, + 192.
@@ -598,6 +616,60 @@ __global__ __launch_bounds__(1024) void evict_list_kernel(EvictParams p) {
   }
 }
 
+// Long caches of which a few rows go: each chunk's least rows, then the least of those (of 65521 rows of 8 heads of
+// 128 one in 10.6 us, six in 21.5, seven by the digits in 32.9).
+__global__ __launch_bounds__(1024) void evict_few_chunk_kernel(EvictParams p) {
+  __shared__ uint64_t least[2][EVICT_NW];
+  __shared__ int red[EVICT_NW];
+  const int c = blockIdx.x, g = blockIdx.y, drop = p.n - p.budget;
+  const EvictRows x = evict_rows(p, g, c);
+  const int64_t old = evict_old(p, g, red);
+  uint64_t place[4], from = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = x.row0 + 64 * e;
+    place[e] = r < p.n ? evict_place(evict_key(x.w[e], x.pos[e], old), r) : ~0ull;
+    if (r < p.budget) {  // (the rows that go are overwritten by the next kernel)
+      p.kept[int64_t(g) * p.khs + r] = r;
+      p.w_out[int64_t(g) * p.wos + r] = x.w[e];
+      p.pos_out[int64_t(g) * p.pos_os + r] = x.pos[e];
+    }
+  }
+  uint32_t* const open = p.open + (int64_t(g) * p.nch + c) * EVICT_CHUNK;
+#pragma unroll 1
+  for (int j = 0; j < drop; ++j) {
+    uint64_t m = ~0ull;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (place[e] >= from) m = min(m, place[e]);
+    m = evict_min(m, least[j & 1]);
+    if (threadIdx.x == 0) open[2 * j] = uint32_t(m), open[2 * j + 1] = uint32_t(m >> 32);
+    from = m == ~0ull ? m : m + 1;  // (no two are alike; ~0: none is left)
+  }
+}
+
+__global__ __launch_bounds__(1024) void evict_few_last_kernel(EvictParams p) {
+  __shared__ uint64_t least[2][EVICT_NW];
+  __shared__ int out[EVICT_FEW], hole[EVICT_FEW], mover[EVICT_FEW];
+  const int t = threadIdx.x, g = blockIdx.x, drop = p.n - p.budget;
+  const uint32_t* const open = p.open + int64_t(g) * p.nch * EVICT_CHUNK;
+  uint64_t from = 0;
+#pragma unroll 1
+  for (int j = 0; j < drop; ++j) {
+    uint64_t m = ~0ull;
+    for (int i = t; i < p.nch * drop; i += 1024) {
+      const uint32_t* const o = open + int64_t(i / drop) * EVICT_CHUNK + 2 * (i % drop);
+      const uint64_t v = uint64_t(o[1]) << 32 | o[0];
+      if (v >= from) m = min(m, v);
+    }
+    m = evict_min(m, least[j & 1]);
+    if (t == 0) out[j] = int(~uint32_t(m));
+    from = m + 1;
+  }
+  __syncthreads();
+  evict_few_move(p, g, out, hole, mover);
+}
+
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictParams p) {
   const int g = blockIdx.y;
   const int64_t total = int64_t(p.count[g]) * p.row_cols;
@@ -753,13 +825,19 @@ extern "C" int w8a8_evict(void* k, int64_t k_head_stride, int64_t k_row_stride, 
   p.k = static_cast<char*>(k); p.kh = k_head_stride; p.kr = k_row_stride;
   p.v = static_cast<char*>(v); p.vh = v_head_stride; p.vr = v_row_stride;
   p.row_cols = int(row_bytes / 16);
-  if (p.nch == 0 && n > budget && n - budget <= EVICT_FEW && (n - budget) * p.row_cols <= EVICT_FEW_COLS) {
-    if (n <= 4 * 1024)
+  if (n > budget && n - budget <= EVICT_FEW && (n - budget) * p.row_cols <= EVICT_FEW_COLS) {
+    if (p.nch > 0) {
+      const dim3 grid{unsigned(p.nch), unsigned(KV), 1};
+      evict_newest_kernel<<<grid, 1024, 0, stream>>>(p);
+      evict_few_chunk_kernel<<<grid, 1024, 0, stream>>>(p);
+      evict_few_last_kernel<<<unsigned(KV), 1024, 0, stream>>>(p);
+    } else if (n <= 4 * 1024) {
       evict_few_kernel<4><<<unsigned(KV), 1024, 0, stream>>>(p);
-    else if (n <= 8 * 1024)
+    } else if (n <= 8 * 1024) {
       evict_few_kernel<8><<<unsigned(KV), 1024, 0, stream>>>(p);
-    else
+    } else {
       evict_few_kernel<16><<<unsigned(KV), 1024, 0, stream>>>(p);
+    }
     return check_launch(what);
   }
   if (p.nch == 0) {

@@ -176,7 +176,8 @@ def run_evict(k, v, w, pos, n, budget, recent, **kw):
     # few rows go
     (1, 3, 3, 128, 1, 1), (2, 9, 9, 64, 1, 0), (1, 10, 10, 64, 1, 1), (1, 16, 12, 64, 7, 3), (3, 1000, 1000, 128, 995, 64), (1, 4096, 4096, 64, 4095, 0),
     (2, 4100, 4097, 512, 4089, 1024), (1, 8192, 8192, 128, 8190, 8190), (2, 8193, 8193, 64, 8186, 100), (1, 16384, 16384, 128, 16383, 17),
-    (1, 500, 500, 4096, 497, 5), (1, 500, 500, 4096, 493, 5),
+    (1, 500, 500, 4096, 497, 5), (1, 500, 500, 4096, 493, 5), (1, 20480, 20480, 64, 20474, 7), (2, 33333, 33333, 64, 33332, 33332),
+    (3, 40000, 36870, 64, 36865, 0), (1, 20000, 20000, 4096, 19998, 5), (1, 17000, 17000, 4096, 16994, 5),
 ], ids=lambda c: "x".join(map(str, c)))
 def test_evict_matches_the_definition(case):
     KV, rows, n, D, budget, recent = case
