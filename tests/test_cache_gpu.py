@@ -233,6 +233,46 @@ def test_evict_strided_in_place_and_other_types():
     run_evict(rand((1, 90, 36), torch.float32, 1), rand((1, 90, 36), torch.float32, 2), torch.rand(1, 90), pos[:1, :90].clone(), 90, 33, 7)
 
 
+@pytest.mark.parametrize("n,few", [(70, 1), (5000, 5), (20000, 6), (20000, 9000)])
+def test_evict_step_by_step_in_place(n, few):
+    """A full cache cut at every step, its weights and positions in place, with the caller's scratch, eager and replayed
+    from a graph."""
+    KV, D, recent, budget = 2, 64, 9, n - few
+    g = torch.Generator().manual_seed(n + few)
+    k, v = rand((KV, n, D), torch.bfloat16, 1), rand((KV, n, D), torch.bfloat16, 2)
+    w = torch.randint(0, 50, (KV, n), generator=g).float()
+    pos = torch.stack([torch.randperm(n, generator=g) for _ in range(KV)]).int()
+    kd, vd, wd, pd = (t.to(DEV) for t in (k, v, w, pos))
+    kept = torch.empty(KV, budget, dtype=torch.int32, device=DEV)
+    ws = torch.empty(cache.evict_workspace_bytes(KV, n, budget), dtype=torch.uint8, device=DEV)
+
+    def step():
+        cache.evict(kd, vd, wd, pd, n, budget, recent, out=(kept, wd[:, :budget], pd[:, :budget]), workspace=ws)
+
+    stream = torch.cuda.Stream()
+    graph = None
+    for i in range(4):
+        want = [evicted(w[h], pos[h], n, budget, recent) for h in range(KV)]
+        for t, d in ((k, kd), (v, vd), (w, wd), (pos, pd)):
+            for h in range(KV):
+                t[h, :budget] = t[h, want[h]]
+        if i == 1:
+            stream.wait_stream(torch.cuda.current_stream())
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step()
+        step() if graph is None else graph.replay()
+        torch.cuda.synchronize()
+        assert kept.tolist() == want, i
+        for t, d in ((k, kd), (v, vd), (w, wd), (pos, pd)):
+            assert torch.equal(d.cpu(), t), i
+        # new rows behind the budget
+        w[:, budget:] = torch.randint(0, 50, (KV, few), generator=g).float()
+        pos[:, budget:] = n + i * few + torch.arange(few, dtype=torch.int32)
+        wd.copy_(w)
+        pd.copy_(pos)
+
+
 def test_evict_past_32_bit_offsets():
     """One head's rows span more than 4 GiB."""
     n, step = 70_000, 65536
