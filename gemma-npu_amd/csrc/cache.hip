@@ -80,9 +80,10 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
 //   evict_least_kernel   one workgroup per KV head finds the key among those, and what is before each chunk
 //   evict_list_kernel    the lists of free places and moving rows, chunk by chunk
 // and evict_move_kernel copies the rows.  A cache that is cut by a few rows (EVICT_FEW, as at every step of a
-// cache that is full) goes without that: the rows that go are taken one by one (evict_few_kernel).  Loops are not unrolled over a thread's rows: a workgroup runs
-// through such code once, and fetching it took longer than the work (65521 rows of 8 heads with the keys in
-// registers 84 us for the select alone, 242 us reading them again at each step; in chunks 34).
+// cache that is full) goes without that: the rows that go are taken one by one (evict_few_kernel).  Loops are not
+// unrolled over a thread's rows: a workgroup runs through such code once, and fetching it took longer than the
+// work (65521 rows of 8 heads with the keys in registers 84 us for the select alone, 242 us reading them again at
+// each step; in chunks 33).
 
 constexpr int EVICT_NW = 16;
 constexpr int EVICT_ONE = 16384;           // most rows of evict_select_kernel

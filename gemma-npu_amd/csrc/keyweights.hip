@@ -353,8 +353,8 @@ static KeyWeightPlan key_weight_plan(int64_t H, int64_t KV, int64_t Tq, int64_t 
 using namespace w8a8;
 
 static bool key_weight_shape_ok(int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D, int64_t window) {
-  return H >= 1 && KV >= 1 && H % KV == 0 && H <= (1 << 16) && KV <= 65535 && Tq >= 1 && Tk >= Tq && Tk <= INT32_MAX / 2 && window >= 0 &&
-         window <= INT32_MAX / 2 && (D == 128 || D == 256 || D == 512);
+  return H >= 1 && KV >= 1 && H % KV == 0 && H <= (1 << 16) && KV <= 65535 && Tq >= 1 && Tk >= Tq &&
+         Tk <= INT32_MAX / 2 && window >= 0 && window <= INT32_MAX / 2 && (D == 128 || D == 256 || D == 512);
 }
 
 extern "C" int64_t w8a8_attention_key_weights_workspace_bytes(int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D,
