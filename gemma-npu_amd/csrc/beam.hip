@@ -324,6 +324,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     nc = count;
     if (nc <= BEAM_LIST || round == BEAM_ROUNDS) break;
     // too many (a group without any of the best beams): the same bound of those that were listed
+    __syncthreads();  // (every wave has read the count that is cleared)
     if (wave == 0) {
       uint32_t high = 0;
       for (int c = lane; c < BEAM_LIST; c += 64) high = max(high, uint32_t(lv[c] >> 32));
