@@ -160,16 +160,16 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
     const float b = wave_kth(gmax[lane], p.k);
     if (lane == 0) bound_s = b;
   }
-  const float l2e = 1.4426950408889634f, mref = top == -__builtin_inff() ? 0.0f : top * l2e;
+  // exp2((v - top) log2 e): subtracted before it is scaled, so that a term is 1 at the maximum and never above,
+  // however far out the logits are (a mask of the type's lowest value over the whole chunk)
+  const float l2e = 1.4426950408889634f, ref = top == -__builtin_inff() ? 0.0f : top;
   float s = 0.0f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], l2e, -mref));
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - ref) * l2e);
   s = wave_sum(s);
   if (lane == 0) red2[wave] = s;
   __syncthreads();
   s = (red2[0] + red2[1]) + (red2[2] + red2[3]);  // NaN with a NaN or +inf among the logits
-  // the sum against exp2(mref), a rounded exponent: against the maximum itself
-  const float scale = __builtin_amdgcn_exp2f(__builtin_fmaf(-top, l2e, mref));
   const float bound = bound_s;
   const bool plain = s == s;
   auto list = [&](int e) __attribute__((always_inline)) {
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
         if (v[e] > -__builtin_inff() || (valid(e) && local(e) < p.k)) list(e);
   }
   __syncthreads();
-  if (t == 0) p.stat[int64_t(row) * p.nch + ch] = make_float2(top, top == -__builtin_inff() ? s : s * scale);
+  if (t == 0) p.stat[int64_t(row) * p.nch + ch] = make_float2(top, s);
   uint2* out = p.cand + (int64_t(row) * p.nch + ch) * p.k;
   const int nc = count;
   auto value = [&](uint32_t o) __attribute__((always_inline)) {  // the logit's bits again (NaN: the quiet one)

@@ -1,5 +1,5 @@
-"""A beam search step's choice (ops.beam_select) where the join lists more candidates than it ranks at once, against its
-definition in 64 bits.
+"""A beam search step's choice (ops.beam_select) where the join lists more candidates than it ranks at once and where
+logits are finite but far out, against its definition in 64 bits.
 
 Tolerance of a score: `err` for the beam's logsumexp (fp32 terms and sums of a chunk: a few 2^-24 of the sum, below 2e-6 in its
 logarithm) and the rounding to fp32 (half a step, 2^-24 of the value)."""
@@ -47,3 +47,39 @@ def test_the_join_tightens_its_bound_more_than_once(scores):
         s = {"equal": 0 * at, "near": -0.01 * at, "far": -0.5 * at, "farther": -10 * at, "one": torch.where(at == 7, 0.0, -900.0),
              "class": torch.where(torch.arange(nb)[None] % 16 == 0, 0.0, -900.0)}[scores]
         check(x, s, k, f"{scores} {seed}")
+
+
+LOWEST = {"fp32": torch.finfo(torch.float32).min, "bf16": torch.finfo(torch.bfloat16).min}
+
+
+def cast(x, dtype):
+    return x.bfloat16() if dtype == "bf16" else x
+
+
+# B, nb, V: chunks of 4096 logits with a short last one, chunks of 8192, one chunk
+SHAPES = [(1, 3, 12293), (9, 8, 60001), (2, 4, 900)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("mask", ["lowest", -1e30, -1e10])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_whole_chunks_under_a_finite_mask(shape, mask, dtype):
+    """A grammar's mask in finite numbers that leaves a few tokens, all in one chunk: the first, one between, the last."""
+    B, nb, V = shape
+    mask = LOWEST[dtype] if mask == "lowest" else mask
+    for seed, first in enumerate((0, V // 2, V - 30)):
+        g = torch.Generator().manual_seed(V + seed)
+        x = torch.full((B, nb, V), mask)
+        x[:, :, first:first + 30] = torch.randn(B, nb, 30, generator=g) * 3
+        s = -20 * torch.rand(B, nb, generator=g)
+        check(cast(x, dtype), s, 8, f"tokens from {first} on")
+        if mask != -1e10:  # more than there are: the masked tokens' scores are the mask's, the lowest token first
+            check(cast(x[:1, :2], dtype), s[:1, :2], 64, f"60 tokens from {first} on")
+    if V < 4096:
+        return
+    # the short last chunk only
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(B, nb, V, generator=g) * 3
+    x[:, :, V - V % 4096:] = mask
+    s = -20 * torch.rand(B, nb, generator=g)
+    check(cast(x, dtype), s, 8, "the last chunk masked")
