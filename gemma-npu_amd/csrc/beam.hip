@@ -227,7 +227,8 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
 }
 
 __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
-  __shared__ double base_s[BEAM_MAX_BEAMS];
+  __shared__ double log_s[BEAM_MAX_BEAMS], score_s[BEAM_MAX_BEAMS];
+  __shared__ float max_s[BEAM_MAX_BEAMS];
   __shared__ uint64_t lv[BEAM_LIST], la[BEAM_LIST];  // candidates: score's order bits, beam << 32 | token
   __shared__ uint32_t gmax[64], bound_s;
   __shared__ int count;
@@ -240,7 +241,8 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
 #pragma unroll
   for (int u = 0; u < BEAM_HELD; ++u) held[u] = t + 1024 * u < total ? cand[t + 1024 * u] : make_uint2(0u, 0xffffffffu);
   if (t == 0) count = 0;
-  // base[i] = score - logsumexp of beam i, one wave per beam
+  // Each beam's maximum, the logarithm of its sum against that, and its score, one wave per beam.  They are kept apart:
+  // a logit is taken from the maximum first, as log_softmax has it, and logits of any size leave the rest its bits.
   for (int i = wave; i < p.nb; i += 16) {
     const float2* st = p.stat + (int64_t(grp) * p.nb + i) * p.nch;
     float m = -__builtin_inff();
@@ -258,20 +260,21 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
     const double sc = double(p.score[int64_t(grp) * p.ss + i]);
     // no token can follow where all logits are -inf; +inf and NaN make NaN, as log_softmax does
     const double b = m == -__builtin_inff() && s == 0.0 ? (sc != sc ? sc : -__builtin_inf()) : sc - (double(m) + log(s));
-    if (lane == 0) base_s[i] = b;
+    const bool finite = b - b == 0.0;
+    if (lane == 0) max_s[i] = m, log_s[i] = finite ? log(s) : 0.0, score_s[i] = finite ? sc : b;
   }
   __syncthreads();
-  // A candidate's score's order bits and place; false where there is none.  A beam whose base is not finite
-  // has that score for every token: its first tokens stand for it.  (j / per, less than 256, from a product
+  // A candidate's score's order bits and place; false where there is none.  A beam whose score or logsumexp is not
+  // finite has that score for every token: its first tokens stand for it.  (j / per, less than 256, from a product
   // that is off by at most one: an integer division is most of the work otherwise.)
   const float rper = 1.0f / float(per);
   auto score = [&](int j, uint2 a, uint64_t& o, uint64_t& at) __attribute__((always_inline)) {
     int i = int(float(j) * rper), c = j - i * per;
     if (c < 0) --i, c += per;
     if (c >= per) ++i, c -= per;
-    const double b = base_s[i];
+    const double b = score_s[i];
     uint32_t tok = a.y;
-    double sc = b + double(__uint_as_float(a.x));
+    double sc = double(__uint_as_float(a.x)) - double(max_s[i]) - log_s[i] + b;
     if (!(b - b == 0.0)) {
       sc = b;
       tok = c < p.k && c < p.V ? uint32_t(c) : 0xffffffffu;

@@ -83,3 +83,30 @@ def test_whole_chunks_under_a_finite_mask(shape, mask, dtype):
     x[:, :, V - V % 4096:] = mask
     s = -20 * torch.rand(B, nb, generator=g)
     check(cast(x, dtype), s, 8, "the last chunk masked")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", [1e9, 1e10, 1e20, 3e38])
+def test_large_finite_logits(size, dtype):
+    for V in (700, 9000):
+        g = torch.Generator().manual_seed(V)
+        x = torch.randn(1, 3, V, generator=g) * 3
+        x[0, 0, V - 5:] = size * (1 - 0.1 * torch.arange(5))      # one token takes all
+        x[0, 1] = -size * torch.rand(V, generator=g)
+        x[0, 2, ::7] = size
+        check(cast(x, dtype), torch.tensor([[-3.0, -4.0, -2.5]]), 5, f"{V}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("level", ["lowest", -1e30, -1e10, 1e10, 3e38])
+def test_beams_whose_every_logit_is_far_out(level, dtype):
+    """log_softmax does not depend on the logits' level: equal logits of any size give -log V, and beams at different levels
+    are weighed by their scores."""
+    level = LOWEST[dtype] if level == "lowest" else level
+    for V in (700, 9000):
+        g = torch.Generator().manual_seed(V)
+        x = torch.randn(1, 4, V, generator=g) * 0.01
+        x[0, 1], x[0, 3] = level, level
+        x[0, 3, 5::V // 4] = -level if level < 0 else level * 0.5
+        check(cast(x, dtype), torch.tensor([[-9.0, -1.25, -9.5, -30.0]]), 8, f"{V} one level")
+        check(torch.full((1, 3, V), level).to(cast(x, dtype).dtype), torch.tensor([[-3.0, -1.0, -2.0]]), 9, f"{V} all")
