@@ -11,11 +11,12 @@
 // counting.  Where too many reach it (equal logits), or there is a NaN, the k are taken one by one instead.
 // Within a beam the order of logits is the order of scores, so nothing else can be among the k best.
 // beam_join_kernel, one workgroup per group of beams, makes the beams' logsumexp and takes the k best of those
-// lists the same way, by scores in 64 bits: beams may differ by less than 32 bits resolve, and the choice
-// between them has to be right.  Where too many reach its bound (k near 64, beams far apart) the listed ones
-// give a tighter one: 64 of 64 beams of 32000 one by one 1189 us, so 125.  The logits' way through memory bounds
-// large calls (64 beams of 262144 fp32 logits: 43 -> 28 us, 67 MB), two kernels' starts and barriers small ones
-// (4 beams of bf16: 20 -> 13 us).
+// lists the same way.  Exponentials, sums and scores are in 64 bits, off by less than 1e-13 before the result is
+// rounded: beams may differ by less than 32 bits resolve, and the choice between them has to be right.  Where too
+// many reach its bound (k near 64, beams far apart) the listed ones give a tighter one: 64 of 64 beams of 32000 one
+// by one 1189 us, so 125.  The logits' way through memory and their exponentials bound large calls (64 beams of
+// 262144 fp32 logits, 67 MB: 34 us, with exponentials of 32 bits 28), two kernels' starts and barriers small ones
+// (4 beams of bf16: 14.6 us, with 32 bits 13.3).
 #include <algorithm>
 
 #include "w8a8_common.h"
@@ -28,11 +29,16 @@ constexpr int BEAM_LIST = 1024;             // most candidates that are ranked b
 constexpr int BEAM_ROUNDS = 8;              // most times that the join tightens its bound
 constexpr int BEAM_HELD = 8;                // candidates that a thread of the join keeps in registers
 
+struct BeamStat {
+  double sum;  // of exponentials against the maximum
+  float top;
+};
+
 struct BeamParams {
   const void* x; int64_t gs, rs;            // logits [B, nb, V] bf16 or fp32 (element strides of groups and beams)
   const float* score; int64_t ss;           // fp32 [B, nb]
   int nb, V, k, nch;
-  float2* stat;                             // [B nb][nch] maximum and sum of exponentials
+  BeamStat* stat;                           // [B nb][nch]
   uint2* cand;                              // [B nb][nch][k] logit's bits and token
   float* out_score; int64_t *out_beam, *out_tok;  // [B, k]
 };
@@ -74,6 +80,25 @@ __device__ __forceinline__ bool before(T a, uint32_t ai, T b, uint32_t bi) {
   return (a > b) | ((a == b) & (ai < bi));  // (no branch: both are read at once)
 }
 
+// e^d in 64 bits for d <= 0, NaN for NaN: 2^n (1 + f q(f)) with n the whole number next to d log2 e, f = d - n ln 2, and q
+// the polynomial of degree 8 that equals (e^f - 1) / f at the nine Chebyshev points of [-ln 2 / 2, ln 2 / 2]: off by 4e-14
+// of the value at most, and 1 at 0.  (The library's exp, right to the last bit: 8 groups of 8 beams 36.4 us for 34.3.)
+__device__ __forceinline__ double exp_64(double d) {
+  constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
+  d = d < -800.0 ? -800.0 : d;                  // (0 there)
+  const double r = __builtin_fma(d, 1.4426950408889634, WHOLE), f = __builtin_fma(r - WHOLE, -0.6931471805599453, d);
+  double q = 2.7625102005388108e-06;
+  q = __builtin_fma(q, f, 2.4876164022625967e-05);
+  q = __builtin_fma(q, f, 0.0001984120875699232);
+  q = __builtin_fma(q, f, 0.0013888821677630362);
+  q = __builtin_fma(q, f, 0.008333333353717156);
+  q = __builtin_fma(q, f, 0.041666666890957);
+  q = __builtin_fma(q, f, 0.16666666666648303);
+  q = __builtin_fma(q, f, 0.49999999999797934);
+  q = __builtin_fma(q, f, 1.0);
+  return __builtin_ldexp(__builtin_fma(q, f, 1.0), int(uint32_t(__double_as_longlong(r))));
+}
+
 // The best of a workgroup's candidates, given to every thread.
 template <class T, int NW>
 __device__ __forceinline__ void block_first(T& v, uint32_t& i, T* sv, uint32_t* si) {
@@ -97,8 +122,8 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
   constexpr int CHUNK = 256 * E;
   __shared__ uint32_t lv[BEAM_LIST], li[BEAM_LIST];
   __shared__ float gmax[64];
-  __shared__ float red[4], red2[4];
-  __shared__ float bound_s;
+  __shared__ float red[4], bound_s;
+  __shared__ double red2[4];
   __shared__ int count;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int row = blockIdx.x / p.nch, ch = blockIdx.x % p.nch;
@@ -160,16 +185,17 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
     const float b = wave_kth(gmax[lane], p.k);
     if (lane == 0) bound_s = b;
   }
-  // exp2((v - top) log2 e): subtracted before it is scaled, so that a term is 1 at the maximum and never above,
-  // however far out the logits are (a mask of the type's lowest value over the whole chunk)
-  const float l2e = 1.4426950408889634f, ref = top == -__builtin_inff() ? 0.0f : top;
-  float s = 0.0f;
+  // e^(v - top): subtracted in 64 bits, so that a term is 1 at the maximum and never above, however far out the logits
+  // are (a mask of the type's lowest value over the whole chunk)
+  const double ref = top == -__builtin_inff() ? 0.0 : double(top);
+  double s = 0.0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - ref) * l2e);
-  s = wave_sum(s);
+  for (int e = 0; e < E; ++e) s += exp_64(double(v[e]) - ref);  // NaN with a NaN or +inf among the logits
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if (lane == 0) red2[wave] = s;
   __syncthreads();
-  s = (red2[0] + red2[1]) + (red2[2] + red2[3]);  // NaN with a NaN or +inf among the logits
+  s = (red2[0] + red2[1]) + (red2[2] + red2[3]);
   const float bound = bound_s;
   const bool plain = s == s;
   auto list = [&](int e) __attribute__((always_inline)) {
@@ -190,7 +216,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(BeamParams p) {
         if (v[e] > -__builtin_inff() || (valid(e) && local(e) < p.k)) list(e);
   }
   __syncthreads();
-  if (t == 0) p.stat[int64_t(row) * p.nch + ch] = make_float2(top, s);
+  if (t == 0) p.stat[int64_t(row) * p.nch + ch] = BeamStat{s, top};
   uint2* out = p.cand + (int64_t(row) * p.nch + ch) * p.k;
   const int nc = count;
   auto value = [&](uint32_t o) __attribute__((always_inline)) {  // the logit's bits again (NaN: the quiet one)
@@ -244,16 +270,16 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamParams p) {
   // Each beam's maximum, the logarithm of its sum against that, and its score, one wave per beam.  They are kept apart:
   // a logit is taken from the maximum first, as log_softmax has it, and logits of any size leave the rest its bits.
   for (int i = wave; i < p.nb; i += 16) {
-    const float2* st = p.stat + (int64_t(grp) * p.nb + i) * p.nch;
+    const BeamStat* st = p.stat + (int64_t(grp) * p.nb + i) * p.nch;
     float m = -__builtin_inff();
-    for (int c = lane; c < p.nch; c += 64) m = fmaxf(m, st[c].x);
+    for (int c = lane; c < p.nch; c += 64) m = fmaxf(m, st[c].top);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     double s = 0.0;
     for (int c = lane; c < p.nch; c += 64) {
-      const float2 a = st[c];
+      const BeamStat a = st[c];
       // a chunk of -inf only has the sum 0 of its reference 0
-      s += a.x == -__builtin_inff() ? double(a.y) : double(a.y) * exp(double(a.x) - double(m));
+      s += a.top == -__builtin_inff() ? a.sum : a.sum * exp(double(a.top) - double(m));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -404,7 +430,7 @@ static bool beam_shape_ok(int64_t B, int64_t nb, int64_t V, int64_t k) {
 
 extern "C" int64_t w8a8_beam_select_workspace_bytes(int64_t B, int64_t nb, int64_t V, int64_t k) {
   if (!beam_shape_ok(B, nb, V, k)) return -1;
-  return B * nb * beam_chunks(B * nb, V) * 8 * (k + 1);
+  return B * nb * beam_chunks(B * nb, V) * (int64_t(sizeof(BeamStat)) + 8 * k);
 }
 
 extern "C" int w8a8_beam_select(const void* logits, int logits_are_f32, int64_t group_stride, int64_t row_stride,
@@ -429,7 +455,7 @@ extern "C" int w8a8_beam_select(const void* logits, int logits_are_f32, int64_t 
   p.x = logits; p.gs = B > 1 ? group_stride : 0; p.rs = nb > 1 ? row_stride : 0;
   p.score = scores; p.ss = B > 1 ? score_stride : 0;
   p.nb = int(nb); p.V = int(V); p.k = int(k); p.nch = int(beam_chunks(B * nb, V));
-  p.stat = static_cast<float2*>(workspace);
+  p.stat = static_cast<BeamStat*>(workspace);
   p.cand = reinterpret_cast<uint2*>(p.stat + B * nb * p.nch);
   p.out_score = out_scores; p.out_beam = out_beams; p.out_tok = out_tokens;
   const unsigned grid = unsigned(B * nb * p.nch);

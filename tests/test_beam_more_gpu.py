@@ -110,3 +110,29 @@ def test_beams_whose_every_logit_is_far_out(level, dtype):
         x[0, 3, 5::V // 4] = -level if level < 0 else level * 0.5
         check(cast(x, dtype), torch.tensor([[-9.0, -1.25, -9.5, -30.0]]), 8, f"{V} one level")
         check(torch.full((1, 3, V), level).to(cast(x, dtype).dtype), torch.tensor([[-3.0, -1.0, -2.0]]), 9, f"{V} all")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V,nb", [(500, 8), (9000, 8), (40000, 5), (12293, 64)])
+def test_beams_that_differ_by_less_than_32_bits_resolve(V, nb, dtype):
+    """The same logits in every beam but for one token that cannot follow, another one each and none of them likely: the
+    beams' scores differ by those tokens' probabilities, 1e-10 to 1e-6.
+
+    In 64 bits a term is off by a few 2^-53 times log2 of its share, a beam's sum by as much, its logarithm and score by a
+    few 2^-53 of themselves: below 1e-13 in all.  The inputs' scores are at least 1e-12 apart."""
+    g = torch.Generator().manual_seed(V + nb)
+    row = cast(torch.randn(V, generator=g) * 3, dtype)
+    x = row[None, None].repeat(1, nb, 1)
+    p = torch.softmax(row.double(), 0)
+    unlikely = torch.nonzero((p > 1e-10) & (p < 1e-6))[:, 0]
+    unlikely = unlikely[torch.randperm(len(unlikely), generator=g)]
+    _, first = torch.unique(p[unlikely], return_inverse=True)         # of different probabilities
+    seen, out = set(), []
+    for t, f in zip(unlikely.tolist(), first.tolist()):
+        if f not in seen:
+            seen.add(f)
+            out.append(t)
+    for i in range(nb):
+        x[0, i, out[i]] = -math.inf
+    for score in (-3.0, -17.375):
+        check(x, torch.full((1, nb), score), 40, f"score {score}", gap=1e-12, err=1e-12)
