@@ -743,6 +743,10 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
                       r.runs > 1 ? r.run_stride : 0, r.run_bytes})
       while (x % align != 0) align = align == 16 ? 4 : 1;
   }
+  // (the last refusal: from here on tensors change)
+  for (int64_t i = 0; i < count; ++i)
+    if (tensors[i].runs > 0 && tensors[i].run_bytes / align > INT32_MAX / tensors[i].runs)
+      return fail(W8A8_ENOTSUP, "%s: tensor %lld too large", what, (long long)i);
   for (int64_t i0 = 0; i0 < count;) {
     ReorderParams p{};
     p.index = index; p.is = outer > 1 ? index_stride : 0; p.n = int(n); p.size = int(size); p.nouter = int(outer);
@@ -755,7 +759,6 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
       d.axis = r.axis_stride; d.outer = r.outer_stride; d.inner = r.run_stride;
       d.run = r.run_bytes / align; d.ninner = int(r.runs);
       const int64_t b = (d.run * d.ninner + 255) / 256;
-      if (d.run * d.ninner > INT32_MAX) return fail(W8A8_ENOTSUP, "%s: tensor %lld too large", what, (long long)i0);
       if (blocks + b > REORDER_BLOCKS) break;  // (one tensor never has so many)
       d.block0 = int(blocks);
       blocks += b;
