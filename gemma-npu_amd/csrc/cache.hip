@@ -743,6 +743,16 @@ extern "C" int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const 
                       r.runs > 1 ? r.run_stride : 0, r.run_bytes})
       while (x % align != 0) align = align == 16 ? 4 : 1;
   }
+  // an index among the rows that change would be read and written at once
+  const uintptr_t at = reinterpret_cast<uintptr_t>(index), behind = at + ((outer > 1 ? (outer - 1) * index_stride : 0) + n) * 8;
+  for (int64_t i = 0; i < count; ++i) {
+    const w8a8_rows& r = tensors[i];
+    if (r.runs == 0 || r.run_bytes == 0) continue;
+    const uintptr_t first = reinterpret_cast<uintptr_t>(r.data);
+    const int64_t bytes = (outer > 1 ? (outer - 1) * r.outer_stride : 0) + (n > 1 ? (n - 1) * r.axis_stride : 0) +
+                          (r.runs > 1 ? (r.runs - 1) * r.run_stride : 0) + r.run_bytes;
+    if (at < first + bytes && first < behind) return fail(W8A8_EINVAL, "%s: the index lies in tensor %lld", what, (long long)i);
+  }
   // (the last refusal: from here on tensors change)
   for (int64_t i = 0; i < count; ++i)
     if (tensors[i].runs > 0 && tensors[i].run_bytes / align > INT32_MAX / tensors[i].runs)

@@ -54,7 +54,8 @@ def reorder(tensors, index, dim=0):
     [outer, n] with one row per entry of the dimensions before dim.  Every row is read before any is written:
     rows may be exchanged, repeated and dropped.  An index outside the dimension leaves its row as it is.
     Views are taken as they are, so k[:, :, :length] moves the live rows only; the tensors must not overlap
-    (one given twice, as a cache that two layers share, is refused)."""
+    (one given twice, as a cache that two layers share, is refused), and the index is none of them: a copy of it
+    reorders the tensor it was taken from."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if _native is not None and _native.reorder(tensors, index, dim):
         return

@@ -636,7 +636,8 @@ typedef struct {
  * entries, or with index_stride > 0 [outer, n] of that row stride.  Rows 0 .. size - 1 can be taken, the
  * first n <= 64 change; every row is read before any is written, so rows may be exchanged, repeated and
  * dropped; an index outside 0 .. size - 1 leaves its row as it is.  Tensors must not overlap each other (the
- * same address twice is refused); outer <= 65535. */
+ * same address twice is refused), nor the index (one between a tensor's first and last changed byte is refused);
+ * outer <= 65535. */
 int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const int64_t *index, int64_t index_stride, int64_t n,
                       int64_t size, int64_t outer, hipStream_t stream);
 

@@ -21,3 +21,13 @@ def test_a_tensor_too_large_is_refused_before_any_is_reordered():
         cache.reorder([*small, large], torch.tensor([1, 1], device=DEV))
     assert all(torch.equal(t, w) for t, w in zip(small, want))
     assert large[:, -1].tolist() == [0, 5]
+
+
+def test_the_index_among_the_tensors_is_refused():
+    """The beams' numbers kept beside their states: a copy of the index reorders them too."""
+    t, beams = torch.arange(12, device=DEV).view(4, 3).clone(), torch.tensor([1, 2, 3, 0], device=DEV)
+    with pytest.raises(W8A8Error, match="index lies in tensor 1"):
+        cache.reorder([t, beams], beams)
+    assert t.flatten().tolist() == list(range(12)) and beams.tolist() == [1, 2, 3, 0]
+    cache.reorder([t, beams], beams.clone())
+    assert t[:, 0].tolist() == [3, 6, 9, 0] and beams.tolist() == [2, 3, 0, 1]
