@@ -36,10 +36,9 @@ struct KeyWeightParams {
 __device__ __forceinline__ float key_weight_log2(float s, float c, float c_lo, float nl2) {
   return __builtin_fmaf(s, c, __builtin_fmaf(s, c_lo, nl2));
 }
-// -lse log2 e; a query that saw nothing (-inf) adds nothing.
-__device__ __forceinline__ float key_weight_ref(float lse) {
-  return lse == -__builtin_inff() ? lse : -lse * 1.4426950408889634f;
-}
+// -lse log2 e.  +inf is a query that saw nothing and adds nothing: its terms are masked like keys that it does not see, for
+// its scores may be NaN (padding that holds anything, or past the last query zeros times an infinite key).
+__device__ __forceinline__ float key_weight_ref(float lse) { return -lse * 1.4426950408889634f; }
 
 // v summed over the 16 lanes of a group (every lane gets the sum).
 __device__ __forceinline__ float lanes16_sum(float v) {
@@ -81,7 +80,7 @@ __global__ __launch_bounds__(256) void key_weights_few_kernel(KeyWeightParams p)
     const bool valid = r < rows;
     const int i = valid ? r / p.G : 0, h = g * p.G + (valid ? r % p.G : 0);
     const uint16_t* qp = p.q + int64_t(h) * p.qhs + int64_t(i) * p.qrs + 8 * qq;
-    const float nl2 = valid ? key_weight_ref(p.lse[int64_t(h) * p.lhs + i]) : -__builtin_inff();
+    const float nl2 = valid ? key_weight_ref(p.lse[int64_t(h) * p.lhs + i]) : __builtin_inff();
     v4f s0 = v4f{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
@@ -93,12 +92,12 @@ __global__ __launch_bounds__(256) void key_weights_few_kernel(KeyWeightParams p)
       else
         s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kk], b, s0, 0, 0, 0);
     }
-    const int pos = start + i;
+    const int pos = nl2 != __builtin_inff() ? start + i : -1;  // (before every key)
     const uint32_t wlim = p.window > 0 ? uint32_t(p.window) : 0x80000000u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int key = kb + 4 * qq + e;
-      const bool vis = valid & (uint32_t(pos - key) < wlim);
+      const bool vis = uint32_t(pos - key) < wlim;
       w[e] += __builtin_amdgcn_exp2f(attn_mask(key_weight_log2(s0[e] + s1[e], p.c, p.c_lo, nl2), vis));
     }
   }
@@ -213,7 +212,11 @@ __global__ __launch_bounds__(key_weight_threads(D), D == 512 ? 1 : 2) void key_w
     const int p0 = p.start + (lo + n / p.G) * QB;  // the block's first position
     const bool none = kw > p0 + QB - 1 || (p.window > 0 && int64_t(kw) + KEYS - 1 <= int64_t(p0) - p.window);
     if (none) continue;
-    const bool whole = kw + KEYS - 1 <= p0 && (p.window <= 0 || kw > p0 + QB - 1 - p.window);
+    float most = nl2[0];
+#pragma unroll
+    for (int t = 1; t < QB / 16; ++t) most = fmaxf(most, nl2[t]);
+    const bool whole = kw + KEYS - 1 <= p0 && (p.window <= 0 || kw > p0 + QB - 1 - p.window) &&
+                       __builtin_amdgcn_ballot_w64(most == __builtin_inff()) == 0;
     auto qfrag = [&](int i) __attribute__((always_inline)) {  // fragment kk = i % NKK of row tile i / NKK
       const int kk = i % NKK;
       return *reinterpret_cast<const v8bf*>(base + qofs[kk % 4] + (kk / 4) * 256 + (i / NKK) * (16 * ROW));
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(key_weight_threads(D), D == 512 ? 1 : 2) void key_w
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[t][e] = key_weight_log2(s[t][e], c, c_lo, nl2[rt]);
       if (!whole) {
-        const int pos = p0 + 16 * rt + qi;
+        const int pos = nl2[rt] != __builtin_inff() ? p0 + 16 * rt + qi : -1;  // (before every key)
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
