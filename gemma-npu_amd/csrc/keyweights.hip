@@ -11,9 +11,10 @@
 // end, when 16 lanes are added.  No atomics: a key's sum is made by one workgroup, or (long prompts) by one
 // per part of the queries, and the parts are added in order, so the result does not depend on timing.
 //
-// A term is exp2(s c - lse log2 e), c = scale log2 e held in two parts: rounded to one, c's error would be
-// the same sign for all keys (6e-8 of |s c|); the others are half a step of the argument, either way.
+// A term is exp2(s c - lse log2 e), c = scale log2 e held in two parts, both above 0: rounded to one, c's error would
+// be the same sign for all keys (6e-8 of |s c|); the others are half a step of the argument, either way.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_common.h"
 
@@ -425,7 +426,10 @@ extern "C" int w8a8_attention_key_weights(const uint16_t* q, int64_t q_head_stri
   p.start_dev = q_start_dev; p.start = int(std::max<int64_t>(q_start, 0)); p.KV = int(KV); p.G = int(H / KV);
   p.Tq = int(Tq); p.Tk = int(Tk); p.window = int(window);
   const double c = double(scale) * 1.4426950408889634;
-  p.c = float(c); p.c_lo = float(c - double(p.c));
+  // c rounded down and c_lo above 0: with parts of either sign, or a c_lo of 0, a score of -inf would make NaN
+  p.c = float(c);
+  if (double(p.c) > c) p.c = std::nextafter(p.c, 0.0f);
+  p.c_lo = std::max(float(c - double(p.c)), p.c * 0x1p-60f);
   const KeyWeightPlan pl = key_weight_plan(H, KV, Tq, D, p.start, window);
   p.key0 = pl.key0; p.keys = pl.keys; p.nkb = pl.nkb; p.nparts = pl.nparts; p.len = pl.len;
   p.part = static_cast<float*>(workspace);

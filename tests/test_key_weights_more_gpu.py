@@ -63,3 +63,22 @@ def test_padding_queries_add_nothing_whatever_they_hold(shape, what):
         attn.add_key_weights(bad.to(DEV), k.to(DEV), given.to(DEV), got, start, window)
         assert torch.isfinite(got).all()
         check(got, w, s, torch.where(pad, math.inf, lse), KV, D, f"{window}")       # exp(s - inf) = 0
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.5, 0.8, 0.1, 128 ** -0.5, 0.3])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_a_key_of_score_minus_infinity_draws_nothing(shape, scale):
+    """Keys that every query scores with -inf, at any scale: their weights stay, the others' are as without them."""
+    H, KV, Tq, Tk, D, start = shape
+    q, k, w = make(H, KV, Tq, Tk, D, seed=sum(shape))
+    q[:, :, 3] = q[:, :, 3].abs().clamp(min=2.0 ** -10)
+    s = scores(q, k, start, 0, scale)
+    out = torch.zeros(Tk, dtype=torch.bool)
+    out[1::9] = True
+    s = s.masked_fill(out, -math.inf)
+    lse = torch.logsumexp(s, 2).float()
+    k[:, out, 3] = -math.inf
+    got = w.to(DEV)
+    attn.add_key_weights(q.to(DEV), k.to(DEV), lse.to(DEV), got, start, 0, scale)
+    assert torch.equal(got.cpu()[:, out], w[:, out])
+    check(got, w, s, lse, KV, D, f"{scale}")
