@@ -82,3 +82,22 @@ def test_a_key_of_score_minus_infinity_draws_nothing(shape, scale):
     attn.add_key_weights(q.to(DEV), k.to(DEV), lse.to(DEV), got, start, 0, scale)
     assert torch.equal(got.cpu()[:, out], w[:, out])
     check(got, w, s, lse, KV, D, f"{scale}")
+
+
+@pytest.mark.parametrize("window", [0, 512])
+def test_a_position_out_of_range_is_the_nearest_in_range(window):
+    """The caller's error: the weights are added at the nearest position, and nothing beside `weights` is touched."""
+    H, D, cap, guard = 8, 256, 900, 64
+    q, k, _ = make(H, 1, 1, cap, D, seed=8)
+    store = torch.full((3, guard + cap + guard), 7.0, device=DEV)
+    w = store[1:2, guard:guard + cap]
+    pos = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for p, nearest in ((-3, 0), (cap, cap - 1), (1 << 30, cap - 1), (-(1 << 31), 0), (cap - 1, cap - 1), (0, 0)):
+        w.zero_()
+        pos.fill_(p)
+        s = scores(q, k, nearest, window, 1.0)
+        lse = torch.logsumexp(s, 2).float()
+        attn.add_key_weights(q.to(DEV), k.to(DEV), lse.to(DEV), w, pos, window)
+        check(w, torch.zeros(1, cap), s, lse, 1, D, f"{p}")
+        assert (store[0] == 7.0).all() and (store[2] == 7.0).all()
+        assert (store[1, :guard] == 7.0).all() and (store[1, guard + cap:] == 7.0).all()
