@@ -735,6 +735,7 @@ extern "C" int w8a8_attention_tree_bf16(const uint16_t* q, int64_t q_head_stride
     if (rs[i] < D || hs[i] < 0) return fail(W8A8_EINVAL, "%s: row strides smaller than head_dim, or negative", what);
     if (rs[i] % 8 != 0 || hs[i] % 8 != 0) return fail(W8A8_EALIGN, "%s: strides must be multiples of 8 elements", what);
   }
+  if (H > 1 && o_head_stride < D) return fail(W8A8_EINVAL, "%s: o's heads overlap, stride %lld", what, (long long)o_head_stride);
   if ((uintptr_t)q % 16 || (uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)o % 16 || (uintptr_t)workspace % 16 ||
       (uintptr_t)parents % 4 || (uintptr_t)n_past_dev % 4 || (uintptr_t)lse % 4)
     return fail(W8A8_EALIGN, "%s: q, k, v, o and the workspace 16-byte, parents, n_past and lse 4-byte aligned", what);
