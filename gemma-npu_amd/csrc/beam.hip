@@ -14,7 +14,7 @@
 // lists the same way.  Exponentials, sums and scores are in 64 bits, off by less than 1e-13 before the result is
 // rounded: beams may differ by less than 32 bits resolve, and the choice between them has to be right.  Where too
 // many reach its bound (k near 64, beams far apart) the listed ones give a tighter one: 64 of 64 beams of 32000 one
-// by one 1189 us, so 125.  The logits' way through memory and their exponentials bound large calls (64 beams of
+// by one 1189 us, so 135.  The logits' way through memory and their exponentials bound large calls (64 beams of
 // 262144 fp32 logits, 67 MB: 34 us, with exponentials of 32 bits 28), two kernels' starts and barriers small ones
 // (4 beams of bf16: 14.6 us, with 32 bits 13.3).
 #include <algorithm>

@@ -112,8 +112,8 @@ __global__ __launch_bounds__(256) void key_weights_few_kernel(KeyWeightParams p)
 // consecutive positions, each fragment read once per wave, KR of them ahead, and fed to KT MFMAs.  A part is a
 // run of (position block, head) pairs among those that see the key block.  At head_dim 512 eight waves of 32
 // keys, two a SIMD, whose products and exponentials overlap, beat four of 64 with half the LDS reads:
-// 205 -> 65 us for 3658 tokens of 8 heads (840 TFLOP/s; a large library product reaches 1210), 299 us for 8192
-// (919 TFLOP/s).  The LDS reads of the queries (as many cycles as the products) and the first load of the keys
+// 205 -> 66 us for 3658 tokens of 8 heads (832 TFLOP/s; a large library product reaches 1210), 268 us for 8192
+// (1024 TFLOP/s).  The LDS reads of the queries (as many cycles as the products) and the first load of the keys
 // bound it.
 template <int D>
 struct KeyWeightShape {
