@@ -644,11 +644,12 @@ int w8a8_reorder_rows(const w8a8_rows *tensors, int64_t count, const int64_t *in
 /* A beam search step: per group of nb beams the k best of scores[i] + log_softmax(logits[i])[v], sorted, ties
  * to the lowest i * V + v: their scores (fp32), beams and tokens (int64), [B, k] each, contiguous.
  *   logits bf16 or fp32 [B, nb, V] (element strides of groups and beams), scores fp32 [B, nb] (group stride)
- * Exponentials, their sums and the ranking in 64 bits (off by less than 1e-13, and by the roundings to 64 bits of
- * a score and of a logit's distance from its beam's largest), for finite logits of any size.  -inf logits are
- * tokens that cannot follow; a beam whose score minus logsumexp is not finite (a score of -inf: a beam that is
- * out; a NaN or +inf logit: NaN) gives that value to all its tokens, all -inf logits give -inf; NaN ranks first,
- * as torch.topk has it.
+ * Exponentials, their sums and the ranking in 64 bits, for finite logits of any size: off by less than 1e-13, and by
+ * the roundings to 64 bits of a score and of a logit's distance from its beam's largest.  (A beam's candidates are
+ * its largest logits, also where a score is so far out that 64 bits hold no difference between them.)  -inf logits
+ * are tokens that cannot follow; a beam whose score minus logsumexp is not finite (a score of -inf: a beam that is
+ * out; a NaN or +inf logit: NaN) gives that value to all its tokens, all -inf logits give -inf; NaN ranks first, as
+ * torch.topk has it.
  * nb <= 256, k <= 64, k <= nb * V, B < 2^22, less than 2^24 chunks (of 4096 logits of a beam, or 8192 where
  * there are many).  workspace: w8a8_beam_select_workspace_bytes(...) bytes (-1: invalid), 8-byte aligned,
  * scratch.  Two launches, deterministic. */

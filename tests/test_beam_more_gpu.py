@@ -1,8 +1,9 @@
 """A beam search step's choice (ops.beam_select) where the join lists more candidates than it ranks at once and where
 logits are finite but far out, against its definition in 64 bits.
 
-Tolerance of a score: `err` for the beam's logsumexp (fp32 terms and sums of a chunk: a few 2^-24 of the sum, below 2e-6 in its
-logarithm) and the rounding to fp32 (half a step, 2^-24 of the value)."""
+Tolerance of a score: `err` for the beam's logsumexp, and the rounding to fp32 (half a step, 2^-24 of the value).  Where the
+order of near ties is not what a test is about its inputs are more than `gap` apart and `err` is 2e-6, what sums in 32 bits
+would be off by."""
 import math
 
 import pytest
