@@ -80,25 +80,6 @@ __device__ __forceinline__ bool before(T a, uint32_t ai, T b, uint32_t bi) {
   return (a > b) | ((a == b) & (ai < bi));  // (no branch: both are read at once)
 }
 
-// e^d in 64 bits for d <= 0, NaN for NaN: 2^n (1 + f q(f)) with n the whole number next to d log2 e, f = d - n ln 2, and q
-// the polynomial of degree 8 that equals (e^f - 1) / f at the nine Chebyshev points of [-ln 2 / 2, ln 2 / 2]: off by 4e-14
-// of the value at most, and 1 at 0.  (The library's exp, right to the last bit: 8 groups of 8 beams 36.4 us for 34.3.)
-__device__ __forceinline__ double exp_64(double d) {
-  constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
-  d = d < -800.0 ? -800.0 : d;                  // (0 there)
-  const double r = __builtin_fma(d, 1.4426950408889634, WHOLE), f = __builtin_fma(r - WHOLE, -0.6931471805599453, d);
-  double q = 2.7625102005388108e-06;
-  q = __builtin_fma(q, f, 2.4876164022625967e-05);
-  q = __builtin_fma(q, f, 0.0001984120875699232);
-  q = __builtin_fma(q, f, 0.0013888821677630362);
-  q = __builtin_fma(q, f, 0.008333333353717156);
-  q = __builtin_fma(q, f, 0.041666666890957);
-  q = __builtin_fma(q, f, 0.16666666666648303);
-  q = __builtin_fma(q, f, 0.49999999999797934);
-  q = __builtin_fma(q, f, 1.0);
-  return __builtin_ldexp(__builtin_fma(q, f, 1.0), int(uint32_t(__double_as_longlong(r))));
-}
-
 // The best of a workgroup's candidates, given to every thread.
 template <class T, int NW>
 __device__ __forceinline__ void block_first(T& v, uint32_t& i, T* sv, uint32_t* si) {

@@ -626,6 +626,69 @@ PyObject* beam_select(PyObject* const* a) {
   return tuple(value, beam, token);
 }
 
+// logits, tokens, uniforms, draft logits, parents, lengths, temperature -> (accepted, path, next)
+PyObject* verify_drafts(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[0]));
+  const ScalarType dt = THPVariable_Unpack(a[0]).scalar_type();
+  need(dt == at::kBFloat16 || dt == at::kFloat);
+  const int64_t dim = THPVariable_Unpack(a[0]).dim();
+  need(dim == 2 || dim == 3);
+  const Tensor &x = c.tensor(a[0], dt, dim), &tok = c.tensor(a[1], at::kLong, dim - 1), &u = c.tensor(a[2], at::kFloat, dim - 1);
+  c.here();
+  const int64_t B = dim == 3 ? x.size(0) : 1, N = x.size(dim - 2) - 1, V = x.size(dim - 1);
+  need(B >= 1 && N >= 0);
+  auto last = [](const Tensor& t) { return t.size(t.dim() - 1) <= 1 || t.stride(t.dim() - 1) == 1; };
+  auto group = [&](const Tensor& t, int64_t n) { return B > 1 ? t.stride(0) : n; };
+  need(tok.size(dim - 2) == N && u.size(dim - 2) == N + 1 && (dim == 2 || (tok.size(0) == B && u.size(0) == B)));
+  need(last(x) && last(tok) && last(u));
+  const void* draft = nullptr;
+  int64_t dgs = 0, drs = V;
+  if (a[3] != Py_None) {
+    const Tensor& d = c.tensor(a[3], dt, dim);
+    need(a[4] == Py_None && d.size(dim - 2) == N && d.size(dim - 1) == V && (dim == 2 || d.size(0) == B) && last(d));
+    draft = d.data_ptr();
+    dgs = group(d, 0);
+    if (N > 1) drs = d.stride(dim - 2);
+  }
+  const int32_t *parents = nullptr, *lengths = nullptr;
+  int64_t ps = 0;
+  if (a[4] != Py_None) {
+    need(THPVariable_CheckExact(a[4]));
+    const int64_t pd = THPVariable_Unpack(a[4]).dim();
+    const Tensor& p = c.tensor(a[4], at::kInt, pd);
+    need((pd == 1 || (pd == 2 && p.size(0) == B)) && p.size(pd - 1) == N && last(p));
+    parents = static_cast<const int32_t*>(p.data_ptr());
+    ps = pd == 2 && B > 1 ? p.stride(0) : 0;
+  }
+  if (a[5] != Py_None) {
+    const Tensor& l = c.vec(a[5], at::kInt);
+    need(l.size(0) == B);
+    lengths = static_cast<const int32_t*>(l.data_ptr());
+  }
+  need(PyFloat_CheckExact(a[6]) || PyLong_CheckExact(a[6]));
+  const double temperature = PyFloat_AsDouble(a[6]);
+  if (temperature == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    throw Decline{};
+  }
+  const int64_t bytes = w8a8_verify_drafts_workspace_bytes(B, N, V);
+  need(bytes > 0);
+  const bool many = dim == 3;
+  const Tensor accepted = many ? c.make({B}, at::kInt) : c.make({}, at::kInt),
+               path = many ? c.make({B, N}, at::kLong) : c.make({N}, at::kLong),
+               next = many ? c.make({B}, at::kLong) : c.make({}, at::kLong), ws = c.make({bytes}, at::kByte);
+  const hipStream_t st = c.stream();
+  launch("w8a8_verify_drafts", [&] {
+    return w8a8_verify_drafts(x.data_ptr(), draft, dt == at::kFloat ? 1 : 0, group(x, 0), N > 0 ? x.stride(dim - 2) : V, dgs, drs,
+                              static_cast<const int64_t*>(tok.data_ptr()), group(tok, N), f32(u), group(u, N + 1), parents, ps,
+                              lengths, B, N, V, temperature, static_cast<int32_t*>(accepted.data_ptr()),
+                              static_cast<int64_t*>(path.data_ptr()), static_cast<int64_t*>(next.data_ptr()), ws.data_ptr(),
+                              bytes, st);
+  });
+  return tuple(accepted, path, next);
+}
+
 // tensors (a list or tuple), index, dim -> True
 PyObject* reorder(PyObject* const* a) {
   Call c;
@@ -762,7 +825,7 @@ PyMethodDef methods[] = {
     W8A8_ENTRY(k_ple_gate, 4),  W8A8_ENTRY(k_ple_out_k_in, 8),  W8A8_ENTRY(k_qkv, 12),    W8A8_ENTRY(attention, 7),
     W8A8_ENTRY(attention_quant, 7), W8A8_ENTRY(decode, 7),      W8A8_ENTRY(wait_stream, 1),
     W8A8_ENTRY(settle, 2),      W8A8_ENTRY(decode_tree, 7),     W8A8_ENTRY(add_key_weights, 7), W8A8_ENTRY(beam_select, 3),
-    W8A8_ENTRY(reorder, 3),     W8A8_ENTRY(evict, 7),
+    W8A8_ENTRY(reorder, 3),     W8A8_ENTRY(evict, 7),         W8A8_ENTRY(verify_drafts, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "The wrappers' launch path in native code.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

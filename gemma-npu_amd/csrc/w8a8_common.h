@@ -26,6 +26,26 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 // bf16(x) as fp32: the value x rounds to.
 __device__ __forceinline__ float round_bf16(float f) { return bf16_to_f32(f32_to_bf16(f)); }
 
+// ---- exponentials in 64 bits -------------------------------------------------------------------
+// e^d in 64 bits for d <= 0, NaN for NaN: 2^n (1 + f q(f)) with n the whole number next to d log2 e, f = d - n ln 2, and q
+// the polynomial of degree 8 that equals (e^f - 1) / f at the nine Chebyshev points of [-ln 2 / 2, ln 2 / 2]: off by 4e-14
+// of the value at most, and 1 at 0.  (The library's exp, right to the last bit: 8 groups of 8 beams 36.4 us for 34.3.)
+__device__ __forceinline__ double exp_64(double d) {
+  constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the nearest whole number
+  d = d < -800.0 ? -800.0 : d;                  // (0 there)
+  const double r = __builtin_fma(d, 1.4426950408889634, WHOLE), f = __builtin_fma(r - WHOLE, -0.6931471805599453, d);
+  double q = 2.7625102005388108e-06;
+  q = __builtin_fma(q, f, 2.4876164022625967e-05);
+  q = __builtin_fma(q, f, 0.0001984120875699232);
+  q = __builtin_fma(q, f, 0.0013888821677630362);
+  q = __builtin_fma(q, f, 0.008333333353717156);
+  q = __builtin_fma(q, f, 0.041666666890957);
+  q = __builtin_fma(q, f, 0.16666666666648303);
+  q = __builtin_fma(q, f, 0.49999999999797934);
+  q = __builtin_fma(q, f, 1.0);
+  return __builtin_ldexp(__builtin_fma(q, f, 1.0), int(uint32_t(__double_as_longlong(r))));
+}
+
 // ---- raw buffer loads -----------------------------------------------------------------------
 // A raw buffer resource over [base, base + bytes).  Loads whose byte offset is at or past
 // `bytes` return zero instead of touching memory, which is how the kernels read ragged M / N

@@ -18,6 +18,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); must match include/w8a8.h.
 SIGNATURES = {
@@ -112,6 +113,9 @@ SIGNATURES = {
     "w8a8_reorder_rows": (_i32, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p]),
     "w8a8_beam_select_workspace_bytes": (_i64, [_i64] * 4),
     "w8a8_beam_select": (_i32, [_p, _i32, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
+    "w8a8_verify_drafts_workspace_bytes": (_i64, [_i64] * 3),
+    "w8a8_verify_drafts": (_i32, [_p, _p, _i32, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _f64,
+                                  _p, _p, _p, _p, _i64, _p]),
 }
 
 

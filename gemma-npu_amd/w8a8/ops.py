@@ -517,6 +517,88 @@ def beam_select(logits, scores, k, workspace=None):
     return (value[0], beam[0], token[0]) if one else (value, beam, token)
 
 
+def verify_drafts_workspace_bytes(B, N, V):
+    """Bytes of scratch verify_drafts() needs (w8a8_verify_drafts_workspace_bytes)."""
+    n = lib().w8a8_verify_drafts_workspace_bytes(int(B), int(N), int(V))
+    if n < 0:
+        raise ValueError(f"verify_drafts: {N} drafted tokens of a vocabulary of {V} in {B} requests (at most 128 tokens)")
+    return n
+
+
+def verify_drafts(logits, tokens, uniforms, draft_logits=None, parents=None, lengths=None, temperature=1.0, workspace=None):
+    """Drafted tokens tested against the target's probabilities, and the token that follows drawn, from given
+    random numbers: accepted tokens and the next one are distributed as the target's own samples.
+
+    logits: bf16 or fp32 [N + 1, V], or [B, N + 1, V] for B requests: the target's after the context (row 0) and
+    after each drafted token (row m + 1 after token m).  tokens: int64 [N] ([B, N]), uniforms: fp32 [N + 1]
+    ([B, N + 1]) in [0, 1): one for each token's test, the last one for the draw.
+      A chain (parents None): draft_logits [N, V] ([B, N, V], the type of logits) hold what each token was drawn
+      from; None: the tokens were drafted with certainty (the draft's best).  lengths: int32 [B] ([1]), a request's
+      drafted tokens where they differ.
+      A tree: parents int32 [N] ([B, N], or [N] for all), as attention.decode_tree takes them (node m hangs on
+      node parents[m] < m, or with -1 on the context), without draft_logits; siblings are tested in order.
+    temperature: logits are divided by it.  Returns (accepted int32 [], path int64 [N], next int64 []), with a
+    leading [B] for B requests: how many tokens were accepted, which ones (then -1: the index that cache.reorder moves
+    their rows up by), and the next token.  -inf logits are tokens that cannot follow; a row with a NaN or +inf logit,
+    or of -inf alone, accepts nothing, and next is -1 where it is the row reached.  N <= 128.  workspace: a device
+    uint8 tensor of verify_drafts_workspace_bytes(...); by default one from torch's allocator."""
+    if _native is not None and workspace is None:
+        r = _native.verify_drafts(logits, tokens, uniforms, draft_logits, parents, lengths, temperature)
+        if r is not None:
+            return r
+    for t, name in ((logits, "logits"), (tokens, "tokens"), (uniforms, "uniforms"), (draft_logits, "draft_logits"),
+                    (parents, "parents"), (lengths, "lengths")):
+        if t is None and name in ("draft_logits", "parents", "lengths"):
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"verify_drafts: {name} must be a tensor")
+        if t.device.type != "cuda" or t.device != logits.device:
+            raise ValueError("verify_drafts: all tensors must be on one GPU")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"verify_drafts: logits must be bf16 or fp32, got {logits.dtype}")
+    if tokens.dtype != torch.int64 or uniforms.dtype != torch.float32:
+        raise TypeError(f"verify_drafts: tokens must be int64 and uniforms fp32, got {tokens.dtype} and {uniforms.dtype}")
+    for t, name in ((parents, "parents"), (lengths, "lengths")):
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError(f"verify_drafts: {name} must be int32, got {t.dtype}")
+    if draft_logits is not None and draft_logits.dtype != logits.dtype:
+        raise TypeError(f"verify_drafts: draft_logits must be {logits.dtype}, got {draft_logits.dtype}")
+    if parents is not None and draft_logits is not None:
+        raise ValueError("verify_drafts: a tree is verified without draft_logits")
+    one = logits.dim() == 2
+    if one:
+        logits, tokens, uniforms = logits[None], tokens[None], uniforms[None]
+        draft_logits = None if draft_logits is None else draft_logits[None]
+    if logits.dim() != 3 or logits.shape[1] < 1:
+        raise ValueError(f"verify_drafts: expected logits [B, N + 1, V], got {tuple(logits.shape)}")
+    B, N, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    want = [(tokens, "tokens", (B, N)), (uniforms, "uniforms", (B, N + 1)), (draft_logits, "draft_logits", (B, N, V)),
+            (lengths, "lengths", (B,)), (parents, "parents", (N,) if parents is not None and parents.dim() == 1 else (B, N))]
+    for t, name, shape in want:
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"verify_drafts: {name} must have shape {shape[1:] if one and len(shape) > 1 else shape}, got {tuple(t.shape)}")
+    for t in (logits, tokens, uniforms, draft_logits, parents, lengths):
+        if t is not None and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError("verify_drafts: the last dimensions must be contiguous")
+    need = verify_drafts_workspace_bytes(B, N, V)
+    ws = workspace if workspace is not None else torch.empty(need, dtype=torch.uint8, device=logits.device)
+    if ws.device != logits.device or not ws.is_contiguous():
+        raise ValueError(f"verify_drafts: the workspace must be a contiguous tensor on {logits.device}")
+    accepted = torch.empty((B,), dtype=torch.int32, device=logits.device)
+    path = torch.empty((B, N), dtype=torch.int64, device=logits.device)
+    token = torch.empty((B,), dtype=torch.int64, device=logits.device)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    group = lambda t, n: t.stride(0) if t is not None and B > 1 else n
+    row = lambda t: t.stride(1) if t is not None and t.shape[1] > 1 else V
+    call_on(logits, "w8a8_verify_drafts", logits.data_ptr(), ptr(draft_logits), 1 if logits.dtype == torch.float32 else 0,
+            group(logits, 0), row(logits), group(draft_logits, 0), row(draft_logits), tokens.data_ptr(), group(tokens, N),
+            uniforms.data_ptr(), group(uniforms, N + 1), ptr(parents),
+            parents.stride(0) if parents is not None and parents.dim() == 2 and B > 1 else 0, ptr(lengths), B, N, V,
+            float(temperature), accepted.data_ptr(), path.data_ptr(), token.data_ptr(), ws.data_ptr(),
+            ws.numel() * ws.element_size(), _stream(logits))
+    return (accepted[0], path[0], token[0]) if one else (accepted, path, token)
+
+
 def rms_residual_norm(y, res, w1, w2, eps, scalar=None):
     """(h, x): h = bf16(bf16(res + bf16(rms(y) * w1)) * scalar) and x = bf16(rms(h) * w2), one launch:
     k_post_attn's two norms (pipeline.py:95-99), or k_ple_out and the next layer's input norm

@@ -659,6 +659,30 @@ int w8a8_beam_select(const void *logits, int logits_are_f32, int64_t group_strid
                      float *out_scores, int64_t *out_beams, int64_t *out_tokens, void *workspace,
                      int64_t workspace_bytes, hipStream_t stream);
 
+/* Drafted tokens tested against the target's probabilities, and the next token drawn, from given random numbers.
+ * logits [B, N + 1, V]: the target's after the context (row 0) and after node m (row m + 1); draft [B, N, V] of the same
+ * type: what node m's token was drawn from, or null: drafted with certainty.  p = softmax(logits / temperature),
+ * q likewise.
+ *   a chain (parents null): node m is accepted while u[m] q(t_m) < p_m(t_m);
+ *   a tree (parents int32, of request stride parent_stride, 0: one for all; no draft): parents[m] in -1 .. m - 1, any other:
+ *   unused; the children of the node reached are tested in order, u[m] (1 - s) < p(t_m), s the probability of the
+ *   tokens refused beside it, a token refused before having none.
+ * next: the first token whose running sum of r passes u[N] times the sum of r: r = p of the row reached, less q of the
+ * refused node where that is less (else 0), or 0 for the tokens refused without draft logits; p itself if that leaves nothing.
+ *   tokens int64 [B, N], uniforms fp32 [B, N + 1] in [0, 1), lengths int32 [B] or null: a request's nodes (brought into 0 .. N)
+ *   accepted int32 [B], path int64 [B, N]: the accepted nodes, then -1; next int64 [B], contiguous
+ * -inf logits are tokens that cannot follow; a row with a NaN or +inf, or of -inf alone, accepts nothing, and next is -1
+ * if it is the row reached.  A token outside the vocabulary is refused.  Exponentials and sums in 64 bits, in a fixed
+ * order.  N <= 128, V < 2^30; strides in elements, rows contiguous.
+ *   workspace: w8a8_verify_drafts_workspace_bytes(...) bytes (-1: invalid), 8-byte aligned, scratch
+ * Two launches. */
+int64_t w8a8_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V);
+int w8a8_verify_drafts(const void *logits, const void *draft, int logits_are_f32, int64_t group_stride, int64_t row_stride,
+                       int64_t draft_group_stride, int64_t draft_row_stride, const int64_t *tokens, int64_t token_stride,
+                       const float *uniforms, int64_t uniform_stride, const int32_t *parents, int64_t parent_stride,
+                       const int32_t *lengths, int64_t B, int64_t N, int64_t V, double temperature, int32_t *accepted,
+                       int64_t *path, int64_t *next, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
