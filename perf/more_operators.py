@@ -288,7 +288,10 @@ def run(s):
         start, first = s["start"], s["start"] // BLOCK * BLOCK
         if own:
             cache = _package().cache
-            cache.append(s["cache"], s["k"][:, start:], s["v"][:, start:], start)
+            # a cache that went on further than a block takes rows back to a whole block only, so a pass over the same
+            # state puts its first block's old rows in again there
+            at = start if (start + s["t"] - 1) // BLOCK - start // BLOCK <= 1 else first
+            cache.append(s["cache"], s["k"][:, at:], s["v"][:, at:], at)
             return list(cache.read(s["cache"], first, start + s["t"]))
         return [_values(_stored(x[:, first:], s["codes"])).bfloat16() for x in (s["k"], s["v"])]
     if own:
