@@ -689,6 +689,89 @@ PyObject* verify_drafts(PyObject* const* a) {
   return tuple(accepted, path, next);
 }
 
+// A BlockCache's data, KV, capacity, D and whether its codes are e4m3.
+struct Blocks {
+  const Tensor* t;
+  int64_t KV, capacity, D;
+  int e4m3;
+};
+Blocks blocks(Call& c, PyObject* const* a) {
+  const Blocks b{&c.tensor(a[0], at::kByte, 1), integer(a[1]), integer(a[2]), integer(a[3]), int(integer(a[4]))};
+  const int64_t bytes = w8a8_block_cache_bytes(b.KV, b.capacity, b.D);
+  need(bytes > 0 && b.t->numel() >= bytes && b.t->is_contiguous());
+  return b;
+}
+// A length: an int from `least` on, or -1 and an int32 GPU tensor of one element.
+int64_t length(const Call& c, PyObject* o, int64_t least, const int32_t*& dev) {
+  dev = nullptr;
+  if (THPVariable_CheckExact(o)) {
+    const Tensor& t = THPVariable_Unpack(o);
+    need(t.is_cuda() && t.get_device() == c.device && t.scalar_type() == at::kInt && t.numel() == 1 && t.has_storage());
+    dev = static_cast<const int32_t*>(t.data_ptr());
+    return -1;
+  }
+  const int64_t n = integer(o);
+  need(n >= least);
+  return n;
+}
+
+// cache (5), k, v, n -> True
+PyObject* block_append(PyObject* const* a) {
+  Call c;
+  const Blocks b = blocks(c, a);
+  const Tensor &k = c.tensor(a[5], at::kBFloat16, 3), &v = c.tensor(a[6], at::kBFloat16, 3);
+  c.here();
+  const int64_t m = k.size(1);
+  need(m > 0 && k.size(0) == b.KV && k.size(2) == b.D && k.sizes() == v.sizes() && k.stride(2) == 1 && v.stride(2) == 1);
+  const int32_t* dev;
+  const int64_t n = length(c, a[7], 0, dev);
+  const hipStream_t st = c.stream();
+  launch("w8a8_block_append", [&] {
+    return w8a8_block_append(b.t->data_ptr(), b.KV, b.capacity, b.D, b.e4m3, bf(k), b.KV > 1 ? k.stride(0) : 0, m > 1 ? k.stride(1) : b.D,
+                             bf(v), b.KV > 1 ? v.stride(0) : 0, m > 1 ? v.stride(1) : b.D, m, n, dev, st);
+  });
+  Py_RETURN_TRUE;
+}
+
+// cache (5), start, n -> (k, v)
+PyObject* block_read(PyObject* const* a) {
+  Call c;
+  const Blocks b = blocks(c, a);
+  c.here();
+  const int64_t start = integer(a[5]), n = integer(a[6]);
+  need(start >= 0 && n > start && n <= b.capacity);
+  const Tensor k = c.make({b.KV, n - start, b.D}, at::kBFloat16), v = c.make({b.KV, n - start, b.D}, at::kBFloat16);
+  const hipStream_t st = c.stream();
+  launch("w8a8_block_read", [&] { return w8a8_block_read(b.t->data_ptr(), b.KV, b.capacity, b.D, b.e4m3, start, n, bfo(k), bfo(v), st); });
+  return tuple(k, v);
+}
+
+// q, cache (5), n, window, sinks, scale -> o
+PyObject* block_attention(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[0]));
+  const bool one = THPVariable_Unpack(a[0]).dim() == 2;
+  const Tensor& q = one ? c.rows(a[0], at::kBFloat16) : c.tensor(a[0], at::kBFloat16, 3);
+  const Blocks b = blocks(c, a + 1);
+  c.here();
+  const int64_t H = q.size(0), N = one ? 1 : q.size(1), D = q.size(one ? 1 : 2);
+  need(D == b.D && (one || q.stride(2) == 1));
+  const int64_t qrs = one || N <= 1 ? D : q.stride(1), qhs = H > 1 ? q.stride(0) : N * qrs;
+  const int32_t* dev;
+  const int64_t n = length(c, a[6], N, dev), window = integer(a[7]), sinks = integer(a[8]);
+  const float scale = real(a[9]);
+  const int64_t bytes = w8a8_block_attention_workspace_bytes(H, b.KV, N, b.capacity, D, n, window, sinks);
+  need(bytes >= 0);
+  const Tensor o = one ? c.make({H, D}, at::kBFloat16) : c.make({H, N, D}, at::kBFloat16);
+  const Tensor ws = bytes ? c.make({bytes}, at::kByte) : Tensor();
+  const hipStream_t st = c.stream();
+  launch("w8a8_block_attention", [&] {
+    return w8a8_block_attention(bf(q), qhs, qrs, b.t->data_ptr(), H, b.KV, N, b.capacity, D, b.e4m3, n, dev, window, sinks, scale, bfo(o),
+                                N * D, D, nullptr, bytes ? ws.data_ptr() : nullptr, bytes, st);
+  });
+  return wrap(o);
+}
+
 // tensors (a list or tuple), index, dim -> True
 PyObject* reorder(PyObject* const* a) {
   Call c;
@@ -826,6 +909,7 @@ PyMethodDef methods[] = {
     W8A8_ENTRY(attention_quant, 7), W8A8_ENTRY(decode, 7),      W8A8_ENTRY(wait_stream, 1),
     W8A8_ENTRY(settle, 2),      W8A8_ENTRY(decode_tree, 7),     W8A8_ENTRY(add_key_weights, 7), W8A8_ENTRY(beam_select, 3),
     W8A8_ENTRY(reorder, 3),     W8A8_ENTRY(evict, 7),         W8A8_ENTRY(verify_drafts, 7),
+    W8A8_ENTRY(block_append, 8), W8A8_ENTRY(block_read, 7),     W8A8_ENTRY(block_attention, 10),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "The wrappers' launch path in native code.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,512 @@
+// Attention over the 8-bit key / value cache (blocks.h): the newest N of n tokens attend to it, causal, with a sliding
+// window and the first tokens beside it if wanted.
+//
+//   o[h, i, :] = sum_j softmax_j(scale q[h, i] . k[g, j]) v[g, j],   g = h / (H / KV),
+//
+// over the rows j that the query at position p = n - N + i sees: j <= p and, with a window W, p - j < W or j < sinks.
+// Row j is code x scale of its block, or the bf16 row of the ring for the n % 64 rows behind the last whole block.
+//
+// A key's scale leaves its product with q as a factor of the score.  A value's scale t enters the softmax weight as
+// an exponent: P'_j = exp2(s_j + log2 t - ms), with ms trailing the maximum of s_j + log2 t by at most 8, so that what
+// contributes most has the most bits, and sum_j exp2(s_j - ms) = sum P'_j / t is added up in fp32 beside it.  Codes
+// become fp16 exactly (|code| <= 127, e4m3 lies within fp16), so both products are fp16 MFMAs summed in fp32.  The
+// roundings: P' to fp16 (2^-11, subnormal below 2^-14: 2^-25 of a weight of 1), and q, scaled by a power of two that
+// brings its row's largest value to 2^10 (exact but for values below 2^-27 of that).  The rows of the ring go
+// through bf16 MFMAs with P' in bf16 (2^-9).
+//
+// Work split.  The rows (query, head) of one KV head, N G of them, are cut into tiles of 16 RT rows and their visible
+// blocks into parts; a workgroup of four waves takes a tile and a part, and attn_part_merge_kernel joins the parts by
+// their logsumexp.  Per block wave w makes S^T = K Q^T for the keys 16 w .. 16 w + 15 and O^T for its quarter of
+// head_dim; the softmax weights go through LDS, with one barrier a block.  Keys and values come straight from
+// memory in fragment order into registers, a block ahead: no LDS, no transposing.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.h"
+#include "attn_parts.h"
+#include "blocks.h"
+
+namespace w8a8 {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+struct BlockAttnParams {
+  BlockCache c;
+  const uint16_t* q; int64_t qhs, qrs;  // bf16 [H, N, D] (element strides, last dim contiguous)
+  PartParams out;                       // o, lse, parts, rows
+  const int32_t* n_dev;                 // n in device memory, or null
+  int n, N, window, sinks, capacity, ntiles;
+  float cs;                             // scale * log2(e)
+};
+
+// The blocks that a tile's rows see: i < nb stands for block i, from `sb` on for block i + skip.
+struct BlockGeom {
+  int n, pmin, pmax, sb, skip, nb, np;
+};
+__device__ __forceinline__ BlockGeom block_geom(const BlockAttnParams& p, int tile, int R) {
+  BlockGeom t;
+  t.n = p.n_dev ? max(p.N, min(*p.n_dev, p.capacity)) : p.n;
+  const int r0 = tile * R, r1 = min(r0 + R, p.out.rows) - 1;
+  t.pmin = t.n - p.N + r0 / p.out.G;
+  t.pmax = t.n - p.N + r1 / p.out.G;
+  const int wb = p.window > 0 ? max(0, t.pmin - p.window + 1) / BLK : 0;
+  t.sb = (min(p.sinks, t.n) + BLK - 1) / BLK;
+  t.skip = max(0, wb - t.sb);
+  t.nb = t.pmax / BLK + 1 - t.skip;
+  t.np = min(p.out.nparts, t.nb);
+  return t;
+}
+
+// Four codes as fp16: int8 through 1024 + code + 128, whose low byte is the code's with its sign bit turned.
+template <bool E4M3>
+__device__ __forceinline__ void codes_f16(uint32_t w, v2h& a, v2h& b) {
+  if constexpr (E4M3) {
+    a = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    b = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+  } else {
+    const uint32_t x = w ^ 0x80808080u;
+    const v2h bias = {_Float16(1152.0f), _Float16(1152.0f)};
+    a = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias;
+    b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias;
+  }
+}
+template <bool E4M3>
+__device__ __forceinline__ v8h codes8_f16(uint32_t lo, uint32_t hi) {
+  v2h a, b, c, d;
+  codes_f16<E4M3>(lo, a, b);
+  codes_f16<E4M3>(hi, c, d);
+  return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Workgroups of a CU: what the registers of the row tile allow.
+constexpr int block_occupancy(int rt, int d) { return rt * d <= 512 ? 2 : 1; }
+
+template <int D, int RT, bool E4M3>
+__global__ __launch_bounds__(256, block_occupancy(RT, D)) void block_attn_kernel(BlockAttnParams p) {
+  constexpr int R = 16 * RT, NJ = D / 64, NKK = D / 32;
+  constexpr int PLD = BLK + 8;  // padded row of softmax weights
+  __shared__ __attribute__((aligned(16))) uint16_t pl[2][R * PLD];
+  __shared__ float smax[2][4][R];
+  __shared__ float lsum[4][R];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qi = lane & 15, qq = lane >> 4;
+  const int G = p.out.G, rows = p.out.rows;
+  const int lb = xcd_remap(blockIdx.x, gridDim.x);
+  const int tile = lb % p.ntiles, pair = lb / p.ntiles, g = pair / p.out.nparts, part = pair % p.out.nparts;
+  const BlockGeom geo = block_geom(p, tile, R);
+  if (part >= geo.np) return;  // (the whole workgroup, before any barrier)
+  const int i_lo = int(int64_t(part) * geo.nb / geo.np), i_hi = int(int64_t(part + 1) * geo.nb / geo.np);
+  const int whole = geo.n / BLK;  // blocks with codes
+  auto block = [&](int i) __attribute__((always_inline)) { return i < geo.sb ? i : i + geo.skip; };
+  const bool has_ring = block(i_hi - 1) >= whole;  // the part's last block is the unfinished one
+  const int ncode = i_hi - i_lo - (has_ring ? 1 : 0);
+  const int win = p.window, sinks = p.sinks;
+
+  const int64_t head = int64_t(g) * p.c.blocks;
+  const uint8_t* const kc = p.c.k + head * BLK * D + wave * (16 * D) + lane * 16;
+  const uint8_t* const vc = p.c.v + head * BLK * D + wave * (16 * D) + lane * 16;
+  v4u kr[NJ], vr[NJ];
+  auto load_k = [&](int i) __attribute__((always_inline)) {
+    const uint8_t* at = kc + int64_t(block(i)) * (BLK * D);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const v4u*>(at + j * 1024);
+  };
+  auto load_v = [&](int i) __attribute__((always_inline)) {
+    const uint8_t* at = vc + int64_t(block(i)) * (BLK * D);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) vr[j] = *reinterpret_cast<const v4u*>(at + j * 1024);
+  };
+  if (ncode > 0) {
+    load_k(i_lo);
+    load_v(i_lo);
+  }
+
+  // the tile's rows: this lane's are 16 rt + qi
+  int pos[RT];
+  const uint16_t* qp[RT];
+  bool valid[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = tile * R + 16 * rt + qi;
+    valid[rt] = r < rows;
+    const int i = valid[rt] ? r / G : 0, h = valid[rt] ? r % G : 0;
+    pos[rt] = valid[rt] ? geo.n - p.N + i : -1;  // (sees nothing)
+    qp[rt] = p.q + int64_t(g * G + h) * p.qhs + int64_t(i) * p.qrs + 16 * qq;
+  }
+  // Q as the B operand of k-step 2 j + h: q[64 j + 16 qq + 8 h .. + 7], which is how the codes lie
+  v8h qf[RT][NKK];
+  float cq[RT];  // what a score of this row is multiplied by
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    v4u w[NKK];
+    uint32_t m2 = 0u;
+#pragma unroll
+    for (int k = 0; k < NKK; ++k) {
+      w[k] = v4u{0u, 0u, 0u, 0u};
+      if (valid[rt]) w[k] = *reinterpret_cast<const v4u*>(qp[rt] + 64 * (k >> 1) + 8 * (k & 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m2 = absmax_bf16x2(m2, w[k][e]);
+    }
+    const float top = lanes4_max(absmax_pair(m2));
+    // 2^10 over the power of two at or below `top` (no smaller than 2^-87: zeros)
+    const uint32_t e = max(__float_as_uint(top) >> 23, 40u);
+    const float f = __uint_as_float((264u - e) << 23);
+    cq[rt] = p.cs * __uint_as_float((e - 10u) << 23);
+#pragma unroll
+    for (int k = 0; k < NKK; ++k) {
+      float x[8];
+      unpack8(w[k], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qf[rt][k][j] = _Float16(x[j] * f);
+    }
+  }
+
+  float ms[RT], l[RT], alpha[RT];
+  bool grew = false;  // some row of this lane's had its O rescaled last time
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) ms[rt] = -__builtin_inff(), l[rt] = 0.0f, alpha[rt] = 1.0f;
+  v4f o[NJ][RT];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) o[j][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  v4f s[RT];
+  float tb = 0.0f, tinv = 1.0f;  // log2 of the block's value scale, and one over the scale
+  auto seen = [&](int key, int at) __attribute__((always_inline)) {
+    return (key <= at) & ((win <= 0) | (at - key < win) | (key < sinks));
+  };
+  auto inner = [&](int b) __attribute__((always_inline)) {  // every row sees the whole block
+    const int kb = b * BLK;
+    return kb + BLK - 1 <= geo.pmin && (win <= 0 || kb > geo.pmax - win || kb + BLK <= sinks) && tile * R + R <= rows;
+  };
+  // scores in exponents (log2), masked; this wave's row maxima into LDS
+  auto finish_s = [&](int slot, int b, float ks) __attribute__((always_inline)) {
+    const bool all = inner(b);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float f = ks * cq[rt];
+      float bm = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = __builtin_fmaf(s[rt][i], f, tb);
+        if (!all) x = attn_mask(x, seen(b * BLK + 16 * wave + 4 * qq + i, pos[rt]));
+        s[rt][i] = x;
+        bm = fmaxf(bm, x);
+      }
+      bm = lanes4_max(bm);
+      if (qq == 0) smax[slot][wave][16 * rt + qi] = bm;
+    }
+  };
+  auto s_phase = [&](int slot, int i) __attribute__((always_inline)) {
+    const int b = block(i);
+    const float ks = p.c.ks[head + b], vs = p.c.vs[head + b];
+    tb = __builtin_amdgcn_logf(vs);
+    tinv = 1.0f / vs;
+    v4f s2[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) s[rt] = s2[rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const v8h a = codes8_f16<E4M3>(kr[j][0], kr[j][1]), c = codes8_f16<E4M3>(kr[j][2], kr[j][3]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[rt][2 * j], s[rt], 0, 0, 0);
+        s2[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[rt][2 * j + 1], s2[rt], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) s[rt] += s2[rt];
+    finish_s(slot, b, ks);
+  };
+  // after the barrier: the rows' new references, P' into LDS
+  auto softmax = [&](int slot, auto half) __attribute__((always_inline)) {
+    grew = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = 16 * rt + qi;
+      const float m = fmaxf(fmaxf(smax[slot][0][r], smax[slot][1][r]), fmaxf(smax[slot][2][r], smax[slot][3][r]));
+      const bool grow = m > ms[rt] + 8.0f;  // false while every key so far is masked
+      const bool had = ms[rt] != -__builtin_inff();
+      alpha[rt] = !grow ? 1.0f : (had ? __builtin_amdgcn_exp2f(ms[rt] - m) : 0.0f);
+      grew |= grow && had;
+      ms[rt] = grow ? m : ms[rt];
+      const float ref = ms[rt] == -__builtin_inff() ? 0.0f : ms[rt];
+      float sum = 0.0f;
+      uint16_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[rt][i] - ref);
+        sum += e;
+        if constexpr (decltype(half)::value)
+          w[i] = __builtin_bit_cast(uint16_t, _Float16(e));
+        else
+          w[i] = f32_to_bf16(e);
+      }
+      // (a block that a row sees nothing of adds nothing, whatever its scale)
+      l[rt] = __builtin_fmaf(sum, sum != 0.0f ? tinv : 0.0f, l[rt] * alpha[rt]);
+      // key 16 wave + 4 qq + i is slot 4 (wave % 2) + i of lane group qq in k-step wave / 2
+      *reinterpret_cast<v2u*>(&pl[slot][r * PLD + 32 * (wave >> 1) + 8 * qq + 4 * (wave & 1)]) =
+          v2u{uint32_t(w[0]) | uint32_t(w[1]) << 16, uint32_t(w[2]) | uint32_t(w[3]) << 16};
+    }
+  };
+  auto rescale = [&]() __attribute__((always_inline)) {
+    if (__builtin_amdgcn_ballot_w64(grew))
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j][rt] *= alpha[rt];
+  };
+  auto pv_phase = [&](int slot) __attribute__((always_inline)) {
+    rescale();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      v8h pb[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        pb[rt] = *reinterpret_cast<const v8h*>(&pl[slot][(16 * rt + qi) * PLD + 32 * h + 8 * qq]);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const v8h a = codes8_f16<E4M3>(vr[j][2 * h], vr[j][2 * h + 1]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[rt], o[j][rt], 0, 0, 0);
+      }
+    }
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+
+  // Block i's scores and maxima are made one iteration ahead of its P V: the barrier between them makes the maxima of
+  // block i + 1 and the weights of block i visible at once.
+  if (ncode > 0) {
+    s_phase(0, i_lo);
+    if (ncode > 1) load_k(i_lo + 1);
+    __syncthreads();
+    softmax(0, Yes{});
+    for (int x = 0; x < ncode; ++x) {
+      const int slot = x & 1;
+      const bool more = x + 1 < ncode;
+      if (more) {
+        s_phase(slot ^ 1, i_lo + x + 1);
+        if (x + 2 < ncode) load_k(i_lo + x + 2);
+      }
+      __syncthreads();
+      pv_phase(slot);
+      if (more) {
+        load_v(i_lo + x + 1);
+        softmax(slot ^ 1, Yes{});
+      }
+    }
+  }
+
+  if (has_ring) {
+    // the unfinished block: bf16 rows, of which the first `live` are there
+    const int b = whole, live = geo.n - whole * BLK, slot = ncode & 1;
+    const uint16_t* const kt = p.c.kt + (int64_t(g) * 2 + (b & 1)) * BLK * D;
+    const uint16_t* const vt = p.c.vt + (int64_t(g) * 2 + (b & 1)) * BLK * D;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) s[rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (16 * wave < live) {
+#pragma unroll 4
+      for (int k = 0; k < NKK; ++k) {
+        const v8bf a = *reinterpret_cast<const v8bf*>(kt + ((wave * NKK + k) * 64 + lane) * 8);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          v4u w = v4u{0u, 0u, 0u, 0u};
+          if (valid[rt]) w = *reinterpret_cast<const v4u*>(qp[rt] + 64 * (k >> 1) + 8 * (k & 1));
+          s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(v8bf, w), s[rt], 0, 0, 0);
+        }
+      }
+    }
+    tb = 0.0f;
+    tinv = 1.0f;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) cq[rt] = p.cs;
+    finish_s(slot, b, 1.0f);  // (rows from `live` on lie behind every position)
+    __syncthreads();
+    softmax(slot, No{});
+    __syncthreads();
+    rescale();
+    bool bad = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (32 * h >= live) break;
+      v8bf pb[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        pb[rt] = *reinterpret_cast<const v8bf*>(&pl[slot][(16 * rt + qi) * PLD + 32 * h + 8 * qq]);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        v4u w = *reinterpret_cast<const v4u*>(vt + (((wave * NJ + j) * 2 + h) * 64 + lane) * 8);
+        // rows that aren't there are zero; infinities and NaN leave the product (0 x inf) and are added below to
+        // the rows that see them
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t m = e & 1 ? 0xffff0000u : 0xffffu;
+          const bool gone = 32 * h + 16 * (e >> 2) + 4 * qq + (e & 3) >= live;
+          const bool inf = (w[e >> 1] & m & 0x7f807f80u) == (m & 0x7f807f80u);
+          bad |= inf && !gone;
+          if (gone || inf) w[e >> 1] &= ~m;
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          o[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), pb[rt], o[j][rt], 0, 0, 0);
+      }
+    }
+    if (__builtin_amdgcn_ballot_w64(bad)) {
+#pragma unroll 1
+      for (int key = 0; key < live; ++key)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = uint32_t(vt[ring_value(key, 16 * (wave * NJ + j) + 4 * qq + i)]) << 16;
+            if ((x & 0x7f800000u) != 0x7f800000u) continue;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              if (seen(b * BLK + key, pos[rt])) o[j][rt][i] += __uint_as_float(x);
+          }
+    }
+  }
+
+  // the rows' sums over the waves' keys
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float x = lanes4_sum(l[rt]);
+    if (qq == 0) lsum[wave][16 * rt + qi] = x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = 16 * rt + qi;
+    const float lt = (lsum[0][r] + lsum[1][r]) + (lsum[2][r] + lsum[3][r]);
+    if (!valid[rt]) continue;
+    const int row = tile * R + r, d = wave * (D / 4) + 4 * qq;  // + 16 j + i
+    if (geo.np > 1) {
+      const int64_t at = (int64_t(g) * p.out.nparts + part) * rows + row;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) *reinterpret_cast<v4f*>(p.out.part_o + at * D + d + 16 * j) = o[j][rt];
+      if (wave == 0 && qq == 0) *reinterpret_cast<v2f*>(p.out.part_ml + at * 2) = v2f{ms[rt], lt};
+      continue;
+    }
+    const float inv = lt > 0.0f ? 1.0f / lt : (lt == lt ? 0.0f : lt);  // (a NaN sum stays one)
+    uint16_t* const op = p.out.o + int64_t(g * G + row % G) * p.out.ohs + int64_t(row / G) * p.out.ors + d;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      *reinterpret_cast<v2u*>(op + 16 * j) =
+          inv != 0.0f ? v2u{pack_bf16x2(o[j][rt][0] * inv, o[j][rt][1] * inv), pack_bf16x2(o[j][rt][2] * inv, o[j][rt][3] * inv)}
+                      : v2u{0u, 0u};
+    if (p.out.lse && wave == 0 && qq == 0)
+      p.out.lse[int64_t(g * G + row % G) * p.N + row / G] = part_lse(ms[rt], lt);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void block_merge_kernel(BlockAttnParams p, int R) {
+  const int row = blockIdx.x % p.out.rows;
+  part_merge<D>(p.out, block_geom(p, row / R, R).np, p.N);
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+struct BlockPlan {
+  int rt, ntiles, nparts;
+};
+
+static BlockPlan block_plan(int64_t H, int64_t KV, int64_t N, int64_t n, int64_t D, int64_t window, int64_t sinks) {
+  const int64_t rows = N * (H / KV);
+  BlockPlan pl;
+  const int most = D == 512 ? 2 : 4;
+  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : most;
+  pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
+  // the blocks of a tile
+  const int64_t span = window > 0 ? std::min<int64_t>(n, window + 16 * pl.rt / (H / KV) + 1 + BLK) / BLK + 1 + (std::min(sinks, n) + BLK - 1) / BLK
+                                  : (n + BLK - 1) / BLK;
+  const int64_t nb = std::min<int64_t>(span, (n + BLK - 1) / BLK);
+  const int64_t cus = attn_cu_count();
+  const int64_t want = std::max<int64_t>(1, cus * block_occupancy(pl.rt, int(D)) / (pl.ntiles * KV));
+  pl.nparts = int(std::min<int64_t>({want, nb, PART_MAX}));
+  return pl;
+}
+
+template <int D, bool E4M3>
+static void block_launch(const BlockAttnParams& p, const BlockPlan& pl, hipStream_t stream) {
+  const dim3 grid{unsigned(pl.ntiles) * unsigned(p.out.KV) * unsigned(p.out.nparts), 1, 1};
+  if (pl.rt == 1)
+    block_attn_kernel<D, 1, E4M3><<<grid, 256, 0, stream>>>(p);
+  else if (pl.rt == 2)
+    block_attn_kernel<D, 2, E4M3><<<grid, 256, 0, stream>>>(p);
+  else if constexpr (D < 512)
+    block_attn_kernel<D, 4, E4M3><<<grid, 256, 0, stream>>>(p);
+  if (p.out.nparts > 1)
+    block_merge_kernel<D><<<dim3{unsigned(p.out.KV) * unsigned(p.out.rows), unsigned(D / 64), 1}, 256, 0, stream>>>(p, 16 * pl.rt);
+}
+
+static bool block_attn_shape_ok(int64_t H, int64_t KV, int64_t N, int64_t capacity, int64_t D, int64_t window, int64_t sinks) {
+  return block_shape_ok(KV, capacity, D) && H >= 1 && H <= (1 << 16) && H % KV == 0 && N >= 1 && N <= capacity && N * H < (int64_t(1) << 28) &&
+         window >= 0 && window <= INT32_MAX / 2 && sinks >= 0 && sinks <= INT32_MAX / 2;
+}
+
+}  // namespace w8a8
+
+using namespace w8a8;
+
+extern "C" int64_t w8a8_block_attention_workspace_bytes(int64_t H, int64_t KV, int64_t N, int64_t capacity, int64_t D,
+                                                        int64_t n, int64_t window, int64_t sinks) {
+  if (!block_attn_shape_ok(H, KV, N, capacity, D, window, sinks) || n < -1 || n > capacity || (n >= 0 && n < N)) return -1;
+  const BlockPlan pl = block_plan(H, KV, N, n < 0 ? capacity : n, D, window, sinks);
+  return pl.nparts > 1 ? H * N * pl.nparts * (D + 2) * 4 : 0;
+}
+
+extern "C" int w8a8_block_attention(const uint16_t* q, int64_t q_head_stride, int64_t q_row_stride, const void* cache,
+                                    int64_t H, int64_t KV, int64_t N, int64_t capacity, int64_t D, int e4m3, int64_t n,
+                                    const int32_t* n_dev, int64_t window, int64_t sinks, float scale, uint16_t* o,
+                                    int64_t o_head_stride, int64_t o_row_stride, float* lse, void* workspace,
+                                    int64_t workspace_bytes, hipStream_t stream) {
+  const char* what = "block_attention";
+  if (D != 128 && D != 256 && D != 512)
+    return fail(W8A8_ENOTSUP, "%s: head_dim %lld (supported: 128, 256, 512)", what, (long long)D);
+  if (!block_attn_shape_ok(H, KV, N, capacity, D, window, sinks))
+    return fail(W8A8_EINVAL, "%s: H=%lld KV=%lld N=%lld capacity=%lld window=%lld sinks=%lld", what, (long long)H, (long long)KV,
+                (long long)N, (long long)capacity, (long long)window, (long long)sinks);
+  if (n_dev ? n != -1 : (n < N || n > capacity))
+    return fail(W8A8_EINVAL, "%s: n=%lld (N .. capacity, or -1 with a length in device memory)", what, (long long)n);
+  if (!(scale > 0.0f) || scale == __builtin_inff()) return fail(W8A8_EINVAL, "%s: scale must be positive", what);
+  if (!q || !cache || !o) return fail(W8A8_EINVAL, "%s: null pointer", what);
+  const int64_t need = w8a8_block_attention_workspace_bytes(H, KV, N, capacity, D, n, window, sinks);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(W8A8_EINVAL, "%s: workspace of %lld bytes, %lld needed", what, (long long)(workspace ? workspace_bytes : 0),
+                (long long)need);
+  const int64_t rs[2] = {N > 1 ? q_row_stride : D, N > 1 ? o_row_stride : D};
+  const int64_t hs[2] = {H > 1 ? q_head_stride : 0, H > 1 ? o_head_stride : 0};
+  for (int i = 0; i < 2; ++i) {
+    if (rs[i] < D || hs[i] < 0) return fail(W8A8_EINVAL, "%s: row strides smaller than head_dim, or negative", what);
+    if (rs[i] % 8 != 0 || hs[i] % 8 != 0) return fail(W8A8_EALIGN, "%s: strides must be multiples of 8 elements", what);
+  }
+  if (H > 1 && o_head_stride < D) return fail(W8A8_EINVAL, "%s: o's heads overlap, stride %lld", what, (long long)o_head_stride);
+  if ((uintptr_t)q % 16 || (uintptr_t)cache % 16 || (uintptr_t)o % 16 || (uintptr_t)workspace % 16 || (uintptr_t)n_dev % 4 ||
+      (uintptr_t)lse % 4)
+    return fail(W8A8_EALIGN, "%s: q, o, the cache and the workspace 16-byte, n and lse 4-byte aligned", what);
+  const BlockPlan pl = block_plan(H, KV, N, n_dev ? capacity : n, D, window, sinks);
+  BlockAttnParams p{};
+  block_layout(const_cast<void*>(cache), KV, capacity, D, p.c);
+  p.q = q; p.qhs = hs[0]; p.qrs = rs[0];
+  p.out.o = o; p.out.ohs = hs[1]; p.out.ors = rs[1]; p.out.lse = lse; p.out.KV = int(KV); p.out.G = int(H / KV);
+  p.out.rows = int(N * (H / KV)); p.out.nparts = pl.nparts;
+  p.out.part_o = static_cast<float*>(workspace);
+  p.out.part_ml = p.out.part_o + H * N * pl.nparts * D;
+  p.n_dev = n_dev; p.n = int(std::max<int64_t>(n, 0)); p.N = int(N); p.window = int(window); p.sinks = window > 0 ? int(sinks) : 0;
+  p.capacity = int(capacity); p.ntiles = pl.ntiles;
+  p.cs = scale * 1.4426950408889634f;
+  switch (int(D) + (e4m3 ? 1 : 0)) {
+    case 128: block_launch<128, false>(p, pl, stream); break;
+    case 129: block_launch<128, true>(p, pl, stream); break;
+    case 256: block_launch<256, false>(p, pl, stream); break;
+    case 257: block_launch<256, true>(p, pl, stream); break;
+    case 512: block_launch<512, false>(p, pl, stream); break;
+    default: block_launch<512, true>(p, pl, stream);
+  }
+  return check_launch(what);
+}

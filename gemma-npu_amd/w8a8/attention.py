@@ -8,6 +8,7 @@ local_attn.py:71-107).
     attention(q, k, v, q_start, window, scale)      -> o (and the logsumexp)
     decode(q, k, v, q_pos, window, scale)           -> o [H, D] (and the logsumexp)
     decode_tree(q, k, v, parents, n_past, window)   -> o [H, N, D] of a tree of drafted tokens
+    block_attention(q, c, n, window, sinks)         -> o [H, N, D] over a cache of 8-bit codes
     add_key_weights(q, k, lse, weights, q_start, W) -> weights [KV, Tk], what each key has drawn added
 
 q is bf16 [H, Tq, D] at positions q_start.., k_all / v_all bf16 [KV, Tk, D] holding positions
@@ -24,6 +25,7 @@ import threading
 import torch
 
 from ._lib import call, call_on, lib
+from .cache import BlockCache
 from .ops import PackedActivation, _native, _stream, current_stream_handle, packed_act_bytes
 
 _WS = {}
@@ -396,6 +398,66 @@ def decode_tree(q, k, v, parents, n_past, window=0, scale=1.0, out=None, return_
             float(scale), out.data_ptr(), ohs, ors, lse.data_ptr() if return_lse else None,
             None if workspace is None else workspace.data_ptr(),
             0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
+    return (out, lse) if return_lse else out
+
+
+def block_attention_workspace_bytes(H, KV, N, capacity, D, n=None, window=0, sinks=0):
+    """Bytes of scratch block_attention() needs (w8a8_block_attention_workspace_bytes); n None: a length held in
+    device memory."""
+    b = lib().w8a8_block_attention_workspace_bytes(H, KV, N, capacity, D, -1 if n is None else int(n), int(window), int(sinks))
+    if b < 0:
+        raise ValueError(f"block_attention: invalid shape H={H} KV={KV} N={N} capacity={capacity} D={D} n={n} window={window} sinks={sinks}")
+    return b
+
+
+def block_attention(q, c, n, window=0, sinks=0, scale=1.0, out=None, return_lse=False, workspace=None):
+    """Attention over an 8-bit cache (cache.BlockCache): the newest N of its n tokens attend to it, one decoded token, a
+    run of drafted ones or a prompt's next piece, after cache.append has put their keys and values there.
+
+    q: bf16 [H, N, D] ([H, D]: one token), at positions n - N .. n - 1.  The query at position p sees rows j <= p,
+    with a window W those with p - j < W and the first `sinks` rows.  n: an int, or an int32 GPU tensor of one element
+    (the launch then does not depend on it, so a captured step replays at each new length).
+    Returns o of q's shape (into `out` if given, any strides with a contiguous last dimension), and with return_lse the
+    fp32 [H, N] ([H]) logsumexp.  workspace: a device uint8 tensor of at least block_attention_workspace_bytes(...);
+    by default one from torch's allocator."""
+    if _native is not None and out is None and workspace is None and not return_lse and isinstance(c, BlockCache):
+        o = _native.block_attention(q, c.data, c.KV, c.capacity, c.D, c.e4m3, n, window, sinks, scale)
+        if o is not None:
+            return o
+    if not isinstance(c, BlockCache):
+        raise TypeError(f"block_attention: expected a BlockCache, got {type(c).__name__}")
+    one = isinstance(q, torch.Tensor) and q.dim() == 2
+    if one:
+        q, out = q[:, None], out[:, None] if isinstance(out, torch.Tensor) and out.dim() == 2 else out
+    _check3(q, "q")
+    H, N, D = q.shape
+    if D != c.D or q.device != c.device:
+        raise ValueError(f"block_attention: q {tuple(q.shape)} on {q.device} and a cache of head_dim {c.D} on {c.device}")
+    dev = None
+    if isinstance(n, torch.Tensor):
+        if n.dtype != torch.int32 or n.numel() != 1 or n.device != q.device:
+            raise ValueError("block_attention: n must be an int or an int32 tensor of one element on q's device")
+        dev, n = n, -1
+    elif not N <= int(n) <= c.capacity:
+        raise ValueError(f"block_attention: {N} queries of {n} rows in a cache of {c.capacity}")
+    if out is None:
+        out = torch.empty((H, N, D), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out(out, "out", (H, N, D), q.device)
+    lse = torch.empty((H, N), dtype=torch.float32, device=q.device) if return_lse else None
+    if workspace is None:
+        need = block_attention_workspace_bytes(H, c.KV, N, c.capacity, D, None if dev is not None else n, window, sinks)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError(f"block_attention: the workspace must be a contiguous tensor on {q.device}")
+    qhs, qrs = _strides(q)
+    ohs, ors = _strides(out)
+    call_on(q, "w8a8_block_attention", q.data_ptr(), qhs, qrs, c.data.data_ptr(), H, c.KV, N, c.capacity, D, c.e4m3, int(n),
+            None if dev is None else dev.data_ptr(), int(window), int(sinks), float(scale), out.data_ptr(), ohs, ors,
+            lse.data_ptr() if return_lse else None, None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
+    if one:
+        out, lse = out[:, 0], lse[:, 0] if return_lse else None
     return (out, lse) if return_lse else out
 
 

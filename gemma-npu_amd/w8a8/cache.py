@@ -1,7 +1,9 @@
-"""Rows of the key / value cache put elsewhere, on the GPU and in place.
+"""Rows of the key / value cache put elsewhere, on the GPU and in place, and caches of 8-bit codes.
 
     reorder(tensors, index, dim)                         t[i] = t[index[i]] along dim, in every tensor
     evict(k, v, weights, positions, n, budget, recent)   a cache cut to a budget of rows per KV head
+    BlockCache(KV, capacity, D, dtype)                   a cache of 8-bit codes with a scale per block of 64 rows
+    append(c, k, v, n), read(c, start, n)                rows put into it and read back
 
 The reference's cache only grows (HF's DynamicCache, gemma_npu.py:278-300); these are for decoding that
 does otherwise: beams (ops.beam_select gives the index), drafted tokens (attention.decode_tree; the
@@ -155,3 +157,85 @@ def evict(k, v, weights, positions, n, budget, recent=0, out=None, workspace=Non
             w_out.data_ptr(), ld(w_out), p_out.data_ptr(), ld(p_out), ws.data_ptr(), ws.numel() * ws.element_size(),
             _stream(k))
     return kept, w_out, p_out
+
+
+class BlockCache:
+    """The keys and values of one layer in 8 bits: `capacity` rows of KV heads, D values each (128, 256, 512).
+
+    Every whole block of 64 rows is held as int8 codes (dtype torch.float8_e4m3fn: e4m3) with one fp32 scale per KV
+    head, for keys and for values: max |x| / 127 (times 1 / 448), as the engine quantises activations.  The rows of the block
+    that is not whole yet stay bf16, so what it holds depends on the rows alone, not on how they were appended.  Holds
+    half a bf16 cache's bytes; attention.block_attention attends to it.  `data` is opaque (the order in which the
+    matrix instructions take the codes)."""
+
+    __slots__ = ("data", "KV", "capacity", "D", "dtype")
+
+    def __init__(self, KV, capacity, D, dtype=torch.int8, device="cuda"):
+        if dtype not in (torch.int8, torch.float8_e4m3fn):
+            raise TypeError(f"BlockCache: codes are torch.int8 or torch.float8_e4m3fn, got {dtype}")
+        n = lib().w8a8_block_cache_bytes(int(KV), int(capacity), int(D))
+        if n < 0:
+            raise ValueError(f"BlockCache: invalid shape KV={KV} capacity={capacity} D={D} (D: 128, 256, 512)")
+        self.KV, self.capacity, self.D, self.dtype = int(KV), int(capacity), int(D), dtype
+        self.data = torch.empty(n, dtype=torch.uint8, device=device)
+        if self.data.device.type != "cuda":
+            raise ValueError(f"BlockCache: expected a GPU, got device {device}")
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def e4m3(self):
+        return 1 if self.dtype == torch.float8_e4m3fn else 0
+
+
+def append(c, k, v, n):
+    """Rows n .. n + m - 1 of BlockCache c: k / v bf16 [KV, m, D] (any strides with a contiguous last dimension).
+
+    n: the rows that are there, an int, or an int32 GPU tensor of one element (the launch then does not depend on it,
+    so a captured step replays at each new length).  n may be less than before, as where drafted tokens are taken
+    back: rows from n on are written anew.  It has to be a multiple of 64 then, or lie in one of the two newest
+    blocks, whose rows are still there in bf16."""
+    if _native is not None and isinstance(c, BlockCache) and _native.block_append(c.data, c.KV, c.capacity, c.D, c.e4m3, k, v, n):
+        return
+    if not isinstance(c, BlockCache):
+        raise TypeError(f"append: expected a BlockCache, got {type(c).__name__}")
+    for t, name in ((k, "k"), (v, "v")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device != c.device:
+            raise TypeError(f"append: {name} must be a bf16 tensor on {c.device}")
+        if t.dim() != 3 or t.shape[0] != c.KV or t.shape[2] != c.D or t.shape[1] != k.shape[1]:
+            raise ValueError(f"append: {name} must be [{c.KV}, rows, {c.D}], got {tuple(t.shape)}")
+        if t.stride(2) != 1:
+            raise ValueError(f"append: {name}: the last dimension must be contiguous, got strides {t.stride()}")
+    m, dev = k.shape[1], None
+    if isinstance(n, torch.Tensor):
+        if n.dtype != torch.int32 or n.numel() != 1 or n.device != c.device:
+            raise ValueError("append: n must be an int or an int32 tensor of one element on the cache's device")
+        dev, n = n, -1
+    elif not 0 <= int(n) <= c.capacity - m:
+        raise ValueError(f"append: {m} rows from {n} on in a cache of {c.capacity}")
+    if m == 0:
+        return
+    call_on(k, "w8a8_block_append", c.data.data_ptr(), c.KV, c.capacity, c.D, c.e4m3, k.data_ptr(), k.stride(0) if c.KV > 1 else 0,
+            k.stride(1) if m > 1 else c.D, v.data_ptr(), v.stride(0) if c.KV > 1 else 0, v.stride(1) if m > 1 else c.D, m, int(n),
+            None if dev is None else dev.data_ptr(), _stream(k))
+
+
+def read(c, start, n):
+    """(k, v) bf16 [KV, n - start, D]: what rows start .. n - 1 of BlockCache c, which holds n rows, stand for, rounded to
+    bf16 (for attention.attention over what came before, or to put the rows elsewhere)."""
+    if not isinstance(c, BlockCache):
+        raise TypeError(f"read: expected a BlockCache, got {type(c).__name__}")
+    if _native is not None:
+        r = _native.block_read(c.data, c.KV, c.capacity, c.D, c.e4m3, start, n)
+        if r is not None:
+            return r
+    start, n = int(start), int(n)
+    if not 0 <= start <= n <= c.capacity:
+        raise ValueError(f"read: rows {start} .. {n} of a cache of {c.capacity}")
+    k = torch.empty((c.KV, n - start, c.D), dtype=torch.bfloat16, device=c.device)
+    v = torch.empty_like(k)
+    if n > start:
+        call_on(k, "w8a8_block_read", c.data.data_ptr(), c.KV, c.capacity, c.D, c.e4m3, start, n, k.data_ptr(), v.data_ptr(), _stream(k))
+    return k, v

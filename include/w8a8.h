@@ -683,6 +683,39 @@ int w8a8_verify_drafts(const void *logits, const void *draft, int logits_are_f32
                        const int32_t *lengths, int64_t B, int64_t N, int64_t V, double temperature, int32_t *accepted,
                        int64_t *path, int64_t *next, void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/* The 8-bit key / value cache of a layer: `capacity` rows of KV heads, D values each (128, 256 or 512).  Whole blocks of 64
+ * rows are held as one-byte codes (int8, or e4m3 with e4m3 != 0) with one fp32 scale per block, head and operand:
+ * scale = max(max |x|, 1e-8) / 127 (times fp32(1 / 448)), code = x / scale rounded to the nearest.  A block with a NaN or an infinity
+ * reads NaN.  The rows of the block that is not whole yet are held in bf16, as are those of the one before it.
+ *   cache: w8a8_block_cache_bytes(KV, capacity, D) bytes (-1: invalid), 16-byte aligned; needs no initialisation
+ * w8a8_block_append writes rows n .. n + m - 1 (k / v bf16 [KV, m, D], strides in elements, multiples of 8; 16-byte
+ * aligned): rows 0 .. n - 1 were written before, and n may be less than what the cache held (drafted tokens taken
+ * back) if n is a multiple of 64 or its block one of the newest two; rows from n + m on are gone then.  n: 0 ..
+ * capacity - m, or -1 and n_dev, an int32 in device memory (brought into that range), which the launch does not
+ * depend on.  One launch.
+ * w8a8_block_read writes what rows start .. n - 1 of a cache of n rows stand for, rounded to bf16, to k / v [KV, n - start,
+ * D] (contiguous). */
+int64_t w8a8_block_cache_bytes(int64_t KV, int64_t capacity, int64_t D);
+int w8a8_block_append(void *cache, int64_t KV, int64_t capacity, int64_t D, int e4m3, const uint16_t *k, int64_t k_head_stride,
+                      int64_t k_row_stride, const uint16_t *v, int64_t v_head_stride, int64_t v_row_stride, int64_t m,
+                      int64_t n, const int32_t *n_dev, hipStream_t stream);
+int w8a8_block_read(const void *cache, int64_t KV, int64_t capacity, int64_t D, int e4m3, int64_t start, int64_t n, uint16_t *k,
+                    uint16_t *v, hipStream_t stream);
+
+/* Attention over such a cache of n rows: q bf16 [H, N, D] are the queries at positions n - N .. n - 1; the query at p sees
+ * rows j <= p, with a window W > 0 those with p - j < W or j < sinks.  o bf16 [H, N, D], lse fp32 [H, N] or null
+ * (natural logarithm).
+ *   n: N .. capacity; or -1 and n_dev, an int32 in device memory (brought into that range), which the launch does not depend on
+ *   workspace: w8a8_block_attention_workspace_bytes(...) bytes (-1: invalid; 0: none), 16-byte aligned, scratch;
+ *   calls that overlap in time need separate ones
+ * strides in elements, multiples of 8; q and o 16-byte aligned.  Sums in fp32 in a fixed order.  One or two launches. */
+int64_t w8a8_block_attention_workspace_bytes(int64_t H, int64_t KV, int64_t N, int64_t capacity, int64_t D, int64_t n,
+                                             int64_t window, int64_t sinks);
+int w8a8_block_attention(const uint16_t *q, int64_t q_head_stride, int64_t q_row_stride, const void *cache, int64_t H, int64_t KV,
+                         int64_t N, int64_t capacity, int64_t D, int e4m3, int64_t n, const int32_t *n_dev, int64_t window,
+                         int64_t sinks, float scale, uint16_t *o, int64_t o_head_stride, int64_t o_row_stride, float *lse,
+                         void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
