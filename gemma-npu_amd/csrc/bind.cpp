@@ -772,6 +772,34 @@ PyObject* block_attention(PyObject* const* a) {
   return wrap(o);
 }
 
+// q, k, v, q_start, window, sinks, scale -> o
+PyObject* sink_attention(PyObject* const* a) {
+  Call c;
+  need(THPVariable_CheckExact(a[0]));
+  const bool one = THPVariable_Unpack(a[0]).dim() == 2;
+  const Tensor& q = one ? c.rows(a[0], at::kBFloat16) : c.tensor(a[0], at::kBFloat16, 3);
+  const int64_t H = q.size(0), Tq = one ? 1 : q.size(1), D = q.size(one ? 1 : 2);
+  need(Tq >= 1 && D > 1 && (one || q.stride(2) == 1));
+  const int64_t qrs = one || Tq <= 1 ? D : q.stride(1), qhs = H > 1 ? q.stride(0) : Tq * qrs;
+  const Heads k = heads(c, a[1]), v = heads(c, a[2]);
+  const int64_t KV = k.t->size(0), Tk = k.t->size(1);
+  need(k.t->size(2) == D && k.t->sizes() == v.t->sizes());
+  c.here();
+  const int32_t* dev;
+  const int64_t start = length(c, a[3], 0, dev), window = integer(a[4]), sinks = integer(a[5]);
+  const float scale = real(a[6]);
+  const int64_t bytes = w8a8_attention_sinks_workspace_bytes(H, KV, Tq, Tk, D, start, window, sinks);
+  need(bytes >= 0);
+  const Tensor o = one ? c.make({H, D}, at::kBFloat16) : c.make({H, Tq, D}, at::kBFloat16);
+  const Tensor ws = bytes ? c.make({bytes}, at::kByte) : Tensor();
+  const hipStream_t st = c.stream();
+  launch("w8a8_attention_sinks_bf16", [&] {
+    return w8a8_attention_sinks_bf16(bf(q), qhs, qrs, bf(*k.t), k.hs, k.rs, bf(*v.t), v.hs, v.rs, H, KV, Tq, Tk, D, start, dev, window,
+                                     sinks, scale, bfo(o), Tq * D, D, nullptr, bytes ? ws.data_ptr() : nullptr, bytes, st);
+  });
+  return wrap(o);
+}
+
 // tensors (a list or tuple), index, dim -> True
 PyObject* reorder(PyObject* const* a) {
   Call c;
@@ -910,6 +938,7 @@ PyMethodDef methods[] = {
     W8A8_ENTRY(settle, 2),      W8A8_ENTRY(decode_tree, 7),     W8A8_ENTRY(add_key_weights, 7), W8A8_ENTRY(beam_select, 3),
     W8A8_ENTRY(reorder, 3),     W8A8_ENTRY(evict, 7),         W8A8_ENTRY(verify_drafts, 7),
     W8A8_ENTRY(block_append, 8), W8A8_ENTRY(block_read, 7),     W8A8_ENTRY(block_attention, 10),
+    W8A8_ENTRY(sink_attention, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "The wrappers' launch path in native code.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -116,6 +116,10 @@ SIGNATURES = {
     "w8a8_verify_drafts_workspace_bytes": (_i64, [_i64] * 3),
     "w8a8_verify_drafts": (_i32, [_p, _p, _i32, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _f64,
                                   _p, _p, _p, _p, _i64, _p]),
+    "w8a8_attention_sinks_workspace_bytes": (_i64, [_i64] * 8),
+    "w8a8_attention_sinks_plan": (_i32, [_i64] * 8 + [_p, _p]),
+    "w8a8_attention_sinks_bf16": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                         _p, _i64, _i64, _f32, _p, _i64, _i64, _p, _p, _i64, _p]),
     "w8a8_block_cache_bytes": (_i64, [_i64] * 3),
     "w8a8_block_append": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p]),
     "w8a8_block_read": (_i32, [_p, _i64, _i64, _i64, _i32, _i64, _i64, _p, _p, _p]),

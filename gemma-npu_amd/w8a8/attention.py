@@ -8,6 +8,7 @@ local_attn.py:71-107).
     attention(q, k, v, q_start, window, scale)      -> o (and the logsumexp)
     decode(q, k, v, q_pos, window, scale)           -> o [H, D] (and the logsumexp)
     decode_tree(q, k, v, parents, n_past, window)   -> o [H, N, D] of a tree of drafted tokens
+    sink_attention(q, k, v, q_start, window, sinks) -> o [H, Tq, D], the first keys visible beside the window
     block_attention(q, c, n, window, sinks)         -> o [H, N, D] over a cache of 8-bit codes
     add_key_weights(q, k, lse, weights, q_start, W) -> weights [KV, Tk], what each key has drawn added
 
@@ -398,6 +399,71 @@ def decode_tree(q, k, v, parents, n_past, window=0, scale=1.0, out=None, return_
             float(scale), out.data_ptr(), ohs, ors, lse.data_ptr() if return_lse else None,
             None if workspace is None else workspace.data_ptr(),
             0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
+    return (out, lse) if return_lse else out
+
+
+def sink_attention_workspace_bytes(H, KV, Tq, Tk, D, q_start=None, window=0, sinks=0):
+    """Bytes of scratch sink_attention() needs (w8a8_attention_sinks_workspace_bytes); q_start None: a position held in
+    device memory."""
+    b = lib().w8a8_attention_sinks_workspace_bytes(H, KV, Tq, Tk, D, -1 if q_start is None else int(q_start), int(window), int(sinks))
+    if b < 0:
+        raise ValueError(f"sink_attention: invalid shape H={H} KV={KV} Tq={Tq} Tk={Tk} D={D} q_start={q_start} window={window} sinks={sinks}")
+    return b
+
+
+def sink_attention(q, k, v, q_start=0, window=0, sinks=0, scale=1.0, out=None, return_lse=False, workspace=None):
+    """attention() with a sliding window and the first `sinks` keys visible beside it: the query at position p sees keys
+    j <= p with p - j < window or j < sinks (window 0: all j <= p).  For conversations that run far past the window.
+
+    q: bf16 [H, Tq, D] at positions q_start .. ([H, D]: one token), k / v: bf16 [KV, Tk, D] holding positions 0 ..
+    q_start: an int, or an int32 GPU tensor of one element (the launch then does not depend on it, so a captured decode
+    step replays at each new position).  Keys that no query sees may hold anything.
+    Returns o of q's shape (into `out` if given, any strides with a contiguous last dimension), and with return_lse the
+    fp32 [H, Tq] ([H]) logsumexp.  workspace: a device uint8 tensor of at least sink_attention_workspace_bytes(...);
+    by default one from torch's allocator."""
+    if _native is not None and out is None and workspace is None and not return_lse:
+        o = _native.sink_attention(q, k, v, q_start, window, sinks, scale)
+        if o is not None:
+            return o
+    one = isinstance(q, torch.Tensor) and q.dim() == 2
+    if one:
+        q, out = q[:, None], out[:, None] if isinstance(out, torch.Tensor) and out.dim() == 2 else out
+    _check3(q, "q")
+    _check3(k, "k")
+    _check3(v, "v")
+    H, Tq, D = q.shape
+    KV, Tk, Dk = k.shape
+    if tuple(v.shape) != (KV, Tk, Dk) or Dk != D:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
+    if len({q.device, k.device, v.device}) != 1:
+        raise ValueError("q, k and v must be on one device")
+    dev = None
+    if isinstance(q_start, torch.Tensor):
+        if q_start.dtype != torch.int32 or q_start.numel() != 1 or q_start.device != q.device:
+            raise ValueError("sink_attention: q_start must be an int or an int32 tensor of one element on q's device")
+        dev, q_start = q_start, -1
+    elif not 0 <= int(q_start) <= Tk - Tq:
+        raise ValueError(f"sink_attention: {Tq} queries from position {q_start} on and {Tk} keys")
+    if out is None:
+        out = torch.empty((H, Tq, D), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out(out, "out", (H, Tq, D), q.device)
+    lse = torch.empty((H, Tq), dtype=torch.float32, device=q.device) if return_lse else None
+    if workspace is None:
+        need = sink_attention_workspace_bytes(H, KV, Tq, Tk, D, None if dev is not None else q_start, window, sinks)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError(f"sink_attention: the workspace must be a contiguous tensor on {q.device}")
+    qhs, qrs = _strides(q)
+    khs, krs = _strides(k)
+    vhs, vrs = _strides(v)
+    ohs, ors = _strides(out)
+    call_on(q, "w8a8_attention_sinks_bf16", q.data_ptr(), qhs, qrs, k.data_ptr(), khs, krs, v.data_ptr(), vhs, vrs, H, KV, Tq, Tk, D,
+            int(q_start), None if dev is None else dev.data_ptr(), int(window), int(sinks), float(scale), out.data_ptr(), ohs, ors,
+            lse.data_ptr() if return_lse else None, None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q))
+    if one:
+        out, lse = out[:, 0], lse[:, 0] if return_lse else None
     return (out, lse) if return_lse else out
 
 

@@ -716,6 +716,27 @@ int w8a8_block_attention(const uint16_t *q, int64_t q_head_stride, int64_t q_row
                          int64_t sinks, float scale, uint16_t *o, int64_t o_head_stride, int64_t o_row_stride, float *lse,
                          void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/* Attention with a sliding window and the first `sinks` keys visible beside it: q bf16 [H, Tq, D] at positions q_start ..,
+ * k / v bf16 [KV, Tk, D] holding positions 0 ..; the query at p sees keys j <= p, with a window W > 0 those with
+ * p - j < W or j < sinks.  o bf16 [H, Tq, D], lse fp32 [H, Tq] or null (natural logarithm).  Keys that no query sees are
+ * not read, or multiplied with nothing: they may hold anything.
+ *   q_start: 0 .. Tk - Tq; or -1 and q_start_dev, an int32 in device memory (brought into that range), which the launch does
+ *   not depend on
+ *   workspace: w8a8_attention_sinks_workspace_bytes(...) bytes (-1: invalid; 0: none), 16-byte aligned, scratch;
+ *   calls that overlap in time need separate ones
+ * D in {128, 256, 512}; strides in elements, multiples of 8; q, k, v and o 16-byte aligned.  Sums in fp32 in a fixed order.
+ * One or two launches.  w8a8_attention_sinks_plan: the rows of a tile and the parts of its keys (at most), for diagnostics. */
+int64_t w8a8_attention_sinks_workspace_bytes(int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D, int64_t q_start,
+                                             int64_t window, int64_t sinks);
+int w8a8_attention_sinks_plan(int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D, int64_t q_start, int64_t window,
+                              int64_t sinks, int *row_tile, int *parts);
+int w8a8_attention_sinks_bf16(const uint16_t *q, int64_t q_head_stride, int64_t q_row_stride, const uint16_t *k,
+                              int64_t k_head_stride, int64_t k_row_stride, const uint16_t *v, int64_t v_head_stride,
+                              int64_t v_row_stride, int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D, int64_t q_start,
+                              const int32_t *q_start_dev, int64_t window, int64_t sinks, float scale, uint16_t *o,
+                              int64_t o_head_stride, int64_t o_row_stride, float *lse, void *workspace,
+                              int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
