@@ -85,4 +85,52 @@ __device__ __forceinline__ void part_merge(const PartParams& p, int np, int N) {
   if (p.lse && col == 0) p.lse[int64_t(h) * N + i] = part_lse(mx, L);
 }
 
+// The same for calls of at most PART_FEW parts, many rows as a rule: a thread takes four columns of a row.
+constexpr int PART_FEW = 8;
+template <int D, class NP>
+__device__ __forceinline__ void part_merge_few(const PartParams& p, NP parts_of, int N) {
+  constexpr int T = D / 4;  // threads of a row
+  const int64_t at = int64_t(blockIdx.x) * (256 / T) + threadIdx.x / T;
+  if (at >= int64_t(p.KV) * p.rows) return;
+  const int g = int(at / p.rows), row = int(at % p.rows), col = 4 * (threadIdx.x % T), np = parts_of(row);
+  if (np <= 1) return;
+  const int64_t base = int64_t(g) * p.nparts * p.rows + row;
+  const v2f* ml = reinterpret_cast<const v2f*>(p.part_ml) + base;
+  const float* po = p.part_o + base * D + col;
+  v2f st[PART_FEW];
+  v4f v[PART_FEW];
+#pragma unroll
+  for (int s = 0; s < PART_FEW; ++s) st[s] = s < np ? ml[int64_t(s) * p.rows] : v2f{-__builtin_inff(), 0.0f};
+#pragma unroll
+  for (int s = 0; s < PART_FEW; ++s)
+    v[s] = s < np ? *reinterpret_cast<const v4f*>(po + int64_t(s) * p.rows * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  float mx = -__builtin_inff();
+#pragma unroll
+  for (int s = 0; s < PART_FEW; ++s) mx = fmaxf(mx, st[s][0]);
+  const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+  float L = 0.0f;
+  v4f acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int s = 0; s < PART_FEW; ++s) {
+    const float w = __builtin_amdgcn_exp2f(st[s][0] - ref);
+    L = __builtin_fmaf(w, st[s][1], L);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(w, v[s][i], acc[i]);
+  }
+  const int i = row / p.G, h = g * p.G + row % p.G;
+  const float inv = L > 0.0f ? 1.0f / L : (L == L ? 0.0f : L);
+  v2u w = v2u{0u, 0u};
+  if (inv != 0.0f) {
+    w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+  }
+  *reinterpret_cast<v2u*>(p.o + int64_t(h) * p.ohs + int64_t(i) * p.ors + col) = w;
+  if (p.lse && col == 0) p.lse[int64_t(h) * N + i] = part_lse(mx, L);
+}
+template <int D>
+inline dim3 part_few_grid(const PartParams& p) {
+  const int64_t per = 256 / (D / 4);
+  return dim3{unsigned((int64_t(p.KV) * p.rows + per - 1) / per), 1, 1};
+}
+
 }  // namespace w8a8

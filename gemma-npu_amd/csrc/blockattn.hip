@@ -80,18 +80,24 @@ __device__ __forceinline__ v8h codes8_f16(uint32_t lo, uint32_t hi) {
   return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Workgroups of a CU: what the registers of the row tile allow.
-constexpr int block_occupancy(int rt, int d) { return rt * d <= 512 ? 2 : 1; }
+// Row groups of a workgroup's waves (four waves each), workgroups of a CU, and blocks on their way in a wave's registers.
+// From 32 rows on two groups hold half of the queries each and an eighth of head_dim of all rows' outputs.
+constexpr int block_groups(int rt) { return rt == 1 ? 1 : 2; }
+constexpr int block_occupancy(int rt, int d) { return rt > 1 ? 1 : d == 128 ? 3 : 2; }
+constexpr int block_ahead(int rt, int d) { return d == 128 ? (rt <= 2 ? 4 : 2) : d == 256 && rt <= 4 ? 2 : 1; }
 
 template <int D, int RT, bool E4M3>
-__global__ __launch_bounds__(256, block_occupancy(RT, D)) void block_attn_kernel(BlockAttnParams p) {
-  constexpr int R = 16 * RT, NJ = D / 64, NKK = D / 32;
-  constexpr int PLD = BLK + 8;  // padded row of softmax weights
+__global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_occupancy(RT, D)) void block_attn_kernel(BlockAttnParams p) {
+  constexpr int R = 16 * RT, RG = block_groups(RT), NW = 4 * RG, RW = RT / RG;  // row tiles of a wave's S phase
+  constexpr int NK = D / 64, NV = D / 16 / NW, NKK = D / 32;                    // a wave's fragments of keys, of values; k-steps
+  constexpr int PLD = BLK + 8;                                                  // padded row of softmax weights
+  __shared__ __attribute__((aligned(16))) uint16_t qs[R * D];  // the tile's queries, chunk c of row r at c ^ (r & 15)
   __shared__ __attribute__((aligned(16))) uint16_t pl[2][R * PLD];
-  __shared__ float smax[2][4][R];
-  __shared__ float lsum[4][R];
+  __shared__ float smax[2][4][R], alpha_s[2][R], lsum[4][R], cqs[R];
+  __shared__ int flag_s[2][8];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 15, qq = lane >> 4;
+  const int kt = wave & 3, r0 = 16 * RW * (wave >> 2);  // this wave's key tile and first row in the S phase
   const int G = p.out.G, rows = p.out.rows;
   const int lb = xcd_remap(blockIdx.x, gridDim.x);
   const int tile = lb % p.ntiles, pair = lb / p.ntiles, g = pair / p.out.nparts, part = pair % p.out.nparts;
@@ -104,133 +110,180 @@ __global__ __launch_bounds__(256, block_occupancy(RT, D)) void block_attn_kernel
   const int ncode = i_hi - i_lo - (has_ring ? 1 : 0);
   const int win = p.window, sinks = p.sinks;
 
+  // Blocks' keys and values on their way in registers, PF of each, with their scales
+  constexpr int PF = block_ahead(RT, D);
   const int64_t head = int64_t(g) * p.c.blocks;
-  const uint8_t* const kc = p.c.k + head * BLK * D + wave * (16 * D) + lane * 16;
-  const uint8_t* const vc = p.c.v + head * BLK * D + wave * (16 * D) + lane * 16;
-  v4u kr[NJ], vr[NJ];
-  auto load_k = [&](int i) __attribute__((always_inline)) {
-    const uint8_t* at = kc + int64_t(block(i)) * (BLK * D);
+  const uint8_t* const kc = p.c.k + head * BLK * D + kt * (16 * D) + lane * 16;
+  const uint8_t* const vc = p.c.v + head * BLK * D + wave * (NV * 1024) + lane * 16;
+  v4u kr[PF][NK], vr[PF][NV];
+  float ksr[PF], vsr[PF];
+  auto load_k = [&](int u, int i) __attribute__((always_inline)) {
+    const int b = block(i);
+    const uint8_t* at = kc + int64_t(b) * (BLK * D);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const v4u*>(at + j * 1024);
+    for (int j = 0; j < NK; ++j) kr[u][j] = *reinterpret_cast<const v4u*>(at + j * 1024);
+    // (vector loads, which are waited for in order: a scalar one would stall the block that needs it)
+    ksr[u] = p.c.ks[head + b + (lane >> 6)];
+    vsr[u] = p.c.vs[head + b + (lane >> 6)];
   };
-  auto load_v = [&](int i) __attribute__((always_inline)) {
+  auto load_v = [&](int u, int i) __attribute__((always_inline)) {
     const uint8_t* at = vc + int64_t(block(i)) * (BLK * D);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) vr[j] = *reinterpret_cast<const v4u*>(at + j * 1024);
+    for (int j = 0; j < NV; ++j) vr[u][j] = *reinterpret_cast<const v4u*>(at + j * 1024);
   };
-  if (ncode > 0) {
-    load_k(i_lo);
-    load_v(i_lo);
-  }
 
-  // the tile's rows: this lane's are 16 rt + qi
-  int pos[RT];
-  const uint16_t* qp[RT];
-  bool valid[RT];
+  // The tile's queries, asked for before the keys and values, whose arrival their conversion hides: a wave takes
+  // R / NW rows, D / 8 lanes a row.
+  constexpr int LPR = D / 8, RPI = 64 / LPR, NI = R / NW / RPI;  // lanes of a row, rows at a time, times
+  auto staged = [&](int i) __attribute__((always_inline)) { return wave * (R / NW) + i * RPI + lane / LPR; };
+  auto place = [&](int r) __attribute__((always_inline)) {
+    return reinterpret_cast<v4u*>(qs + r * D + 8 * ((lane % LPR) ^ (r & 15)));
+  };
+  v4u qw[NI];
+  auto ask_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = tile * R + 16 * rt + qi;
-    valid[rt] = r < rows;
-    const int i = valid[rt] ? r / G : 0, h = valid[rt] ? r % G : 0;
-    pos[rt] = valid[rt] ? geo.n - p.N + i : -1;  // (sees nothing)
-    qp[rt] = p.q + int64_t(g * G + h) * p.qhs + int64_t(i) * p.qrs + 16 * qq;
+    for (int i = 0; i < NI; ++i) {
+      const int row = tile * R + staged(i);
+      qw[i] = v4u{0u, 0u, 0u, 0u};
+      if (row < rows)
+        qw[i] = *reinterpret_cast<const v4u*>(p.q + int64_t(g * G + row % G) * p.qhs + int64_t(row / G) * p.qrs + 8 * (lane % LPR));
+    }
+  };
+  auto put_q = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) *place(staged(i)) = qw[i];
+  };
+  ask_q();
+  __builtin_amdgcn_sched_barrier(0);
+  if (ncode > 0) load_k(0, i_lo);
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {  // in the order of their use
+    if (u + 1 < PF && u + 1 < ncode) load_k(u + 1, i_lo + u + 1);
+    if (u < ncode) load_v(u, i_lo + u);
   }
-  // Q as the B operand of k-step 2 j + h: q[64 j + 16 qq + 8 h .. + 7], which is how the codes lie
-  v8h qf[RT][NKK];
-  float cq[RT];  // what a score of this row is multiplied by
+  __builtin_amdgcn_sched_barrier(0);
+  int pos[RW];  // of this lane's rows r0 + 16 rt + qi
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    v4u w[NKK];
+  for (int rt = 0; rt < RW; ++rt) {
+    const int row = tile * R + r0 + 16 * rt + qi;
+    pos[rt] = row < rows ? geo.n - p.N + row / G : -1;  // (sees nothing)
+  }
+  put_q();
+  // .. made fp16 in their places (a short loop: what such a kernel waits for first is its own instructions)
+#pragma unroll 2
+  for (int i = 0; i < NI; ++i) {
+    const int r = staged(i);
+    const v4u w = *place(r);
     uint32_t m2 = 0u;
 #pragma unroll
-    for (int k = 0; k < NKK; ++k) {
-      w[k] = v4u{0u, 0u, 0u, 0u};
-      if (valid[rt]) w[k] = *reinterpret_cast<const v4u*>(qp[rt] + 64 * (k >> 1) + 8 * (k & 1));
+    for (int e = 0; e < 4; ++e) m2 = absmax_bf16x2(m2, w[e]);
+    float top = absmax_pair(m2);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m2 = absmax_bf16x2(m2, w[k][e]);
-    }
-    const float top = lanes4_max(absmax_pair(m2));
+    for (int o = LPR / 2; o > 0; o >>= 1) top = absmax2(top, __shfl_xor(top, o, 64));
     // 2^10 over the power of two at or below `top` (no smaller than 2^-87: zeros)
     const uint32_t e = max(__float_as_uint(top) >> 23, 40u);
     const float f = __uint_as_float((264u - e) << 23);
-    cq[rt] = p.cs * __uint_as_float((e - 10u) << 23);
+    v4u h;
 #pragma unroll
-    for (int k = 0; k < NKK; ++k) {
-      float x[8];
-      unpack8(w[k], x);
+    for (int j = 0; j < 4; ++j)  // (exact but for subnormals, whose rounding towards zero is below 2^-24 of 2^10)
+      h[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w[j] << 16) * f,
+                                                                     __uint_as_float(w[j] & 0xffff0000u) * f));
+    *place(r) = h;
+    if (lane % LPR == 0) cqs[r] = p.cs * __uint_as_float((e - 10u) << 23);
+  }
+  __syncthreads();
+  // .. and read as the B operand of k-step 2 j + h: q[64 j + 16 qq + 8 h .. + 7], which is how the codes lie
+  // (where registers are short half of them stay in LDS)
+  constexpr int NQ = 4 * (RW * NKK + NV * RT) > 180 ? NKK / 2 : NKK;
+  v8h qf[RW][NQ];
+  auto frag = [&](int rt, int k) __attribute__((always_inline)) {
+    return *reinterpret_cast<const v4u*>(qs + (r0 + 16 * rt + qi) * D + 8 * ((8 * (k >> 1) + 2 * qq + (k & 1)) ^ qi));
+  };
+  float cq[RW];  // what a score of the row is multiplied by
 #pragma unroll
-      for (int j = 0; j < 8; ++j) qf[rt][k][j] = _Float16(x[j] * f);
-    }
+  for (int rt = 0; rt < RW; ++rt) {
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) qf[rt][k] = __builtin_bit_cast(v8h, frag(rt, k));
+    cq[rt] = cqs[r0 + 16 * rt + qi];
   }
 
-  float ms[RT], l[RT], alpha[RT];
-  bool grew = false;  // some row of this lane's had its O rescaled last time
+  float ms[RW], l[RW];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) ms[rt] = -__builtin_inff(), l[rt] = 0.0f, alpha[rt] = 1.0f;
-  v4f o[NJ][RT];
+  for (int rt = 0; rt < RW; ++rt) ms[rt] = -__builtin_inff(), l[rt] = 0.0f;
+  v4f o[NV][RT];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j)
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) o[j][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  v4f s[RT];
+  v4f s[RW];
   float tb = 0.0f, tinv = 1.0f;  // log2 of the block's value scale, and one over the scale
-  auto seen = [&](int key, int at) __attribute__((always_inline)) {
-    return (key <= at) & ((win <= 0) | (at - key < win) | (key < sinks));
+  const uint32_t near = win > 0 ? uint32_t(win) : 0x80000000u;
+  auto seen = [&](int key, int at) __attribute__((always_inline)) {  // (compares alone: a branch here is one per score)
+    return (uint32_t(at - key) < near) | ((key <= at) & (key < sinks));
   };
   auto inner = [&](int b) __attribute__((always_inline)) {  // every row sees the whole block
     const int kb = b * BLK;
     return kb + BLK - 1 <= geo.pmin && (win <= 0 || kb > geo.pmax - win || kb + BLK <= sinks) && tile * R + R <= rows;
   };
   // scores in exponents (log2), masked; this wave's row maxima into LDS
-  auto finish_s = [&](int slot, int b, float ks) __attribute__((always_inline)) {
+  auto finish_s = [&](int slot, int b, float ks, bool codes) __attribute__((always_inline)) {
     const bool all = inner(b);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float f = ks * cq[rt];
-      float bm = -__builtin_inff();
+    for (int rt = 0; rt < RW; ++rt) {
+      const float f = codes ? ks * cq[rt] : p.cs;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = __builtin_fmaf(s[rt][i], f, tb);
-        if (!all) x = attn_mask(x, seen(b * BLK + 16 * wave + 4 * qq + i, pos[rt]));
-        s[rt][i] = x;
-        bm = fmaxf(bm, x);
-      }
-      bm = lanes4_max(bm);
-      if (qq == 0) smax[slot][wave][16 * rt + qi] = bm;
+      for (int i = 0; i < 4; ++i) s[rt][i] = __builtin_fmaf(s[rt][i], f, tb);
+    }
+    if (!all)
+#pragma unroll
+      for (int rt = 0; rt < RW; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[rt][i] = attn_mask(s[rt][i], seen(b * BLK + 16 * kt + 4 * qq + i, pos[rt]));
+#pragma unroll
+    for (int rt = 0; rt < RW; ++rt) {
+      const float bm = lanes4_max(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3])));
+      if (qq == 0) smax[slot][kt][r0 + 16 * rt + qi] = bm;
     }
   };
-  auto s_phase = [&](int slot, int i) __attribute__((always_inline)) {
-    const int b = block(i);
-    const float ks = p.c.ks[head + b], vs = p.c.vs[head + b];
+  auto s_phase = [&](int slot, int u, int i) __attribute__((always_inline)) {
+    const float ks = ksr[u], vs = vsr[u];
     tb = __builtin_amdgcn_logf(vs);
     tinv = 1.0f / vs;
-    v4f s2[RT];
+    constexpr int NS = RW == 1 ? 2 : 1;  // one row tile: two chains of products
+    v4f acc[NS][RW];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) s[rt] = s2[rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int n = 0; n < NS; ++n)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const v8h a = codes8_f16<E4M3>(kr[j][0], kr[j][1]), c = codes8_f16<E4M3>(kr[j][2], kr[j][3]);
+      for (int rt = 0; rt < RW; ++rt) acc[n][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[rt][2 * j], s[rt], 0, 0, 0);
-        s2[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[rt][2 * j + 1], s2[rt], 0, 0, 0);
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v8h a = codes8_f16<E4M3>(kr[u][j][2 * h], kr[u][j][2 * h + 1]);
+#pragma unroll
+        for (int rt = 0; rt < RW; ++rt) {
+          const v8h q = 2 * j + h < NQ ? qf[rt][(2 * j + h) % NQ] : __builtin_bit_cast(v8h, frag(rt, 2 * j + h));
+          acc[h % NS][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q, acc[h % NS][rt], 0, 0, 0);
+        }
       }
+#pragma unroll
+    for (int rt = 0; rt < RW; ++rt) {
+      s[rt] = acc[0][rt];
+      if constexpr (NS == 2) s[rt] += acc[1][rt];
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) s[rt] += s2[rt];
-    finish_s(slot, b, ks);
+    finish_s(slot, block(i), ks, true);
   };
-  // after the barrier: the rows' new references, P' into LDS
+  // after the barrier: the rows' new references and P' into LDS, with what O is rescaled by
   auto softmax = [&](int slot, auto half) __attribute__((always_inline)) {
-    grew = false;
+    bool grew = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = 16 * rt + qi;
+    for (int rt = 0; rt < RW; ++rt) {
+      const int r = r0 + 16 * rt + qi;
       const float m = fmaxf(fmaxf(smax[slot][0][r], smax[slot][1][r]), fmaxf(smax[slot][2][r], smax[slot][3][r]));
       const bool grow = m > ms[rt] + 8.0f;  // false while every key so far is masked
       const bool had = ms[rt] != -__builtin_inff();
-      alpha[rt] = !grow ? 1.0f : (had ? __builtin_amdgcn_exp2f(ms[rt] - m) : 0.0f);
+      const float alpha = !grow ? 1.0f : (had ? __builtin_amdgcn_exp2f(ms[rt] - m) : 0.0f);
       grew |= grow && had;
       ms[rt] = grow ? m : ms[rt];
       const float ref = ms[rt] == -__builtin_inff() ? 0.0f : ms[rt];
@@ -246,32 +299,41 @@ __global__ __launch_bounds__(256, block_occupancy(RT, D)) void block_attn_kernel
           w[i] = f32_to_bf16(e);
       }
       // (a block that a row sees nothing of adds nothing, whatever its scale)
-      l[rt] = __builtin_fmaf(sum, sum != 0.0f ? tinv : 0.0f, l[rt] * alpha[rt]);
-      // key 16 wave + 4 qq + i is slot 4 (wave % 2) + i of lane group qq in k-step wave / 2
-      *reinterpret_cast<v2u*>(&pl[slot][r * PLD + 32 * (wave >> 1) + 8 * qq + 4 * (wave & 1)]) =
+      l[rt] = __builtin_fmaf(sum, sum != 0.0f ? tinv : 0.0f, l[rt] * alpha);
+      // key 16 kt + 4 qq + i is slot 4 (kt % 2) + i of lane group qq in k-step kt / 2
+      *reinterpret_cast<v2u*>(&pl[slot][r * PLD + 32 * (kt >> 1) + 8 * qq + 4 * (kt & 1)]) =
           v2u{uint32_t(w[0]) | uint32_t(w[1]) << 16, uint32_t(w[2]) | uint32_t(w[3]) << 16};
+      if (kt == 0 && qq == 0) alpha_s[slot][r] = alpha;
     }
+    const bool any = __builtin_amdgcn_ballot_w64(grew) != 0;
+    if (kt == 0 && lane == 0) flag_s[slot][wave >> 2] = any ? 1 : 0;
   };
-  auto rescale = [&]() __attribute__((always_inline)) {
-    if (__builtin_amdgcn_ballot_w64(grew))
+  auto rescale = [&](int slot) __attribute__((always_inline)) {
+    int f = flag_s[slot][0];
+    if constexpr (RG == 2) f |= flag_s[slot][1];
+    if (f != 0)
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int rt = 0; rt < RT; ++rt) {
+        const float a = alpha_s[slot][16 * rt + qi];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o[j][rt] *= alpha[rt];
+        for (int j = 0; j < NV; ++j) o[j][rt] *= a;
+      }
   };
-  auto pv_phase = [&](int slot) __attribute__((always_inline)) {
-    rescale();
+  auto weights = [&](int slot, int rt, int h) __attribute__((always_inline)) {
+    return *reinterpret_cast<const v4u*>(&pl[slot][(16 * rt + qi) * PLD + 32 * h + 8 * qq]);
+  };
+  auto pv_phase = [&](int slot, int u) __attribute__((always_inline)) {
+    rescale(slot);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      v8h pb[RT];
+      v8h a[NV];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        pb[rt] = *reinterpret_cast<const v8h*>(&pl[slot][(16 * rt + qi) * PLD + 32 * h + 8 * qq]);
+      for (int j = 0; j < NV; ++j) a[j] = codes8_f16<E4M3>(vr[u][j][2 * h], vr[u][j][2 * h + 1]);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const v8h a = codes8_f16<E4M3>(vr[j][2 * h], vr[j][2 * h + 1]);
+      for (int rt = 0; rt < RT; ++rt) {
+        const v8h pb = __builtin_bit_cast(v8h, weights(slot, rt, h));
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pb[rt], o[j][rt], 0, 0, 0);
+        for (int j = 0; j < NV; ++j) o[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], pb, o[j][rt], 0, 0, 0);
       }
     }
   };
@@ -281,125 +343,142 @@ __global__ __launch_bounds__(256, block_occupancy(RT, D)) void block_attn_kernel
   // Block i's scores and maxima are made one iteration ahead of its P V: the barrier between them makes the maxima of
   // block i + 1 and the weights of block i visible at once.
   if (ncode > 0) {
-    s_phase(0, i_lo);
-    if (ncode > 1) load_k(i_lo + 1);
+    s_phase(0, 0, i_lo);
+    if (PF < ncode) load_k(0, i_lo + PF);
     __syncthreads();
     softmax(0, Yes{});
-    for (int x = 0; x < ncode; ++x) {
-      const int slot = x & 1;
-      const bool more = x + 1 < ncode;
-      if (more) {
-        s_phase(slot ^ 1, i_lo + x + 1);
-        if (x + 2 < ncode) load_k(i_lo + x + 2);
+    for (int x0 = 0; x0 < ncode; x0 += PF)
+#pragma unroll
+      for (int u = 0; u < PF; ++u) {
+        const int x = x0 + u, slot = x & 1;
+        if (x >= ncode) break;
+        const bool more = x + 1 < ncode;
+        if (more) {
+          s_phase(slot ^ 1, (u + 1) % PF, i_lo + x + 1);
+          if (x + 1 + PF < ncode) load_k((u + 1) % PF, i_lo + x + 1 + PF);
+        }
+        __syncthreads();
+        pv_phase(slot, u);
+        if (x + PF < ncode) load_v(u, i_lo + x + PF);
+        if (more) softmax(slot ^ 1, Yes{});
       }
-      __syncthreads();
-      pv_phase(slot);
-      if (more) {
-        load_v(i_lo + x + 1);
-        softmax(slot ^ 1, Yes{});
-      }
-    }
   }
 
   if (has_ring) {
-    // the unfinished block: bf16 rows, of which the first `live` are there
+    // the unfinished block: bf16 rows, of which the first `live` are there, against the queries in bf16
     const int b = whole, live = geo.n - whole * BLK, slot = ncode & 1;
-    const uint16_t* const kt = p.c.kt + (int64_t(g) * 2 + (b & 1)) * BLK * D;
-    const uint16_t* const vt = p.c.vt + (int64_t(g) * 2 + (b & 1)) * BLK * D;
+    const uint16_t* const rk = p.c.kt + (int64_t(g) * 2 + (b & 1)) * BLK * D + (kt * NKK * 64 + lane) * 8;
+    const uint16_t* const rv = p.c.vt + (int64_t(g) * 2 + (b & 1)) * BLK * D + (wave * NV * 2 * 64 + lane) * 8;
+    ask_q();
+    v4u vw[NV][2];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) s[rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (16 * wave < live) {
-#pragma unroll 4
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) vw[j][h] = *reinterpret_cast<const v4u*>(rv + (2 * j + h) * 512);
+    put_q();
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RW; ++rt) s[rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (16 * kt < live) {
+#pragma unroll 8
       for (int k = 0; k < NKK; ++k) {
-        const v8bf a = *reinterpret_cast<const v8bf*>(kt + ((wave * NKK + k) * 64 + lane) * 8);
+        const v8bf a = *reinterpret_cast<const v8bf*>(rk + k * 512);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          v4u w = v4u{0u, 0u, 0u, 0u};
-          if (valid[rt]) w = *reinterpret_cast<const v4u*>(qp[rt] + 64 * (k >> 1) + 8 * (k & 1));
-          s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(v8bf, w), s[rt], 0, 0, 0);
-        }
+        for (int rt = 0; rt < RW; ++rt)
+          s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(v8bf, frag(rt, k)), s[rt], 0, 0, 0);
       }
     }
     tb = 0.0f;
     tinv = 1.0f;
+    finish_s(slot, b, 1.0f, false);  // (rows from `live` on lie behind every position)
+    // values of rows that aren't there are zero, infinities and NaN (0 x inf) leave the product and are added below to
+    // the rows that see them
+    uint32_t bad = 0u;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) cq[rt] = p.cs;
-    finish_s(slot, b, 1.0f);  // (rows from `live` on lie behind every position)
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = 32 * h + 16 * (e >> 1) + 4 * qq + 2 * (e & 1);  // of the word's low half
+        const uint32_t there = (key < live ? 0xffffu : 0u) | (key + 1 < live ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          vw[j][h][e] &= there;
+          bad |= (vw[j][h][e] & 0x7f807f80u) + 0x00800080u;
+        }
+      }
+    const bool any = __builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0u) != 0;
+    if (any)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = ((vw[j][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+            vw[j][h][e] &= ~((x >> 15) * 0xffffu);
+          }
     __syncthreads();
     softmax(slot, No{});
     __syncthreads();
-    rescale();
-    bool bad = false;
+    rescale(slot);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (32 * h >= live) break;
-      v8bf pb[RT];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        pb[rt] = *reinterpret_cast<const v8bf*>(&pl[slot][(16 * rt + qi) * PLD + 32 * h + 8 * qq]);
+      for (int rt = 0; rt < RT; ++rt) {
+        const v8bf pb = __builtin_bit_cast(v8bf, weights(slot, rt, h));
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        v4u w = *reinterpret_cast<const v4u*>(vt + (((wave * NJ + j) * 2 + h) * 64 + lane) * 8);
-        // rows that aren't there are zero; infinities and NaN leave the product (0 x inf) and are added below to
-        // the rows that see them
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t m = e & 1 ? 0xffff0000u : 0xffffu;
-          const bool gone = 32 * h + 16 * (e >> 2) + 4 * qq + (e & 3) >= live;
-          const bool inf = (w[e >> 1] & m & 0x7f807f80u) == (m & 0x7f807f80u);
-          bad |= inf && !gone;
-          if (gone || inf) w[e >> 1] &= ~m;
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          o[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), pb[rt], o[j][rt], 0, 0, 0);
+        for (int j = 0; j < NV; ++j)
+          o[j][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, vw[j][h]), pb, o[j][rt], 0, 0, 0);
       }
-    }
-    if (__builtin_amdgcn_ballot_w64(bad)) {
+    if (any) {
+      const uint16_t* const vt = p.c.vt + (int64_t(g) * 2 + (b & 1)) * BLK * D;
 #pragma unroll 1
       for (int key = 0; key < live; ++key)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t x = uint32_t(vt[ring_value(key, 16 * (wave * NJ + j) + 4 * qq + i)]) << 16;
+            const uint32_t x = uint32_t(vt[ring_value(key, 16 * (wave * NV + j) + 4 * qq + i)]) << 16;
             if ((x & 0x7f800000u) != 0x7f800000u) continue;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              if (seen(b * BLK + key, pos[rt])) o[j][rt][i] += __uint_as_float(x);
+            for (int rt = 0; rt < RT; ++rt) {
+              const int row = tile * R + 16 * rt + qi;
+              if (row < rows && seen(b * BLK + key, geo.n - p.N + row / G)) o[j][rt][i] += __uint_as_float(x);
+            }
           }
     }
   }
 
   // the rows' sums over the waves' keys
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
+  for (int rt = 0; rt < RW; ++rt) {
     const float x = lanes4_sum(l[rt]);
-    if (qq == 0) lsum[wave][16 * rt + qi] = x;
+    if (qq == 0) {
+      lsum[kt][r0 + 16 * rt + qi] = x;
+      if (kt == 0) cqs[r0 + 16 * rt + qi] = ms[rt];
+    }
   }
   __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = 16 * rt + qi;
+    const int r = 16 * rt + qi, row = tile * R + r, d = wave * (16 * NV) + 4 * qq;  // + 16 j + i
     const float lt = (lsum[0][r] + lsum[1][r]) + (lsum[2][r] + lsum[3][r]);
-    if (!valid[rt]) continue;
-    const int row = tile * R + r, d = wave * (D / 4) + 4 * qq;  // + 16 j + i
+    if (row >= rows) continue;
     if (geo.np > 1) {
       const int64_t at = (int64_t(g) * p.out.nparts + part) * rows + row;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) *reinterpret_cast<v4f*>(p.out.part_o + at * D + d + 16 * j) = o[j][rt];
-      if (wave == 0 && qq == 0) *reinterpret_cast<v2f*>(p.out.part_ml + at * 2) = v2f{ms[rt], lt};
+      for (int j = 0; j < NV; ++j) *reinterpret_cast<v4f*>(p.out.part_o + at * D + d + 16 * j) = o[j][rt];
+      if (wave == 0 && qq == 0) *reinterpret_cast<v2f*>(p.out.part_ml + at * 2) = v2f{cqs[r], lt};
       continue;
     }
     const float inv = lt > 0.0f ? 1.0f / lt : (lt == lt ? 0.0f : lt);  // (a NaN sum stays one)
     uint16_t* const op = p.out.o + int64_t(g * G + row % G) * p.out.ohs + int64_t(row / G) * p.out.ors + d;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NV; ++j)
       *reinterpret_cast<v2u*>(op + 16 * j) =
           inv != 0.0f ? v2u{pack_bf16x2(o[j][rt][0] * inv, o[j][rt][1] * inv), pack_bf16x2(o[j][rt][2] * inv, o[j][rt][3] * inv)}
                       : v2u{0u, 0u};
-    if (p.out.lse && wave == 0 && qq == 0)
-      p.out.lse[int64_t(g * G + row % G) * p.N + row / G] = part_lse(ms[rt], lt);
+    if (p.out.lse && wave == 0 && qq == 0) p.out.lse[int64_t(g * G + row % G) * p.N + row / G] = part_lse(cqs[r], lt);
   }
 }
 
@@ -407,6 +486,10 @@ template <int D>
 __global__ __launch_bounds__(256) void block_merge_kernel(BlockAttnParams p, int R) {
   const int row = blockIdx.x % p.out.rows;
   part_merge<D>(p.out, block_geom(p, row / R, R).np, p.N);
+}
+template <int D>
+__global__ __launch_bounds__(256) void block_merge_few_kernel(BlockAttnParams p, int R) {
+  part_merge_few<D>(p.out, [&](int row) { return block_geom(p, row / R, R).np; }, p.N);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -418,8 +501,7 @@ struct BlockPlan {
 static BlockPlan block_plan(int64_t H, int64_t KV, int64_t N, int64_t n, int64_t D, int64_t window, int64_t sinks) {
   const int64_t rows = N * (H / KV);
   BlockPlan pl;
-  const int most = D == 512 ? 2 : 4;
-  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : most;
+  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : D == 512 || rows <= 64 ? 4 : 8;
   pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
   // the blocks of a tile
   const int64_t span = window > 0 ? std::min<int64_t>(n, window + 16 * pl.rt / (H / KV) + 1 + BLK) / BLK + 1 + (std::min(sinks, n) + BLK - 1) / BLK
@@ -434,14 +516,17 @@ static BlockPlan block_plan(int64_t H, int64_t KV, int64_t N, int64_t n, int64_t
 template <int D, bool E4M3>
 static void block_launch(const BlockAttnParams& p, const BlockPlan& pl, hipStream_t stream) {
   const dim3 grid{unsigned(pl.ntiles) * unsigned(p.out.KV) * unsigned(p.out.nparts), 1, 1};
-  if (pl.rt == 1)
-    block_attn_kernel<D, 1, E4M3><<<grid, 256, 0, stream>>>(p);
-  else if (pl.rt == 2)
-    block_attn_kernel<D, 2, E4M3><<<grid, 256, 0, stream>>>(p);
-  else if constexpr (D < 512)
-    block_attn_kernel<D, 4, E4M3><<<grid, 256, 0, stream>>>(p);
-  if (p.out.nparts > 1)
+  switch (pl.rt) {
+    case 1: block_attn_kernel<D, 1, E4M3><<<grid, 256, 0, stream>>>(p); break;
+    case 2: block_attn_kernel<D, 2, E4M3><<<grid, 512, 0, stream>>>(p); break;
+    case 4: block_attn_kernel<D, 4, E4M3><<<grid, 512, 0, stream>>>(p); break;
+    default:
+      if constexpr (D < 512) block_attn_kernel<D, 8, E4M3><<<grid, 512, 0, stream>>>(p);
+  }
+  if (p.out.nparts > PART_FEW)
     block_merge_kernel<D><<<dim3{unsigned(p.out.KV) * unsigned(p.out.rows), unsigned(D / 64), 1}, 256, 0, stream>>>(p, 16 * pl.rt);
+  else if (p.out.nparts > 1)
+    block_merge_few_kernel<D><<<part_few_grid<D>(p.out), 256, 0, stream>>>(p, 16 * pl.rt);
 }
 
 static bool block_attn_shape_ok(int64_t H, int64_t KV, int64_t N, int64_t capacity, int64_t D, int64_t window, int64_t sinks) {

@@ -173,8 +173,9 @@ __global__ __launch_bounds__(sink_waves(RT, D) * 64, 1) void attn_sink_kernel(Si
   }
   if (nblk > 1) issue_k(Odd{}, 1);
 
-  auto seen = [&](int key, int at) __attribute__((always_inline)) {
-    return (key <= at) & ((win <= 0) | (at - key < win) | (key < sinks));
+  const uint32_t near = win > 0 ? uint32_t(win) : 0x80000000u;
+  auto seen = [&](int key, int at) __attribute__((always_inline)) {  // (compares alone: a branch here is one per score)
+    return (uint32_t(at - key) < near) | ((key <= at) & (key < sinks));
   };
   // Block n is seen whole by every row.
   const bool full = tile * R + R <= rows;
@@ -440,6 +441,10 @@ __global__ __launch_bounds__(256) void sink_merge_kernel(SinkParams p, int R) {
   const int row = blockIdx.x % p.out.rows;
   part_merge<D>(p.out, sink_geom<BN>(p, row / R, R).np, p.Tq);
 }
+template <int D, int BN>
+__global__ __launch_bounds__(256) void sink_merge_few_kernel(SinkParams p, int R) {
+  part_merge_few<D>(p.out, [&](int row) { return sink_geom<BN>(p, row / R, R).np; }, p.Tq);
+}
 
 // ---- host ----------------------------------------------------------------------------------------
 
@@ -494,9 +499,11 @@ static void sink_launch(const SinkParams& p, int rt, hipStream_t stream) {
     case 4: attn_sink_kernel<D, 4><<<grid, SinkShape<D, 4>::NT, 0, stream>>>(p); break;
     default: attn_sink_kernel<D, 8><<<grid, SinkShape<D, 8>::NT, 0, stream>>>(p);
   }
-  if (p.out.nparts > 1)
+  if (p.out.nparts > PART_FEW)
     sink_merge_kernel<D, SinkShape<D, 1>::BN>
         <<<dim3{unsigned(p.out.KV) * unsigned(p.out.rows), unsigned(D / 64), 1}, 256, 0, stream>>>(p, 16 * rt);
+  else if (p.out.nparts > 1)
+    sink_merge_few_kernel<D, SinkShape<D, 1>::BN><<<part_few_grid<D>(p.out), 256, 0, stream>>>(p, 16 * rt);
 }
 
 static bool sink_shape_ok(int64_t H, int64_t KV, int64_t Tq, int64_t Tk, int64_t D, int64_t window, int64_t sinks) {
