@@ -501,7 +501,7 @@ struct BlockPlan {
 static BlockPlan block_plan(int64_t H, int64_t KV, int64_t N, int64_t n, int64_t D, int64_t window, int64_t sinks) {
   const int64_t rows = N * (H / KV);
   BlockPlan pl;
-  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : D == 512 || rows <= 64 ? 4 : 8;
+  pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : D >= 256 || rows <= 64 ? 4 : 8;
   pl.ntiles = int((rows + 16 * pl.rt - 1) / (16 * pl.rt));
   // the blocks of a tile
   const int64_t span = window > 0 ? std::min<int64_t>(n, window + 16 * pl.rt / (H / KV) + 1 + BLK) / BLK + 1 + (std::min(sinks, n) + BLK - 1) / BLK
@@ -521,7 +521,7 @@ static void block_launch(const BlockAttnParams& p, const BlockPlan& pl, hipStrea
     case 2: block_attn_kernel<D, 2, E4M3><<<grid, 512, 0, stream>>>(p); break;
     case 4: block_attn_kernel<D, 4, E4M3><<<grid, 512, 0, stream>>>(p); break;
     default:
-      if constexpr (D < 512) block_attn_kernel<D, 8, E4M3><<<grid, 512, 0, stream>>>(p);
+      if constexpr (D == 128) block_attn_kernel<D, 8, E4M3><<<grid, 512, 0, stream>>>(p);
   }
   if (p.out.nparts > PART_FEW)
     block_merge_kernel<D><<<dim3{unsigned(p.out.KV) * unsigned(p.out.rows), unsigned(D / 64), 1}, 256, 0, stream>>>(p, 16 * pl.rt);

@@ -6,9 +6,9 @@
 // rows came, and rows may be written again (drafted tokens taken back) while the ring has their block's others.
 //
 // block_append_kernel: a workgroup takes a block's keys (or values) of one head.  New rows go into the ring if their block is
-// one of the call's last two; a block that is whole is staged in LDS (new rows from the call's, old ones from the
-// ring), its largest magnitude taken on the way, and its codes written in fragment order.  Memory bounds long calls, one
-// kernel's start short ones.
+// one of the call's last two.  A block that has become whole is taken from the ring, which lies as the codes do, if some
+// of its rows were there before, else staged in LDS; its largest magnitude is taken on the way.  Memory bounds long calls
+// (65521 rows of 8 heads of 128: 82 us of 79 at a copy's rate), one kernel's start and two round trips short ones.
 #include <algorithm>
 
 #include "blocks.h"
@@ -78,54 +78,54 @@ __global__ __launch_bounds__(256) void block_append_kernel(AppendParams p) {
     }
   };
 
-  const bool whole = hi == BLK;
-  if (whole) {
+  const bool whole = hi == BLK, old = lo > 0;  // (old rows: the call's first block alone)
+  const int64_t blk = int64_t(g) * p.c.blocks + b;
+  uint8_t* const out = (value ? p.c.v : p.c.k) + blk * BLK * D;
+  auto block_top = [&](uint32_t m2) __attribute__((always_inline)) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m2 = absmax_bf16x2(m2, __shfl_xor(m2, o, 64));
+    if ((t & 63) == 0) red[t >> 6] = m2;
+    __syncthreads();
+    return absmax_pair(absmax_bf16x2(absmax_bf16x2(red[0], red[1]), absmax_bf16x2(red[2], red[3])));
+  };
+  if (whole && old) {
+    // its new rows join the others in the ring, which lies as the codes do: 16 codes are two of its chunks
+    to_ring(b);
+    __syncthreads();
+    const uint16_t* const at = ring + (b & 1) * BLK * D;
+    v4u w[NU];
+    uint32_t m2 = 0u;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int i = t + 256 * (u >> 1);
+      w[u] = *reinterpret_cast<const v4u*>(at + ((2 * (i >> 6) + (u & 1)) * 64 + (i & 63)) * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m2 = absmax_bf16x2(m2, w[u][e]);
+    }
+    const float s = code_scale(block_top(m2), E4M3), inv = 1.0f / s;
+    const bool finite = quant_finite(s);
+    if (t == 0) (value ? p.c.vs : p.c.ks)[blk] = s;
+#pragma unroll
+    for (int u = 0; u < NU; u += 2) {
+      float x[2][8];
+      unpack8(w[u], x[0]);
+      unpack8(w[u + 1], x[1]);
+      const v2u a = block_codes<E4M3>(x[0], s, inv, finite), c = block_codes<E4M3>(x[1], s, inv, finite);
+      *reinterpret_cast<v4u*>(out + int64_t(t + 128 * u) * 16) = v4u{a[0], a[1], c[0], c[1]};
+    }
+  } else if (whole) {
     uint32_t m2 = 0u;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int i = u * 256 + t, r = i / KCH, d = i % KCH * 8;
-      if (r < lo) continue;
       const v4u w = *reinterpret_cast<const v4u*>(src + (int64_t(b) * BLK + r - n) * rs + d);
       *reinterpret_cast<v4u*>(st + r * LD + d) = w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) m2 = absmax_bf16x2(m2, w[e]);
     }
-    if (lo > 0) {  // (the call's first block alone)
-      const uint16_t* const at = ring + (b & 1) * BLK * D;
-      if (value) {
-        for (int i = t; i < BLK * KCH; i += 256) {  // chunk i of the slot: d, and keys 32 h + 4 qq + ..
-          const int dt = i >> 7, h = (i >> 6) & 1, qq = (i >> 4) & 3, d = 16 * dt + (i & 15);
-          const v4u w = *reinterpret_cast<const v4u*>(at + i * 8);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int r = 32 * h + 16 * (e >> 2) + 4 * qq + (e & 3);
-            const uint16_t x = uint16_t(w[e >> 1] >> (16 * (e & 1)));
-            if (r < lo) {
-              st[r * LD + d] = x;
-              m2 = absmax_bf16x2(m2, x);
-            }
-          }
-        }
-      } else {
-        for (int i = t; i < lo * KCH; i += 256) {
-          const int r = i / KCH, d = i % KCH * 8;
-          const v4u w = *reinterpret_cast<const v4u*>(at + ring_key(r, d, D));
-          *reinterpret_cast<v4u*>(st + r * LD + d) = w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) m2 = absmax_bf16x2(m2, w[e]);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m2 = absmax_bf16x2(m2, __shfl_xor(m2, o, 64));
-    if ((t & 63) == 0) red[t >> 6] = m2;
-    __syncthreads();
-    m2 = absmax_bf16x2(absmax_bf16x2(red[0], red[1]), absmax_bf16x2(red[2], red[3]));
-    const float s = code_scale(absmax_pair(m2), E4M3), inv = 1.0f / s;
+    const float s = code_scale(block_top(m2), E4M3), inv = 1.0f / s;
     const bool finite = quant_finite(s);
-    const int64_t blk = int64_t(g) * p.c.blocks + b;
     if (t == 0) (value ? p.c.vs : p.c.ks)[blk] = s;
-    uint8_t* const out = (value ? p.c.v : p.c.k) + blk * BLK * D;
     for (int i = t; i < BLK * D / 16; i += 256) {  // 16 codes: lane i % 64 of fragment i / 64
       const int f = i >> 6, qi = i & 15, qq = (i >> 4) & 3;
       float x[2][8];
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256) void block_append_kernel(AppendParams p) {
   }
   // The ring.  A later block in the slot of the call's first one is written by that one's workgroup, once it has read
   // the slot.
-  if (b >= bl - 1 && (b == b0 || ((b ^ b0) & 1))) to_ring(b);
+  if (b >= bl - 1 && (b == b0 || ((b ^ b0) & 1)) && !(whole && old)) to_ring(b);
   if (b == b0 && bl - b0 >= 2) {
     const int later = bl - ((bl ^ b0) & 1);  // of bl and bl - 1 the one in b0's slot
     if (later > b0) {
