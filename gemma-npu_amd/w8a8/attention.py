@@ -481,8 +481,9 @@ def block_attention(q, c, n, window=0, sinks=0, scale=1.0, out=None, return_lse=
     run of drafted ones or a prompt's next piece, after cache.append has put their keys and values there.
 
     q: bf16 [H, N, D] ([H, D]: one token), at positions n - N .. n - 1.  The query at position p sees rows j <= p,
-    with a window W those with p - j < W and the first `sinks` rows.  n: an int, or an int32 GPU tensor of one element
-    (the launch then does not depend on it, so a captured step replays at each new length).
+    with a window W those with p - j < W and the first `sinks` rows.  n: the rows that the cache holds, or fewer as
+    cache.append may go back to (a multiple of 64, or a length in the newest two blocks); an int, or an int32 GPU tensor
+    of one element (the launch then does not depend on it, so a captured step replays at each new length).
     Returns o of q's shape (into `out` if given, any strides with a contiguous last dimension), and with return_lse the
     fp32 [H, N] ([H]) logsumexp.  workspace: a device uint8 tensor of at least block_attention_workspace_bytes(...);
     by default one from torch's allocator."""

@@ -223,8 +223,8 @@ def append(c, k, v, n):
 
 
 def read(c, start, n):
-    """(k, v) bf16 [KV, n - start, D]: what rows start .. n - 1 of BlockCache c, which holds n rows, stand for, rounded to
-    bf16 (for attention.attention over what came before, or to put the rows elsewhere)."""
+    """(k, v) bf16 [KV, n - start, D]: what rows start .. n - 1 of BlockCache c, which holds n rows (or more, if n is a multiple
+    of 64 or lies in the newest two blocks), stand for, rounded to bf16 (for attention.attention over what came before, or to put the rows elsewhere)."""
     if not isinstance(c, BlockCache):
         raise TypeError(f"read: expected a BlockCache, got {type(c).__name__}")
     if _native is not None:

@@ -705,7 +705,8 @@ int w8a8_block_read(const void *cache, int64_t KV, int64_t capacity, int64_t D, 
 /* Attention over such a cache of n rows: q bf16 [H, N, D] are the queries at positions n - N .. n - 1; the query at p sees
  * rows j <= p, with a window W > 0 those with p - j < W or j < sinks.  o bf16 [H, N, D], lse fp32 [H, N] or null
  * (natural logarithm).
- *   n: N .. capacity; or -1 and n_dev, an int32 in device memory (brought into that range), which the launch does not depend on
+ *   n: N .. capacity, the rows that the cache holds (or fewer, as w8a8_block_append may go back to); or -1 and n_dev, an
+ *   int32 in device memory (brought into that range), which the launch does not depend on
  *   workspace: w8a8_block_attention_workspace_bytes(...) bytes (-1: invalid; 0: none), 16-byte aligned, scratch;
  *   calls that overlap in time need separate ones
  * strides in elements, multiples of 8; q and o 16-byte aligned.  Sums in fp32 in a fixed order.  One or two launches. */

@@ -60,7 +60,8 @@ def test_native_path(both):
     c = cache.BlockCache(2, 400, 256)
     cache.append(c, k, v, 0)
     both("block_read", lambda: cache.read(c, 17, 390))
-    for n in (6, 390, pos):
+    held = torch.tensor([330], dtype=torch.int32, device=DEV)
+    for n in (64, 390, held):  # (whole blocks, or within the newest two)
         both("block_attention", lambda: attention.block_attention(q, c, n, 64, 4))
         both("block_attention", lambda: attention.block_attention(q[:, 0], c, n))
 
