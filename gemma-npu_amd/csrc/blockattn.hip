@@ -105,6 +105,11 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
   if (part >= geo.np) return;  // (the whole workgroup, before any barrier)
   const int i_lo = int(int64_t(part) * geo.nb / geo.np), i_hi = int(int64_t(part + 1) * geo.nb / geo.np);
   const int whole = geo.n / BLK;  // blocks with codes
+  // Row r of the tile is query `first + t / G` and head t % G of the group, t = odd + r < 2^17: a quotient that fp32 has exactly
+  // (an integer division is some forty instructions, which are waited for one cache line at a time).
+  const int first = tile * R / G, odd = tile * R - first * G;
+  const float per = 1.0f / float(G);
+  auto query = [&](int r) __attribute__((always_inline)) { return int((float(odd + r) + 0.5f) * per); };  // less `first`
   auto block = [&](int i) __attribute__((always_inline)) { return i < geo.sb ? i : i + geo.skip; };
   const bool has_ring = block(i_hi - 1) >= whole;  // the part's last block is the unfinished one
   const int ncode = i_hi - i_lo - (has_ring ? 1 : 0);
@@ -143,10 +148,10 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
   auto ask_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int row = tile * R + staged(i);
+      const int r = staged(i), x = query(r), h = odd + r - x * G;
       qw[i] = v4u{0u, 0u, 0u, 0u};
-      if (row < rows)
-        qw[i] = *reinterpret_cast<const v4u*>(p.q + int64_t(g * G + row % G) * p.qhs + int64_t(row / G) * p.qrs + 8 * (lane % LPR));
+      if (tile * R + r < rows)
+        qw[i] = *reinterpret_cast<const v4u*>(p.q + int64_t(g * G + h) * p.qhs + int64_t(first + x) * p.qrs + 8 * (lane % LPR));
     }
   };
   auto put_q = [&]() __attribute__((always_inline)) {
@@ -165,8 +170,8 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
   int pos[RW];  // of this lane's rows r0 + 16 rt + qi
 #pragma unroll
   for (int rt = 0; rt < RW; ++rt) {
-    const int row = tile * R + r0 + 16 * rt + qi;
-    pos[rt] = row < rows ? geo.n - p.N + row / G : -1;  // (sees nothing)
+    const int r = r0 + 16 * rt + qi;
+    pos[rt] = tile * R + r < rows ? geo.n - p.N + first + query(r) : -1;  // (sees nothing)
   }
   put_q();
   // .. made fp16 in their places (a short loop: what such a kernel waits for first is its own instructions)
@@ -193,8 +198,8 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
   }
   __syncthreads();
   // .. and read as the B operand of k-step 2 j + h: q[64 j + 16 qq + 8 h .. + 7], which is how the codes lie
-  // (where registers are short half of them stay in LDS)
-  constexpr int NQ = 4 * (RW * NKK + NV * RT) > 180 ? NKK / 2 : NKK;
+  // (where registers are short three quarters of them stay in LDS)
+  constexpr int NQ = 4 * (RW * NKK + NV * RT) > 180 ? NKK / 4 : NKK;
   v8h qf[RW][NQ];
   auto frag = [&](int rt, int k) __attribute__((always_inline)) {
     return *reinterpret_cast<const v4u*>(qs + (r0 + 16 * rt + qi) * D + 8 * ((8 * (k >> 1) + 2 * qq + (k & 1)) ^ qi));
@@ -442,8 +447,8 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
             if ((x & 0x7f800000u) != 0x7f800000u) continue;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-              const int row = tile * R + 16 * rt + qi;
-              if (row < rows && seen(b * BLK + key, geo.n - p.N + row / G)) o[j][rt][i] += __uint_as_float(x);
+              const int r = 16 * rt + qi;
+              if (tile * R + r < rows && seen(b * BLK + key, geo.n - p.N + first + query(r))) o[j][rt][i] += __uint_as_float(x);
             }
           }
     }
@@ -472,13 +477,14 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
       continue;
     }
     const float inv = lt > 0.0f ? 1.0f / lt : (lt == lt ? 0.0f : lt);  // (a NaN sum stays one)
-    uint16_t* const op = p.out.o + int64_t(g * G + row % G) * p.out.ohs + int64_t(row / G) * p.out.ors + d;
+    const int x = query(r), h = g * G + odd + r - x * G;
+    uint16_t* const op = p.out.o + int64_t(h) * p.out.ohs + int64_t(first + x) * p.out.ors + d;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       *reinterpret_cast<v2u*>(op + 16 * j) =
           inv != 0.0f ? v2u{pack_bf16x2(o[j][rt][0] * inv, o[j][rt][1] * inv), pack_bf16x2(o[j][rt][2] * inv, o[j][rt][3] * inv)}
                       : v2u{0u, 0u};
-    if (p.out.lse && wave == 0 && qq == 0) p.out.lse[int64_t(g * G + row % G) * p.N + row / G] = part_lse(cqs[r], lt);
+    if (p.out.lse && wave == 0 && qq == 0) p.out.lse[int64_t(h) * p.N + first + x] = part_lse(cqs[r], lt);
   }
 }
 
