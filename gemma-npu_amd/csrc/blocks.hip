@@ -8,7 +8,7 @@
 // block_append_kernel: a workgroup takes a block's keys (or values) of one head.  New rows go into the ring if their block is
 // one of the call's last two.  A block that has become whole is taken from the ring, which lies as the codes do, if some
 // of its rows were there before, else staged in LDS; its largest magnitude is taken on the way.  Memory bounds long calls
-// (65521 rows of 8 heads of 128: 82 us of 79 at a copy's rate), one kernel's start and two round trips short ones.
+// (65521 rows of 8 heads of 128: 86 us of 79 at a copy's rate), one kernel's start and two round trips short ones.
 #include <algorithm>
 
 #include "blocks.h"

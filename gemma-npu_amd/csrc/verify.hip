@@ -17,7 +17,8 @@
 // rows (each workgroup for itself: a few KiB), decides, and sums r over its tokens; the last workgroup of a request
 // to arrive finds the chunk in which the running sum passes its bound, and the token in it.  Exponentials and sums are
 // in 64 bits: of 262144 tokens two neighbours' running sums differ by a few 1e-6 of the whole, and sums of
-// 32-bit terms would draw another token once in some hundred calls.  Every sum has a fixed order.
+// 32-bit terms would draw another token once in some hundred calls.  Every sum has a fixed order.  4 drafted tokens of
+// 262144 (4.7 MB): 6 us and 13; 8 requests of 8 in fp32 (142 MB): 22.7, 17 64-bit operations a logit, and 18.
 #include <algorithm>
 
 #include "w8a8_common.h"

@@ -196,7 +196,7 @@ def append(c, k, v, n):
     n: the rows that are there, an int, or an int32 GPU tensor of one element (the launch then does not depend on it,
     so a captured step replays at each new length).  n may be less than before, as where drafted tokens are taken
     back: rows from n on are written anew.  It has to be a multiple of 64 then, or lie in one of the two newest
-    blocks, whose rows are still there in bf16."""
+    blocks, whose rows are still there in bf16 (not in one before an n that it went back to from further on)."""
     if _native is not None and isinstance(c, BlockCache) and _native.block_append(c.data, c.KV, c.capacity, c.D, c.e4m3, k, v, n):
         return
     if not isinstance(c, BlockCache):
@@ -224,7 +224,8 @@ def append(c, k, v, n):
 
 def read(c, start, n):
     """(k, v) bf16 [KV, n - start, D]: what rows start .. n - 1 of BlockCache c, which holds n rows (or more, if n is a multiple
-    of 64 or lies in the newest two blocks), stand for, rounded to bf16 (for attention.attention over what came before, or to put the rows elsewhere)."""
+    of 64 or lies in the newest two blocks), stand for, rounded to bf16 (for attention.attention over what came before,
+    or to put the rows elsewhere)."""
     if not isinstance(c, BlockCache):
         raise TypeError(f"read: expected a BlockCache, got {type(c).__name__}")
     if _native is not None:
