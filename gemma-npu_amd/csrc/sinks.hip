@@ -10,8 +10,9 @@
 // are those of the sinks, then, without those between, those from its first query's window on to its last query;
 // few tiles split theirs into parts, which a second kernel joins by their logsumexp.  Neighbouring tiles run on one
 // XCD and share its L2's copy of the window.  In a kernel trace 3658 queries of 8 heads of 256,
-// window 512: 47 us (tiles of 64 rows 71); 2048 of 32 heads of 128 on 8, window 4096: 240 us (360), untraced 211 a call, 655
-// TFLOP/s; one token over a window of 1020: 5.8 us and 4 to join.
+// window 512: 40 us (tiles of 64 rows took 71 where those of 128 took 47: edge blocks' values were looked through in LDS then, a
+// barrier more); 2048 of 32 heads of 128 on 8, window 4096: 239 us, untraced 203 a call, 681 TFLOP/s (four waves of 32 rows
+// each 300); one token over a window of 1020: 5.3 us and 4 to join.
 //
 // Within a workgroup the key blocks pass through a two-slot LDS ring (buffer_load ... lds, K one block further ahead than
 // V), one barrier per block: iteration n makes S^T = K Q^T and the softmax of block n + 1 and multiplies P V of block n.
@@ -70,8 +71,8 @@ struct SinkShape {
   static constexpr int PLD = BN + 8;                 // padded P row, elements
   static constexpr int P_SLOT = R * PLD * 2;
   static constexpr int A_OFF = 2 * P_SLOT;           // P [2]; alpha [2][R]
-  static constexpr int F_OFF = A_OFF + 2 * R * 4;    // flags [2][16], found [16]
-  static constexpr int AUX = F_OFF + 3 * 16 * 4;
+  static constexpr int F_OFF = A_OFF + 2 * R * 4;    // flags [2][16]
+  static constexpr int AUX = F_OFF + 2 * 16 * 4;
   static constexpr int NDW = D / NW / 16;            // 16-wide d tiles of O^T per wave
   static constexpr int KR = 3;                       // K fragments in flight
   static constexpr bool SPLIT = D < 512 || RT < 5;   // a variable per slot (the others would spill)
@@ -105,7 +106,6 @@ __global__ __launch_bounds__(sink_waves(RT, D) * 64, 1) void attn_sink_kernel(Si
   else aux = lds + 4 * S::KV_SLOT;
   float* const alpha_s = reinterpret_cast<float*>(aux + S::A_OFF);
   int* const flag_s = reinterpret_cast<int*>(aux + S::F_OFF);
-  int* const found_s = flag_s + 32;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 15, qq = lane >> 4;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(sink_waves(RT, D) * 64, 1) void attn_sink_kernel(Si
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) o[dt][rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const int vsrc = qq * 8 + (qi >> 2);  // this lane's V source row within a 32-key chunk (+4)
-  int found = 0;                        // infinities or NaN were taken out of V (the same for the workgroup)
+  bool found = false;                   // infinities or NaN were taken out of the wave's columns of V
   auto pv_phase = [&](auto slot, int n) __attribute__((always_inline)) {
     int f = 0;
 #pragma unroll
@@ -280,31 +280,9 @@ __global__ __launch_bounds__(sink_waves(RT, D) * 64, 1) void attn_sink_kernel(Si
         for (int dt = 0; dt < NDW; ++dt) o[dt][rt] *= a;
       }
     }
-    char* const vl = v_slot(slot);
+    const char* const vl = v_slot(slot);
     const uint16_t* pl = reinterpret_cast<const uint16_t*>(aux + slot * S::P_SLOT);
-    if (!inner(n)) {
-      // infinities and NaN in the block's V are taken out of the product (0 * inf would be NaN) and added
-      // at the end to the rows that see them
-      int bad = 0;
-#pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        v4u* const at = reinterpret_cast<v4u*>(vl + (u * NT + tid) * 16);
-        v4u w = *at;
-        int b = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, b = 1;
-          if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, b = 1;
-        }
-        if (b) *at = w;
-        bad |= b;
-      }
-      const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-      if (lane == 0) found_s[wave] = any ? 1 : 0;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < NW; ++w) found |= found_s[w];
-    }
+    const bool edge = !inner(n);
 #pragma unroll
     for (int ch = 0; ch < NKC; ++ch) {
       v8bf va[NDW];
@@ -317,6 +295,28 @@ __global__ __launch_bounds__(sink_waves(RT, D) * 64, 1) void attn_sink_kernel(Si
         const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(
             vl + r1 * ROW + (((d >> 3) ^ (2 * (r1 & 3))) * 16) + (d & 7) * 2));
         va[dt] = __builtin_bit_cast(v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+      if (edge) {
+        // infinities and NaN in the block's V are taken out of the product (0 * inf would be NaN) and added
+        // at the end to the rows that see them
+        uint32_t bad = 0u;
+        auto odd = [](uint32_t w) __attribute__((always_inline)) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+#pragma unroll
+        for (int dt = 0; dt < NDW; ++dt) {
+          const v4u w = __builtin_bit_cast(v4u, va[dt]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad |= odd(w[e]);
+        }
+        if (__builtin_amdgcn_ballot_w64(bad != 0u) != 0) {
+          found = true;
+#pragma unroll
+          for (int dt = 0; dt < NDW; ++dt) {
+            v4u w = __builtin_bit_cast(v4u, va[dt]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] &= ~((odd(w[e]) >> 15) * 0xffffu);
+            va[dt] = __builtin_bit_cast(v8bf, w);
+          }
+        }
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
