@@ -7,14 +7,18 @@
 // Row j is code x scale of its block, or the bf16 row of the ring for the n % 64 rows behind the last whole block.
 //
 // A key's scale leaves its product with q as a factor of the score.  A value's scale t enters the softmax weight as
-// an exponent: P'_j = exp2(s_j + log2 t - ms), with ms trailing the maximum of s_j + log2 t by at most 8, so that what
-// contributes most has the most bits, and sum_j exp2(s_j - ms) = sum P'_j / t is added up in fp32 beside it.  Codes
-// become fp16 exactly (|code| <= 127, e4m3 lies within fp16), so both products are fp16 MFMAs summed in fp32.  The
-// roundings: P' to fp16 (2^-11, subnormal below 2^-14: 2^-25 of a weight of 1), and q, scaled by a power of two that
-// brings its row's largest value to 2^10 (exact but for values below 2^-27 of that).  The rows of the ring go
-// through bf16 MFMAs with P' in bf16 (2^-9).
+// an exponent: P'_j = exp2(s_j + log2 t - ms), and sum_j exp2(s_j - ms) = sum P'_j / t is added up in fp32 beside it.
+// ms lies 7 below a value that trails the maximum of s_j + log2 t by at most 8: P' is at most 2^15, and what contributes
+// most has the most bits.  Codes become fp16 exactly (|code| <= 127, e4m3 lies within fp16), so both products are fp16
+// MFMAs summed in fp32.  The roundings: P' to fp16 (2^-11, subnormal below 2^-14: 2^-32 of the row's largest), and q,
+// scaled by a power of two that brings its row's largest value to 2^10 (exact but for values below 2^-27 of that).  The
+// rows of the ring go through bf16 MFMAs with P' in bf16 (2^-8).
 //
-// Blocks' value scales may differ by 2^90: a smaller one's keys then leave fp32 beside a larger one's.
+// A block whose value scale is far below the largest so far, by more than 2^8, would have its P' among fp16's
+// subnormals, and one value far out in a block leaves its other columns to such blocks alone.  So ms is lowered for it, by
+// what its scale lies below the largest, 2^46 at most, or to 7 below its own maximum if that is higher; sums and outputs are
+// rescaled in fp32, as where the maximum grows.  (Of 2^30 rows the sums stay below 2^(30 + 15 + 36 + 46), the outputs far
+// below.)  Scales further apart than 2^46 cost the smaller one's weights a bit for every factor of two.
 //
 // Work split.  The rows (query, head) of one KV head, N G of them, are cut into tiles of 16 RT rows and their visible
 // blocks into parts; a workgroup takes a tile and a part, and a second kernel joins the parts by their logsumexp.  In each
@@ -24,7 +28,7 @@
 //
 // One token of 8 KV heads of 128 over 65521 rows (134 MB of codes): 31 us, 4.8 TB/s once the blocks flow.  One of a head of 512
 // over 3659 rows: 7.7 us, of which the queries' way into registers is 3, a block and its products 2.  5 queries of 8 heads of
-// 512 over 32749 rows: 19.7 us.  509 queries of 8 heads of 256 over a window of 4096 (17 GFLOP): 46 us, 2.2 a block of 64 rows, whose
+// 512 over 32749 rows: 19.7 us.  509 queries of 8 heads of 256 over a window of 4096 (17 GFLOP): 47 us, 2.2 a block of 64 rows, whose
 // S, softmax and P V follow one another in the two waves of a SIMD.
 #include <algorithm>
 #include <type_traits>
@@ -219,9 +223,10 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
     cq[rt] = cqs[r0 + 16 * rt + qi];
   }
 
-  float ms[RW], l[RW];
+  // A row's exponent that its weights and sums are held against, the largest score's that it follows, and its sum.
+  float ms[RW], mt[RW], l[RW];
 #pragma unroll
-  for (int rt = 0; rt < RW; ++rt) ms[rt] = -__builtin_inff(), l[rt] = 0.0f;
+  for (int rt = 0; rt < RW; ++rt) ms[rt] = mt[rt] = -__builtin_inff(), l[rt] = 0.0f;
   v4f o[NV][RT];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -230,6 +235,7 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
 
   v4f s[RW];
   float tb = 0.0f, tinv = 1.0f;  // log2 of the block's value scale, and one over the scale
+  float tmax = -__builtin_inff(), low = 0.0f;  // the largest so far, and how far below it this one lies, if it is far
   const uint32_t near = win > 0 ? uint32_t(win) : 0x80000000u;
   auto seen = [&](int key, int at) __attribute__((always_inline)) {  // (compares alone: a branch here is one per score)
     return (uint32_t(at - key) < near) | ((key <= at) & (key < sinks));
@@ -262,6 +268,8 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
     const float ks = ksr[u], vs = vsr[u];
     tb = __builtin_amdgcn_logf(vs);
     tinv = 1.0f / vs;
+    low = tmax - tb > 8.0f ? fminf(tmax - tb, 46.0f) : 0.0f;  // (a block that reads NaN has no part in this)
+    tmax = tb < __builtin_inff() ? fmaxf(tmax, tb) : tmax;
     constexpr int NS = RW == 1 ? 2 : 1;  // one row tile: two chains of products
     v4f acc[NS][RW];
 #pragma unroll
@@ -293,11 +301,12 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
     for (int rt = 0; rt < RW; ++rt) {
       const int r = r0 + 16 * rt + qi;
       const float m = fmaxf(fmaxf(smax[slot][0][r], smax[slot][1][r]), fmaxf(smax[slot][2][r], smax[slot][3][r]));
-      const bool grow = m > ms[rt] + 8.0f;  // false while every key so far is masked
-      const bool had = ms[rt] != -__builtin_inff();
-      const float alpha = !grow ? 1.0f : (had ? __builtin_amdgcn_exp2f(ms[rt] - m) : 0.0f);
-      grew |= grow && had;
-      ms[rt] = grow ? m : ms[rt];
+      mt[rt] = m > mt[rt] + 8.0f ? m : mt[rt];  // (-inf while every key so far is masked)
+      const float to = __builtin_amdgcn_fmed3f(mt[rt] - 7.0f - low, m - 7.0f, mt[rt] - 7.0f);
+      const bool moved = to != ms[rt], had = ms[rt] != -__builtin_inff();
+      const float alpha = !moved ? 1.0f : (had ? __builtin_amdgcn_exp2f(ms[rt] - to) : 0.0f);
+      grew |= moved && had;
+      ms[rt] = to;
       const float ref = ms[rt] == -__builtin_inff() ? 0.0f : ms[rt];
       float sum = 0.0f;
       uint16_t w[4];
@@ -402,6 +411,7 @@ __global__ __launch_bounds__(256 * block_groups(RT), block_groups(RT) * block_oc
     }
     tb = 0.0f;
     tinv = 1.0f;
+    low = 0.0f;  // (weights in bf16, whose range is that of fp32)
     finish_s(slot, b, 1.0f, false);  // (rows from `live` on lie behind every position)
     // values of rows that aren't there are zero, infinities and NaN (0 x inf) leave the product and are added below to
     // the rows that see them
