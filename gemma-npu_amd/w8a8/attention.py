@@ -482,17 +482,19 @@ def block_attention(q, c, n, window=0, sinks=0, scale=1.0, out=None, return_lse=
 
     q: bf16 [H, N, D] ([H, D]: one token), at positions n - N .. n - 1.  The query at position p sees rows j <= p,
     with a window W those with p - j < W and the first `sinks` rows.  n: the rows that the cache holds, or fewer as
-    cache.append may go back to (a multiple of 64, or a length in the newest two blocks); an int, or an int32 GPU tensor
-    of one element (the launch then does not depend on it, so a captured step replays at each new length).
+    cache.append may go back to (a multiple of 64, or a length in one of the two blocks whose rows are held in bf16; another
+    int is refused); an int, or an int32 GPU tensor of one element (the launch then does not depend on it, so a captured
+    step replays at each new length).
     Returns o of q's shape (into `out` if given, any strides with a contiguous last dimension), and with return_lse the
     fp32 [H, N] ([H]) logsumexp.  workspace: a device uint8 tensor of at least block_attention_workspace_bytes(...);
     by default one from torch's allocator."""
-    if _native is not None and out is None and workspace is None and not return_lse and isinstance(c, BlockCache):
+    if not isinstance(c, BlockCache):
+        raise TypeError(f"block_attention: expected a BlockCache, got {type(c).__name__}")
+    lost = c._lost(n)
+    if lost is None and _native is not None and out is None and workspace is None and not return_lse:
         o = _native.block_attention(q, c.data, c.KV, c.capacity, c.D, c.e4m3, n, window, sinks, scale)
         if o is not None:
             return o
-    if not isinstance(c, BlockCache):
-        raise TypeError(f"block_attention: expected a BlockCache, got {type(c).__name__}")
     one = isinstance(q, torch.Tensor) and q.dim() == 2
     if one:
         q, out = q[:, None], out[:, None] if isinstance(out, torch.Tensor) and out.dim() == 2 else out
@@ -507,6 +509,8 @@ def block_attention(q, c, n, window=0, sinks=0, scale=1.0, out=None, return_lse=
         dev, n = n, -1
     elif not N <= int(n) <= c.capacity:
         raise ValueError(f"block_attention: {N} queries of {n} rows in a cache of {c.capacity}")
+    elif lost is not None:
+        raise ValueError(f"block_attention: {lost}")
     if out is None:
         out = torch.empty((H, N, D), dtype=torch.bfloat16, device=q.device)
     else:

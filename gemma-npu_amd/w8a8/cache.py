@@ -15,6 +15,8 @@ import torch
 from ._lib import Rows, call_on, lib
 from .ops import _native, _stream
 
+BLOCK = 64  # rows of a BlockCache that share a scale
+
 
 def _runs(t, dim, name):
     """The tensor as w8a8_rows: dims before `dim` as one, those behind it as runs of contiguous bytes."""
@@ -166,9 +168,14 @@ class BlockCache:
     head, for keys and for values: max |x| / 127 (times 1 / 448), as the engine quantises activations.  The rows of the block
     that is not whole yet stay bf16, so what it holds depends on the rows alone, not on how they were appended.  Holds
     half a bf16 cache's bytes; attention.block_attention attends to it.  `data` is opaque (the order in which the
-    matrix instructions take the codes)."""
+    matrix instructions take the codes).
 
-    __slots__ = ("data", "KV", "capacity", "D", "dtype")
+    bf16 rows are held of two blocks: of the even and of the odd ones that which append() last put rows into, as one of
+    its last two blocks.  A length that append(), read() or block_attention() is given has to be a multiple of 64 or lie
+    in one of these.  Lengths given as ints are checked against the ints given before; once a length came from device
+    memory, or an append was captured into a graph, nothing is known on the host and nothing is checked."""
+
+    __slots__ = ("data", "KV", "capacity", "D", "dtype", "_ring", "_made")
 
     def __init__(self, KV, capacity, D, dtype=torch.int8, device="cuda"):
         if dtype not in (torch.int8, torch.float8_e4m3fn):
@@ -177,9 +184,12 @@ class BlockCache:
         if n < 0:
             raise ValueError(f"BlockCache: invalid shape KV={KV} capacity={capacity} D={D} (D: 128, 256, 512)")
         self.KV, self.capacity, self.D, self.dtype = int(KV), int(capacity), int(D), dtype
-        self.data = torch.empty(n, dtype=torch.uint8, device=device)
+        with torch.inference_mode(False):  # (a tensor that counts what torch writes to it)
+            self.data = torch.empty(n, dtype=torch.uint8, device=device)
         if self.data.device.type != "cuda":
             raise ValueError(f"BlockCache: expected a GPU, got device {device}")
+        # the even and the odd block whose rows are held (None: unknown), data's version at that time, whether this is kept
+        self._ring, self._made = [None, None, self.data._version, True], self.data
 
     @property
     def device(self):
@@ -189,18 +199,56 @@ class BlockCache:
     def e4m3(self):
         return 1 if self.dtype == torch.float8_e4m3fn else 0
 
+    def _lost(self, n):
+        """Why there are no n rows, or None: the bf16 rows of n's block have made way for another's."""
+        if type(n) is not int:
+            if isinstance(n, torch.Tensor):
+                return None
+            n = int(n)
+        b, r = n // BLOCK, self._ring
+        if n % BLOCK == 0 or r[b & 1] is None or r[b & 1] == b or not self._known():
+            return None
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            return None
+        return (f"{n} rows: those of block {b} ({BLOCK * b} ..) are not held in bf16 any more, block {r[b & 1]}'s came in "
+                f"their place; a multiple of {BLOCK} is possible")
+
+    def _appended(self, n, m):
+        """m rows were appended to n."""
+        r = self._ring
+        if not r[3]:
+            return
+        if torch.cuda.is_current_stream_capturing() or (type(n) is not int and isinstance(n, torch.Tensor)):
+            r[3] = False
+            return
+        if not self._known():
+            r[0] = r[1] = None
+            r[2] = self.data._version if self.data is self._made else -1
+        first, last = int(n) // BLOCK, (int(n) + m - 1) // BLOCK
+        r[last & 1] = last
+        if first < last:
+            r[last - 1 & 1] = last - 1
+
+    def _known(self):
+        """Whether the ring is what the calls made it: `data` is the tensor it was, and torch has written nothing to it (as
+        where one cache is copied over another)."""
+        return self._ring[3] and self.data is self._made and self._ring[2] == self.data._version
+
 
 def append(c, k, v, n):
     """Rows n .. n + m - 1 of BlockCache c: k / v bf16 [KV, m, D] (any strides with a contiguous last dimension).
 
     n: the rows that are there, an int, or an int32 GPU tensor of one element (the launch then does not depend on it,
     so a captured step replays at each new length).  n may be less than before, as where drafted tokens are taken
-    back: rows from n on are written anew.  It has to be a multiple of 64 then, or lie in one of the two newest
-    blocks, whose rows are still there in bf16 (not in one before an n that it went back to from further on)."""
-    if _native is not None and isinstance(c, BlockCache) and _native.block_append(c.data, c.KV, c.capacity, c.D, c.e4m3, k, v, n):
-        return
+    back: rows from n on are written anew.  It has to be a multiple of 64 then, or lie in one of the two blocks whose
+    rows are held in bf16 (BlockCache): in the newest two, as long as it did not go back from further on before.  After 600
+    rows and 10 put to 128, for instance, 100 is refused: of the odd blocks the ring holds the rows from 576 on."""
     if not isinstance(c, BlockCache):
         raise TypeError(f"append: expected a BlockCache, got {type(c).__name__}")
+    lost = c._lost(n)
+    if lost is None and _native is not None and _native.block_append(c.data, c.KV, c.capacity, c.D, c.e4m3, k, v, n):
+        c._appended(n, k.shape[1])
+        return
     for t, name in ((k, "k"), (v, "v")):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device != c.device:
             raise TypeError(f"append: {name} must be a bf16 tensor on {c.device}")
@@ -217,24 +265,30 @@ def append(c, k, v, n):
         raise ValueError(f"append: {m} rows from {n} on in a cache of {c.capacity}")
     if m == 0:
         return
+    if lost is not None:
+        raise ValueError(f"append: {lost}")
     call_on(k, "w8a8_block_append", c.data.data_ptr(), c.KV, c.capacity, c.D, c.e4m3, k.data_ptr(), k.stride(0) if c.KV > 1 else 0,
             k.stride(1) if m > 1 else c.D, v.data_ptr(), v.stride(0) if c.KV > 1 else 0, v.stride(1) if m > 1 else c.D, m, int(n),
             None if dev is None else dev.data_ptr(), _stream(k))
+    c._appended(n if dev is None else dev, m)
 
 
 def read(c, start, n):
-    """(k, v) bf16 [KV, n - start, D]: what rows start .. n - 1 of BlockCache c, which holds n rows (or more, if n is a multiple
-    of 64 or lies in the newest two blocks), stand for, rounded to bf16 (for attention.attention over what came before,
+    """(k, v) bf16 [KV, n - start, D]: what rows start .. n - 1 of BlockCache c, which holds n rows (or more, if n is one of the
+    lengths that append() may go back to), stand for, rounded to bf16 (for attention.attention over what came before,
     or to put the rows elsewhere)."""
     if not isinstance(c, BlockCache):
         raise TypeError(f"read: expected a BlockCache, got {type(c).__name__}")
-    if _native is not None:
+    lost = c._lost(n)
+    if lost is None and _native is not None:
         r = _native.block_read(c.data, c.KV, c.capacity, c.D, c.e4m3, start, n)
         if r is not None:
             return r
     start, n = int(start), int(n)
     if not 0 <= start <= n <= c.capacity:
         raise ValueError(f"read: rows {start} .. {n} of a cache of {c.capacity}")
+    if lost is not None and n > start:
+        raise ValueError(f"read: {lost}")
     k = torch.empty((c.KV, n - start, c.D), dtype=torch.bfloat16, device=c.device)
     v = torch.empty_like(k)
     if n > start:

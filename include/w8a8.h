@@ -690,11 +690,14 @@ int w8a8_verify_drafts(const void *logits, const void *draft, int logits_are_f32
  *   cache: w8a8_block_cache_bytes(KV, capacity, D) bytes (-1: invalid), 16-byte aligned; needs no initialisation
  * w8a8_block_append writes rows n .. n + m - 1 (k / v bf16 [KV, m, D], strides in elements, multiples of 8; 16-byte
  * aligned): rows 0 .. n - 1 were written before, and n may be less than what the cache held (drafted tokens taken
- * back) if n is a multiple of 64 or its block one of the newest two; rows from n + m on are gone then.  n: 0 ..
+ * back); rows from n + m on are gone then.  bf16 rows are held of two blocks: of the even and of the odd ones that which a
+ * call last put rows into as one of its last two blocks.  n has to be a multiple of 64 or lie in one of these: in the
+ * newest two, as long as the cache did not go back before.  (600 rows, then 10 put to 128: 128 .. 138 are possible, 100 is
+ * not, of the odd blocks rows 576 .. are held.)  Nothing checks this: another n reads the other block's rows.  n: 0 ..
  * capacity - m, or -1 and n_dev, an int32 in device memory (brought into that range), which the launch does not
  * depend on.  One launch.
- * w8a8_block_read writes what rows start .. n - 1 of a cache of n rows stand for, rounded to bf16, to k / v [KV, n - start,
- * D] (contiguous). */
+ * w8a8_block_read writes what rows start .. n - 1 of a cache of n rows (a length that append may go back to) stand for,
+ * rounded to bf16, to k / v [KV, n - start, D] (contiguous). */
 int64_t w8a8_block_cache_bytes(int64_t KV, int64_t capacity, int64_t D);
 int w8a8_block_append(void *cache, int64_t KV, int64_t capacity, int64_t D, int e4m3, const uint16_t *k, int64_t k_head_stride,
                       int64_t k_row_stride, const uint16_t *v, int64_t v_head_stride, int64_t v_row_stride, int64_t m,
