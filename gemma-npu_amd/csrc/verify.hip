@@ -522,10 +522,12 @@ static int64_t verify_tiles(int64_t rows, int64_t V) {
   return std::max((tiles + 127) / 128, std::min<int64_t>(8, rows * tiles / 1500));
 }
 static int64_t verify_stats(int64_t rows, int64_t V) { return verify_chunks(V, VERIFY_STAT * std::max<int64_t>(1, verify_tiles(rows, V))); }
+// Workgroups of a launch: 2^32 threads are too many.
+constexpr int64_t VERIFY_BLOCKS = (int64_t(1) << 24) - 1;
 static bool verify_shape_ok(int64_t B, int64_t N, int64_t V) {
   return B >= 1 && N >= 0 && N <= VERIFY_MAX_NODES && V >= 1 && V < (int64_t(1) << 30) &&
          B <= (int64_t(1) << 22) && B * (2 * N + 1) * verify_chunks(V, VERIFY_STAT) < (int64_t(1) << 31) &&
-         B * verify_chunks(V, VERIFY_DRAW) < (int64_t(1) << 31);
+         B * (N + 1) * verify_stats(B * (N + 1), V) <= VERIFY_BLOCKS && B * verify_chunks(V, VERIFY_DRAW) <= VERIFY_BLOCKS;
 }
 
 static int64_t verify_sums_at(int64_t B, int64_t N, int64_t V) { return B * (2 * N + 1) * verify_stats(B * (N + 1), V) * int64_t(sizeof(VerifyStat)); }
@@ -549,6 +551,9 @@ extern "C" int w8a8_verify_drafts(const void* logits, const void* draft, int log
   if (!(temperature > 0.0) || temperature == __builtin_inf() || 1.0 / temperature == __builtin_inf())
     return fail(W8A8_EINVAL, "%s: the temperature must be positive", what);
   if (draft && parents) return fail(W8A8_ENOTSUP, "%s: a tree is verified without draft logits", what);
+  const int64_t rows = B * (N + 1 + (draft ? N : 0));
+  if (rows * verify_stats(B * (N + 1), V) > VERIFY_BLOCKS)
+    return fail(W8A8_EINVAL, "%s: B=%lld N=%lld V=%lld with draft logits", what, (long long)B, (long long)N, (long long)V);
   if (!logits || !uniforms || !accepted || !next || (N > 0 && (!tokens || !path)))
     return fail(W8A8_EINVAL, "%s: null pointer", what);
   if ((N > 0 && row_stride < V) || (B > 1 && group_stride < 0) || (draft && N > 1 && draft_row_stride < V) ||
@@ -575,8 +580,7 @@ extern "C" int w8a8_verify_drafts(const void* logits, const void* draft, int log
   p.sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + verify_sums_at(B, N, V));
   p.arrived = reinterpret_cast<int*>(p.sums + B * p.ndr);
   p.count = accepted; p.path = path; p.next = next;
-  const unsigned rows = unsigned(B * (N + 1 + (p.d ? N : 0)));
-  const dim3 g1{rows * unsigned(p.nst), 1, 1}, g2{unsigned(B) * unsigned(p.ndr), 1, 1};
+  const dim3 g1{unsigned(rows * p.nst), 1, 1}, g2{unsigned(B) * unsigned(p.ndr), 1, 1};
   if (logits_are_f32) {
     verify_stat_kernel<float><<<g1, 256, 0, stream>>>(p);
     verify_draw_kernel<float><<<g2, 256, 0, stream>>>(p);

@@ -673,7 +673,8 @@ int w8a8_beam_select(const void *logits, int logits_are_f32, int64_t group_strid
  *   accepted int32 [B], path int64 [B, N]: the accepted nodes, then -1; next int64 [B], contiguous
  * -inf logits are tokens that cannot follow; a row with a NaN or +inf, or of -inf alone, accepts nothing, and next is -1
  * if it is the row reached.  A token outside the vocabulary is refused.  Exponentials and sums in 64 bits, in a fixed
- * order.  N <= 128, V < 2^30; strides in elements, rows contiguous.
+ * order.  N <= 128, V < 2^30; a launch takes fewer than 2^24 workgroups, one or more for each of the B (N + 1) rows (B (2 N + 1)
+ * with draft logits) and for each 2048 logits of a request's row.  Strides in elements, rows contiguous.
  *   workspace: w8a8_verify_drafts_workspace_bytes(...) bytes (-1: invalid), 8-byte aligned, scratch
  * Two launches. */
 int64_t w8a8_verify_drafts_workspace_bytes(int64_t B, int64_t N, int64_t V);
