@@ -9,7 +9,7 @@
 // tested one after the other, u[m] (1 - s) < p(t_m) with s the probability of the tokens refused beside it, which
 // have none left.  The next token is the first whose running sum of r passes u[N] times the sum of all, with r = p of
 // the row reached, less q of the chain's refused node where that is less (max(p - q, 0)), or without the refused
-// siblings' tokens.  Accepted tokens and the next one are then distributed as the target's own samples.  The
+// siblings' tokens; where that leaves nothing, p.  Accepted tokens and the next one are then distributed as the target's own samples.  The
 // reference decodes greedily, one token at a time (gemma_npu.py:292-295).
 //
 // verify_stat_kernel reads every row once: a workgroup takes 4096 logits of one row into registers and leaves
@@ -28,6 +28,11 @@ namespace w8a8 {
 constexpr int VERIFY_MAX_NODES = 128;
 constexpr int VERIFY_STAT_E = 16, VERIFY_STAT = 256 * VERIFY_STAT_E;  // logits of a thread, of a workgroup: statistics
 constexpr int VERIFY_DRAW_E = 8, VERIFY_DRAW = 256 * VERIFY_DRAW_E;   // and the draw
+
+// A difference p - q of less than this share of p is what rounding left of two equal ones: exponentials are off by 4e-14, a
+// row's and those that join its chunks, and sums by some 1e-14, and a row that begins elsewhere in its 16-byte words is cut
+// into other chunks.
+constexpr double VERIFY_NONE = 0x1p-40;
 
 constexpr int VERIFY_LINE = 32;                   // a request's arrival count has a cache line of its own
 
@@ -423,7 +428,10 @@ __global__ __launch_bounds__(256, 5) void verify_draw_kernel(VerifyParams p) {
     for (int e = 0; e < VERIFY_DRAW_E; ++e) {
       const v2f w = sh.x[PAD * t + e];
       double a = exp_64((double(w[0]) - top) * p.inv_t) * inv;
-      if (q && !plain) a -= exp_64((double(w[1]) - qtop) * p.inv_t) * qinv;
+      if (q && !plain) {
+        const double less = a - exp_64((double(w[1]) - qtop) * p.inv_t) * qinv;
+        a = less > a * VERIFY_NONE ? less : 0.0;
+      }
       a = a > 0.0 && !((out >> e) & 1u) ? a : 0.0;  // (false for NaN)
       sh.r[PAD * t + e] = a;
       sum += a;

@@ -669,6 +669,7 @@ int w8a8_beam_select(const void *logits, int logits_are_f32, int64_t group_strid
  *   tokens refused beside it, a token refused before having none.
  * next: the first token whose running sum of r passes u[N] times the sum of r: r = p of the row reached, less q of the
  * refused node where that is less (else 0), or 0 for the tokens refused without draft logits; p itself if that leaves nothing.
+ * (A difference of at most 2^-40 of p is a rounding's, and none.)
  *   tokens int64 [B, N], uniforms fp32 [B, N + 1] in [0, 1), lengths int32 [B] or null: a request's nodes (brought into 0 .. N)
  *   accepted int32 [B], path int64 [B, N]: the accepted nodes, then -1; next int64 [B], contiguous
  * -inf logits are tokens that cannot follow; a row with a NaN or +inf, or of -inf alone, accepts nothing, and next is -1
