@@ -12,13 +12,15 @@
 // siblings' tokens; where that leaves nothing, p.  Accepted tokens and the next one are then distributed as the target's own samples.  The
 // reference decodes greedily, one token at a time (gemma_npu.py:292-295).
 //
-// verify_stat_kernel reads every row once: a workgroup takes 4096 logits of one row into registers and leaves
-// their sum of exponentials.  verify_draw_kernel, 2048 tokens a workgroup, joins those of the call's
+// verify_stat_kernel reads every row once: a workgroup takes tiles of 4096 logits of one row into registers, one or a few
+// (verify_tiles), and leaves their sum of exponentials.  verify_draw_kernel, 2048 tokens a workgroup, joins those of the call's
 // rows (each workgroup for itself: a few KiB), decides, and sums r over its tokens; the last workgroup of a request
 // to arrive finds the chunk in which the running sum passes its bound, and the token in it.  Exponentials and sums are
 // in 64 bits: of 262144 tokens two neighbours' running sums differ by a few 1e-6 of the whole, and sums of
 // 32-bit terms would draw another token once in some hundred calls.  Every sum has a fixed order.  4 drafted tokens of
-// 262144 (4.7 MB): 6 us and 13; 8 requests of 8 in fp32 (142 MB): 22.7, 17 64-bit operations a logit, and 18.
+// 262144 (9 rows, 4.7 MB): 6 us and 13; a tree of 48 (49 rows, 26 MB): 16.4 and 19.5; 8 requests of up to 8, 4 on average, in
+// fp32 (72 rows, 75 MB): 23 and 19.  The statistics take 1.2-1.3 ps a logit, where their 17 64-bit operations are issued in
+// 0.58: a workgroup's tiles are few, and it begins with a load, a maximum over all of it and a barrier.
 #include <algorithm>
 
 #include "w8a8_common.h"
@@ -29,7 +31,7 @@ constexpr int VERIFY_MAX_NODES = 128;
 constexpr int VERIFY_STAT_E = 16, VERIFY_STAT = 256 * VERIFY_STAT_E;  // logits of a thread, of a workgroup: statistics
 constexpr int VERIFY_DRAW_E = 8, VERIFY_DRAW = 256 * VERIFY_DRAW_E;   // and the draw
 
-// A difference p - q of less than this share of p is what rounding left of two equal ones: exponentials are off by 4e-14, a
+// A difference p - q of less than this share of p is what rounding left of two equal ones: exponentials are off by 6e-14, a
 // row's and those that join its chunks, and sums by some 1e-14, and a row that begins elsewhere in its 16-byte words is cut
 // into other chunks.
 constexpr double VERIFY_NONE = 0x1p-40;
@@ -523,8 +525,8 @@ using namespace w8a8;
 // Chunks of a row, which begins up to 7 elements behind a whole 16-byte word.
 static int64_t verify_chunks(int64_t V, int64_t chunk) { return (V + 7 + chunk - 1) / chunk; }
 // Tiles of 4096 logits in a chunk of the statistics: as many as leave six workgroups for every CU (the fewer chunks, the
-// fewer each workgroup of the draw joins; tree of 48 of 262144, 5 tiles a chunk for 1: draw 23 -> 19 us, statistics 16.6 both),
-// and a row at most 128 chunks.
+// fewer each workgroup of the draw joins; tree of 48 of 262144, 2 tiles a chunk for 1: draw 23.0 -> 19.5 us, statistics
+// 16.8 -> 16.4), and a row at most 128 chunks.
 static int64_t verify_tiles(int64_t rows, int64_t V) {
   const int64_t tiles = verify_chunks(V, VERIFY_STAT);
   return std::max((tiles + 127) / 128, std::min<int64_t>(8, rows * tiles / 1500));
