@@ -10,9 +10,10 @@
 // an exponent: P'_j = exp2(s_j + log2 t - ms), and sum_j exp2(s_j - ms) = sum P'_j / t is added up in fp32 beside it.
 // ms lies 7 below a value that trails the maximum of s_j + log2 t by at most 8: P' is at most 2^15, and what contributes
 // most has the most bits.  Codes become fp16 exactly (|code| <= 127, e4m3 lies within fp16), so both products are fp16
-// MFMAs summed in fp32.  The roundings: P' to fp16 (2^-11, subnormal below 2^-14: 2^-32 of the row's largest), and q,
-// scaled by a power of two that brings its row's largest value to 2^10 (exact but for values below 2^-27 of that).  The
-// rows of the ring go through bf16 MFMAs with P' in bf16 (2^-8).
+// MFMAs summed in fp32.  The roundings: P' to fp16 (2^-11; subnormal below 2^-14, off by 2^-32 of the row's largest, where
+// the codes of the largest's block are off by 2^-8 of that block's values), and q, scaled by a power of two that brings its
+// row's largest value to 2^10 (exact but for values below 2^-27 of that).  The rows of the ring go through bf16 MFMAs
+// with P' in bf16 (2^-8).
 //
 // A block whose value scale is far below the largest so far, by more than 2^8, would have its P' among fp16's
 // subnormals, and one value far out in a block leaves its other columns to such blocks alone.  So ms is lowered for it, by
